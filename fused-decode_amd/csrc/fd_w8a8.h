@@ -1,0 +1,119 @@
+// Products of E4M3 activations and E4M3 weights, shared by the kernels for few and for
+// many activation rows:
+//
+//   v[m,n] = x_scale[m] * w_scale[n] * sum_k x[m,k] * w[n,k] + bias[n]
+//   y[m,n] = round(act(v[m,n]) + row_add[m,n])
+//   FD_ACT_SWIGLU, w [2I,K]: y[m,j] = round(silu(v[m,j]) * v[m,I+j] + row_add[m,j])
+//
+// Products of two codes are exact in float32, sums, scales, the activation and row_add are
+// float32, and the output is rounded once.
+//
+// v_mfma_f32_16x16x128_f8f6f4 takes 128 k a step: lane L holds 32 codes of row L % 16 of
+// either operand. Any k order that both share gives the same sum; here lane group g = L / 16
+// takes bytes 16 g and 64 + 16 g of the step's 128, so that the 16-byte reads of a group
+// and of the four groups together run along a row. Weights are the A operand: a lane's four
+// sums are weight rows 4 g + r of one activation row L % 16.
+#pragma once
+
+#include "fd_device.h"
+#include "fd_gemv.h"
+#include "fd_host.h"
+
+namespace fd {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kStep = 128;  // k of one MFMA step
+
+// acc += A B over one step; no block scales (both scale operands 0 select the plain form).
+__device__ __forceinline__ f32x4 mfma_e4m3(const u32x4& a0, const u32x4& a1, const u32x4& b0, const u32x4& b1,
+                                           f32x4 c) {
+  const i32x8 a = {(int)a0[0], (int)a0[1], (int)a0[2], (int)a0[3], (int)a1[0], (int)a1[1], (int)a1[2], (int)a1[3]};
+  const i32x8 b = {(int)b0[0], (int)b0[1], (int)b0[2], (int)b0[3], (int)b1[0], (int)b1[1], (int)b1[2], (int)b1[3]};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+}
+
+// One 16-byte-per-lane DMA into LDS at byte address `lds` (wave-uniform; lane L lands at
+// 16 L). The s_nop is the wait state a load that reads m0 needs after the write of m0. (m0
+// is a reserved register, which the compiler warns of; the clobber still keeps it from
+// reusing a value of its own across the asm.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+template <bool NT>
+__device__ __forceinline__ void dma16(const void* src, unsigned lds) {
+  if constexpr (NT)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds), "v"(src)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// This wave's LDS operations are done, then the workgroup's barrier; nothing moves across.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// What a product's epilogue reads beside its sums.
+struct W8Epi {
+  const float *xs, *ws;
+  const void* bias;
+  int bias_dtype;
+  int64_t sb;
+  int act;  // FD_ACT_*, not FD_ACT_SWIGLU, which is a kernel's form
+  const void* row;
+  int row_dtype;
+  int64_t srm, srn;
+};
+
+// GELU through erfc, which keeps its relative accuracy where 1 + erf cancels.
+__device__ __forceinline__ float activate(float v, int act) {
+  switch (act) {
+    case FD_ACT_RELU: return v < 0.f ? 0.f : v;
+    case FD_ACT_SILU: return silu_stable(v);
+    case FD_ACT_GELU: return 0.5f * v * erfcf(v * -0.70710678118654752f);
+    case FD_ACT_GELU_TANH: {  // 0.5 (1 + tanh(u)) = sigmoid(2 u)
+      const float u = 1.5957691216057308f * (v + 0.044715f * v * v * v), e = __expf(-fabsf(u));
+      return v * (u >= 0.f ? 1.f / (1.f + e) : e / (1.f + e));
+    }
+    default: return v;
+  }
+}
+
+__device__ __forceinline__ float w8_bias(const W8Epi& e, int64_t n) {
+  return e.bias ? load_any(e.bias, e.bias_dtype, n * e.sb) : 0.f;
+}
+
+// One output from its sum (SWIGLU: and the up row's, weight row n + half).
+template <bool SWIGLU>
+__device__ __forceinline__ float w8_out(const W8Epi& e, float acc, float up, int64_t m, int64_t n, int64_t half) {
+  const float xs = e.xs[m];
+  float v = acc * xs * e.ws[n] + w8_bias(e, n);
+  if constexpr (SWIGLU)
+    v = silu_stable(v) * (up * xs * e.ws[n + half] + w8_bias(e, n + half));
+  else
+    v = activate(v, e.act);
+  if (e.row) v += load_any(e.row, e.row_dtype, m * e.srm + n * e.srn);
+  return v;
+}
+
+// A checked product, as the launchers take it.
+struct W8Args {
+  void* y;
+  const uint8_t *x, *w;
+  int M, N, K;  // N: rows of w
+  int64_t sxm, swn, sym, syn;
+  bool swiglu;
+  W8Epi e;
+  float* scratch;
+  int64_t scratch_bytes;
+  int act_dtype;
+  hipStream_t st;
+};
+
+// Few rows (w8a8_few.hip): whether a product fits, and its launch.
+bool w8_few_fits(const W8Args& a);
+int w8_few_launch(const W8Args& a);
+
+}  // namespace fd

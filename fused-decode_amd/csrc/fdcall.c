@@ -120,6 +120,16 @@ static int (*p_pre_attn_qkv_fp8)(void*, void*, const void*, const void*, int, co
                                  const float*, const void*, int, const void*, const void*, int,
                                  int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, float, int,
                                  void*);
+static int (*p_quantize_rows_fp8)(void*, float*, const void*, const fd_rows*, int, void*);
+static int (*p_rms_norm_fp8)(void*, float*, const void*, const void*, int, int64_t, const fd_rows*,
+                             float, int, void*);
+static int (*p_add_rms_norm_fp8)(void*, float*, void*, const void*, const void*, const void*, int,
+                                 int64_t, const fd_rows*, const fd_rows*, const fd_rows*, float,
+                                 int, void*);
+static int (*p_linear_w8a8)(void*, const void*, const float*, const void*, const float*,
+                            const void*, int, int, const void*, int, int64_t, int64_t, int64_t,
+                            int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, float*,
+                            int64_t, int, void*);
 static int (*p_copy)(void*, const void*, int64_t, void*);
 static int (*p_triad)(void*, const void*, const void*, float, int64_t, int, void*);
 static int (*p_read)(const void*, int64_t, int, void*, void*);
@@ -189,6 +199,20 @@ WRAP(pre_attn_qkv_fp8, "ppppipppippillllllfis",
      p_pre_attn_qkv_fp8(a[0].p, a[1].p, a[2].p, a[3].p, a[4].i, a[5].p, (const float*)a[6].p,
                         a[7].p, a[8].i, a[9].p, a[10].p, a[11].i, a[12].l, a[13].l, a[14].l,
                         a[15].l, a[16].l, a[17].l, a[18].f, a[19].i, a[20].p))
+WRAP(quantize_rows_fp8, "pppris",
+     p_quantize_rows_fp8(a[0].p, (float*)a[1].p, a[2].p, (const fd_rows*)a[3].p, a[4].i, a[5].p))
+WRAP(rms_norm_fp8, "ppppilrfis",
+     p_rms_norm_fp8(a[0].p, (float*)a[1].p, a[2].p, a[3].p, a[4].i, a[5].l, (const fd_rows*)a[6].p,
+                    a[7].f, a[8].i, a[9].p))
+WRAP(add_rms_norm_fp8, "ppppppilrrrfis",
+     p_add_rms_norm_fp8(a[0].p, (float*)a[1].p, a[2].p, a[3].p, a[4].p, a[5].p, a[6].i, a[7].l,
+                        (const fd_rows*)a[8].p, (const fd_rows*)a[9].p, (const fd_rows*)a[10].p,
+                        a[11].f, a[12].i, a[13].p))
+WRAP(linear_w8a8, "ppppppiipillllllllllplis",
+     p_linear_w8a8(a[0].p, a[1].p, (const float*)a[2].p, a[3].p, (const float*)a[4].p, a[5].p,
+                   a[6].i, a[7].i, a[8].p, a[9].i, a[10].l, a[11].l, a[12].l, a[13].l, a[14].l,
+                   a[15].l, a[16].l, a[17].l, a[18].l, a[19].l, (float*)a[20].p, a[21].l, a[22].i,
+                   a[23].p))
 WRAP(copy, "ppls", p_copy(a[0].p, a[1].p, a[2].l, a[3].p))
 WRAP(triad, "pppflis", p_triad(a[0].p, a[1].p, a[2].p, a[3].f, a[4].l, a[5].i, a[6].p))
 WRAP(read, "plips", p_read(a[0].p, a[1].l, a[2].i, a[3].p, a[4].p))
@@ -243,6 +267,10 @@ static PyObject* w_bind(PyObject* self, PyObject* arg) {
   RESOLVE(p_gate_up_fp8_wide, "fd_gate_up_fp8_wide");
   RESOLVE(p_post_attn_mlp_fp8, "fd_post_attn_mlp_fp8");
   RESOLVE(p_pre_attn_qkv_fp8, "fd_pre_attn_qkv_fp8");
+  RESOLVE(p_quantize_rows_fp8, "fd_quantize_rows_fp8");
+  RESOLVE(p_rms_norm_fp8, "fd_rms_norm_fp8");
+  RESOLVE(p_add_rms_norm_fp8, "fd_add_rms_norm_fp8");
+  RESOLVE(p_linear_w8a8, "fd_linear_w8a8");
   RESOLVE(p_copy, "fd_copy");
   RESOLVE(p_triad, "fd_triad");
   RESOLVE(p_read, "fd_read");
@@ -270,6 +298,10 @@ static PyMethodDef methods[] = {
     FAST(gate_up_fp8_wide),
     FAST(post_attn_mlp_fp8),
     FAST(pre_attn_qkv_fp8),
+    FAST(quantize_rows_fp8),
+    FAST(rms_norm_fp8),
+    FAST(add_rms_norm_fp8),
+    FAST(linear_w8a8),
     FAST(copy),
     FAST(triad),
     FAST(read),

@@ -385,6 +385,109 @@ def _cols_of(weight: str) -> Callable[[dict], int]:
     return lambda a: a[weight].shape[1]
 
 
+# ------------------------------------------------------ 8-bit activations (w8a8.py)
+
+
+def has_rows(name: str) -> Rule:
+    """At least one dimension: the last one is the row."""
+
+    def rule(a: dict) -> None:
+        if a[name].ndim == 0:
+            raise ValueError(f"{name} needs at least one dimension")
+
+    return rule
+
+
+def codes_out(name: str, ref: str) -> Rule:
+    """Optional contiguous E4M3 output of ``ref``'s shape."""
+
+    def rule(a: dict) -> None:
+        t, r = a[name], a[ref]
+        if t is None:
+            return
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+        if t.dtype != FP8:
+            raise TypeError(f"{name} must be torch.float8_e4m3fn, got {t.dtype}")
+        if t.device != r.device or t.shape != r.shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {tuple(r.shape)} tensor on {r.device}, got shape "
+                             f"{tuple(t.shape)} strides {t.stride()} on {t.device}")
+
+    return rule
+
+
+def scale_of_rows(name: str, ref: str, *, optional: bool = False) -> Rule:
+    """float32 scales, one a row of ``ref`` (its shape without the last dimension); as an output
+    (``optional``) contiguous."""
+
+    def rule(a: dict) -> None:
+        t, r = a[name], a[ref]
+        if t is None and optional:
+            return
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+        if t.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32, got {t.dtype}")
+        if t.device != r.device or t.shape != r.shape[:-1] or (optional and not t.is_contiguous()):
+            raise ValueError(f"{name} must hold one scale a row of {ref}, shape {tuple(r.shape[:-1])} on {r.device}, "
+                             f"got shape {tuple(t.shape)} strides {t.stride()} on {t.device}")
+
+    return rule
+
+
+ACTIVATIONS = (None, "relu", "silu", "gelu", "gelu_tanh", "swiglu")
+
+
+def activation_name(name: str, weight: str) -> Rule:
+    """An epilogue activation; "swiglu" takes gate rows above up rows of ``weight``."""
+
+    def rule(a: dict) -> None:
+        v = a[name]
+        if not (v is None or isinstance(v, str)) or v not in ACTIVATIONS:
+            raise ValueError(f"{name} must be None or one of {', '.join(map(repr, ACTIVATIONS[1:]))}, got {v!r}")
+        if v == "swiglu" and a[weight].shape[0] % 2:
+            raise ValueError(f"{name} 'swiglu' needs gate and up rows: {weight} has {a[weight].shape[0]}, must be even")
+
+    return rule
+
+
+def bias_of(name: str, ref: str, weight: str) -> Rule:
+    """Optional ``[N]`` bias of any float dtype."""
+
+    def rule(a: dict) -> None:
+        b = a[name]
+        if b is None:
+            return
+        if not isinstance(b, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor or None, got {type(b).__name__}")
+        if b.ndim != 1 or b.shape[0] != a[weight].shape[0]:
+            raise ValueError(f"{name} must have shape ({a[weight].shape[0]},), got {tuple(b.shape)}")
+        if b.device != a[ref].device:
+            raise ValueError(f"{name} must be on {ref}'s device {a[ref].device}, got {b.device}")
+        if b.dtype not in FLOAT:
+            raise TypeError(f"{name} must be {_names(FLOAT)}, got {b.dtype}")
+
+    return rule
+
+
+def output_dtype(name: str, out: str) -> Rule:
+    """The output's dtype: ``out``'s where that is given, else bfloat16 by default."""
+
+    def rule(a: dict) -> None:
+        d, o = a[name], a[out]
+        if o is not None and not isinstance(o, torch.Tensor):
+            raise TypeError(f"{out} must be a tensor or None, got {type(o).__name__}")
+        if d is None:
+            d = torch.bfloat16 if o is None else o.dtype
+        if d not in ACTIVATION:
+            raise TypeError(f"{name} must be {_names(ACTIVATION)}, got {d}")
+        if o is not None and o.dtype != d:
+            raise TypeError(f"{out} is {o.dtype}, {name} is {d}")
+        a[name] = d
+
+    return rule
+
+
 # ------------------------------------------------------------------ contract
 
 CONTRACT: dict[str, tuple[Rule, ...]] = {
@@ -415,6 +518,20 @@ CONTRACT: dict[str, tuple[Rule, ...]] = {
                          bias_for("bias", "hidden", "w_qkv")),
 }
 
+
+CONTRACT.update({
+    "quantize_rows_fp8": (tensor_on_gpu("x"), has_rows("x"), codes_out("out", "x"),
+                          scale_of_rows("scale_out", "x", optional=True)),
+    "rms_norm_fp8": (tensor_on_gpu("x"), has_rows("x"), vector_for("weight", "x"), finite_eps(), codes_out("out", "x"),
+                     scale_of_rows("scale_out", "x", optional=True)),
+    "add_rms_norm_fp8": (tensor_on_gpu("x"), has_rows("x"), tensor_on_gpu("residual"), like("residual", "x"),
+                         vector_for("weight", "x"), finite_eps(), codes_out("out", "x"),
+                         scale_of_rows("scale_out", "x", optional=True), output_like("residual_out", "x")),
+    "linear_w8a8": (tensor_on_gpu("x", (FP8,)), has_rows("x"), scale_of_rows("x_scale", "x"),
+                    weight_matrix("weight", "x", fp8=True), inner_dim("x", "weight"), row_scales("scale", "weight"),
+                    activation_name("activation", "weight"), bias_of("bias", "x", "weight"),
+                    row_add_for("row_add", "x", "weight"), output_dtype("dtype", "out")),
+})
 
 
 def dot_kind_if(*sums: str, name: str = "kind") -> Rule:

@@ -26,6 +26,8 @@ FD_KIND_DOT, FD_KIND_SIMT = 0, 1
 FD_OK, FD_EINVAL, FD_EUNSUPPORTED, FD_ELAUNCH = 0, 1, 2, 3
 
 DTYPE_CODE = {torch.float16: FD_F16, torch.bfloat16: FD_BF16, torch.float32: FD_F32}
+# activations of fd_linear_w8a8's epilogue
+ACT_CODE = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "swiglu": 5}
 KIND_CODE = {"dot": FD_KIND_DOT, "simt": FD_KIND_SIMT}
 
 
@@ -93,6 +95,11 @@ SIGNATURES: dict[str, list] = {
     "fd_post_attn_mlp_fp8_sumsq": [_p, _p, _p, _p, _i, _p, _p, _p, _p, _l, _l, _l, _f, _i, _p, _l, _p, _p],
     "fd_pre_attn_qkv_fp8_sumsq": [_p, _p, _p, _i, _p, _p, _p, _i, _p, _p, _i, _l, _l, _l, _l, _l, _l, _f, _i,
                                   _p, _l, _p],
+    "fd_quantize_rows_fp8": [_p, _p, _p, _rows, _i, _p],
+    "fd_rms_norm_fp8": [_p, _p, _p, _p, _i, _l, _rows, _f, _i, _p],
+    "fd_add_rms_norm_fp8": [_p, _p, _p, _p, _p, _p, _i, _l, _rows, _rows, _rows, _f, _i, _p],
+    "fd_linear_w8a8": [_p, _p, _p, _p, _p, _p, _i, _i, _p, _i, _l, _l, _l, _l, _l, _l, _l, _l, _l, _l, _p, _l, _i, _p],
+    "fd_linear_w8a8_scratch": [_l, _l, _l, ctypes.POINTER(_l)],
     "fd_copy": [_p, _p, _l, _p],
     "fd_copy_persistent": [_p, _p, _l, _i, _p],
     "fd_clock_probe": [_p, _i, ctypes.POINTER(ctypes.c_int), _p],

@@ -10,9 +10,13 @@
     torch.ops.fused_decode.linear_decode_fp8(x, weight, scale, bias, row_add)
     torch.ops.fused_decode.post_attn_mlp_fp8(hidden, norm_weight, w_gate_up, gate_up_scale, w_down, down_scale, eps)
     torch.ops.fused_decode.pre_attn_qkv_fp8(hidden, norm_weight, w_qkv, scale, cos, sin, eps, rope_cols, bias)
+    torch.ops.fused_decode.quantize_rows_fp8(x) -> (codes, scale)
+    torch.ops.fused_decode.rms_norm_fp8(x, weight, eps) -> (codes, scale)
+    torch.ops.fused_decode.add_rms_norm_fp8(x, residual, weight, eps) -> (codes, scale, residual_out)
+    torch.ops.fused_decode.linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add, dtype)
 
 Each is the functional form (no ``out=``) of the operator of the same name in
-``fused_decode.ops``, registered as a custom op with a fake (meta) kernel, so
+``fused_decode.ops``, ``fp8`` or ``w8a8``, registered as a custom op with a fake (meta) kernel, so
 ``torch.compile``, ``torch.export`` and AOT tracing keep the HIP launch as one
 opaque node: the Python argument checks run once per call at run time, and
 graph breaks do not happen around the operators. The reference names this as a
@@ -28,7 +32,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from . import fp8, ops
+from . import fp8, ops, w8a8
 
 _NS = "fused_decode"
 
@@ -146,5 +150,60 @@ def _pre_attn_qkv_fp8_fake(hidden, norm_weight, w_qkv, scale, cos, sin, eps, rop
     return hidden.new_empty((*_lead(hidden), w_qkv.shape[0]))
 
 
+# The implementations run their plans directly: the public w8a8 functions come here when a call is
+# recorded or transformed.
+
+
+@torch.library.custom_op(f"{_NS}::quantize_rows_fp8", mutates_args=())
+def quantize_rows_fp8(x: Tensor) -> tuple[Tensor, Tensor]:
+    return w8a8._plan_rows_fp8("quantize_rows_fp8", x, None, None, 0.0, None, None, None)(x, None, None, None, None, None)
+
+
+def _row_codes(x):
+    return x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+@quantize_rows_fp8.register_fake
+def _quantize_rows_fp8_fake(x):
+    return _row_codes(x)
+
+
+@torch.library.custom_op(f"{_NS}::rms_norm_fp8", mutates_args=())
+def rms_norm_fp8(x: Tensor, weight: Tensor, eps: float = 1e-6) -> tuple[Tensor, Tensor]:
+    return w8a8._plan_rows_fp8("rms_norm_fp8", x, weight, None, eps, None, None, None)(x, weight, None, None, None, None)
+
+
+@rms_norm_fp8.register_fake
+def _rms_norm_fp8_fake(x, weight, eps=1e-6):
+    return _row_codes(x)
+
+
+@torch.library.custom_op(f"{_NS}::add_rms_norm_fp8", mutates_args=())
+def add_rms_norm_fp8(x: Tensor, residual: Tensor, weight: Tensor,
+                     eps: float = 1e-6) -> tuple[Tensor, Tensor, Tensor]:
+    return w8a8._plan_rows_fp8("add_rms_norm_fp8", x, weight, residual, eps, None, None, None)(x, weight, residual, None,
+                                                                                                None, None)
+
+
+@add_rms_norm_fp8.register_fake
+def _add_rms_norm_fp8_fake(x, residual, weight, eps=1e-6):
+    return (*_row_codes(x), x.new_empty(x.shape))
+
+
+@torch.library.custom_op(f"{_NS}::linear_w8a8", mutates_args=())
+def linear_w8a8(x: Tensor, x_scale: Tensor, weight: Tensor, scale: Tensor, bias: Tensor | None = None,
+                activation: str | None = None, row_add: Tensor | None = None,
+                dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    return w8a8._plan_linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add, None, dtype)(
+        x, x_scale, weight, scale, bias, row_add, None)
+
+
+@linear_w8a8.register_fake
+def _linear_w8a8_fake(x, x_scale, weight, scale, bias=None, activation=None, row_add=None, dtype=torch.bfloat16):
+    n = weight.shape[0] // 2 if activation == "swiglu" else weight.shape[0]
+    return x.new_empty((*_lead(x), n), dtype=dtype)
+
+
 OPS = ("rms_norm", "add_rms_norm", "rope", "swiglu", "linear_decode", "post_attn_mlp", "pre_attn_qkv",
        "linear_decode_fp8", "post_attn_mlp_fp8", "pre_attn_qkv_fp8")
+OPS_W8A8 = ("quantize_rows_fp8", "rms_norm_fp8", "add_rms_norm_fp8", "linear_w8a8")

@@ -1,0 +1,282 @@
+"""Operators with 8-bit (OCP E4M3) activations: rows to codes, and products of codes.
+
+    codes, scale = quantize_rows_fp8(x)                              # [..., K] -> codes, float32 [...]
+    codes, scale = rms_norm_fp8(x, norm_w, eps)
+    codes, scale, stream = add_rms_norm_fp8(x, residual, norm_w, eps)
+    y = linear_w8a8(codes, scale, q, q_scale, bias, activation="gelu", row_add=r)
+
+A row has one float32 scale, ``max|y| / 448`` for the float32 row ``y`` (never below 2^-126, and 1 for
+a row of zeros), and its codes are ``y / scale`` rounded to the nearest E4M3 value; the norms
+quantise their float32 result, which is never rounded to 16 bits in between. A row whose largest
+magnitude is not finite gets a NaN scale and NaN codes. Weights are those of ``quantize_fp8``
+(codes ``[N, K]`` and one scale a row), so that
+
+    y[m, n] = round(act(scale[m] * q_scale[n] * sum_k codes[m, k] q[n, k] + bias[n]) + row_add[m, n])
+
+is computed on the 8-bit matrix cores, with float32 sums and one rounding. A layer's four products
+with everything between them but the attention:
+
+    c, s = rms_norm_fp8(x, attn_norm)
+    qkv  = linear_w8a8(c, s, *w_qkv, bias)
+    c, s = quantize_rows_fp8(attention(qkv))
+    h    = linear_w8a8(c, s, *w_o, row_add=x)
+    c, s = rms_norm_fp8(h, mlp_norm)
+    mid  = linear_w8a8(c, s, *w_gate_up, activation="swiglu")
+    c, s = quantize_rows_fp8(mid)
+    x    = linear_w8a8(c, s, *w_down, row_add=h)
+
+Inference only. Where a gradient, a trace or a transform is asked for, the call goes to the custom op
+of the same name (``torch.ops.fused_decode.*``), which a graph keeps whole and which says that it has
+no gradient. There is no reference counterpart (the reference's activations are fp16/bf16 only).
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd import forward_ad
+
+from . import _lib
+from ._checks import check
+from ._lib import ACT_CODE, DTYPE_CODE, FD_EUNSUPPORTED, FdRows, fail, native
+from ._layout import contiguous_strides, plan_rows
+from .fp8 import FP8_DTYPE
+from .ops import (_PLANS, _as_rows, _check_out, _dispatch_modes, _function_modes, _function_modes_watch, _is_tracing,
+                  _raw_stream, _remember, _row_add_rows, _sig, _transform, _written)
+
+__all__ = ["add_rms_norm_fp8", "linear_w8a8", "quantize_rows_fp8", "rms_norm_fp8"]
+
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else (lambda: -1)
+_grad = torch.is_grad_enabled
+
+
+def _recorded(*tensors) -> bool:
+    """Whether something records or transforms a call on these tensors (None: absent), which a launch
+    on their pointers would be missing from."""
+    if (torch.compiler.is_compiling() or forward_ad._current_level >= 0 or _transform() is not None or _is_tracing()
+            or _dispatch_modes() or (_function_modes() and _function_modes_watch())):
+        return True
+    return _grad() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _on(dev: int, call, *args) -> int:
+    """``call(*args, stream)`` with ``dev`` current: a launch on the default stream goes to the current device."""
+    if _current_device() == dev:
+        return call(*args, _raw_stream(dev))
+    with torch.cuda.device(dev):
+        return call(*args, _raw_stream(dev))
+
+
+# ------------------------------------------------------------------ rows to codes
+
+
+def quantize_rows_fp8(
+    x: torch.Tensor,
+    *,
+    out: torch.Tensor | None = None,
+    scale_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """E4M3 codes of ``x``'s rows (its last dimension) and their float32 scales ``x.shape[:-1]``, in one
+    launch. For finite rows the codes and scales that ``quantize_fp8`` gives the same rows."""
+    return _rows("quantize_rows_fp8", x, None, None, 0.0, out, scale_out, None)
+
+
+def rms_norm_fp8(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    eps: float = 1e-6,
+    *,
+    out: torch.Tensor | None = None,
+    scale_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``rms_norm`` with E4M3 codes and float32 row scales for its result. ``weight`` is ``(N,)``
+    (float16, bfloat16 or float32)."""
+    return _rows("rms_norm_fp8", x, weight, None, eps, out, scale_out, None)
+
+
+def add_rms_norm_fp8(
+    x: torch.Tensor,
+    residual: torch.Tensor,
+    weight: torch.Tensor,
+    eps: float = 1e-6,
+    *,
+    out: torch.Tensor | None = None,
+    scale_out: torch.Tensor | None = None,
+    residual_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``add_rms_norm`` with E4M3 codes and float32 row scales for the norm of the float32 sum:
+    ``(codes, scale, residual_out)``. ``residual_out=residual`` updates the residual stream in place."""
+    return _rows("add_rms_norm_fp8", x, weight, residual, eps, out, scale_out, residual_out)
+
+
+def _rows(op, x, weight, residual, eps, out, scale_out, residual_out):
+    try:
+        if _recorded(x, weight, residual):
+            return _rows_op(op, x, weight, residual, eps, out, scale_out, residual_out)
+        key = (op, x.shape, x.stride(), x.dtype, x.get_device(), _sig(weight), _sig(residual), eps, _sig(out),
+               _sig(scale_out), _sig(residual_out))
+        plan = _PLANS.get(key)
+    except (AttributeError, TypeError):  # a non-tensor or unhashable argument: checked below
+        key, plan = None, None
+    if plan is None:
+        plan = _remember(key, _plan_rows_fp8(op, x, weight, residual, eps, out, scale_out, residual_out))
+    return plan(x, weight, residual, out, scale_out, residual_out)
+
+
+def _rows_op(op, x, weight, residual, eps, out, scale_out, residual_out):
+    """The custom op of the same name, its results copied where outputs are given."""
+    f = getattr(torch.ops.fused_decode, op)
+    got = (f(x) if op == "quantize_rows_fp8" else f(x, weight, eps) if op == "rms_norm_fp8" else
+           f(x, residual, weight, eps))
+    return tuple(v if o is None else o.copy_(v) for v, o in zip(got, (out, scale_out, residual_out)))
+
+
+def _plan_rows_fp8(op, x, weight, residual, eps, out, scale_out, residual_out):
+    """Launch plan of a row operator for one argument signature."""
+    add, norm = residual is not None or op == "add_rms_norm_fp8", op != "quantize_rows_fp8"
+    args = dict(x=x, out=out, scale_out=scale_out)
+    if norm:
+        args.update(weight=weight, eps=eps)
+    if add:
+        args.update(residual=residual, residual_out=residual_out)
+    eps = check(op, **args).get("eps", 0.0)
+    shape, lead, device = tuple(x.shape), tuple(x.shape[:-1]), x.device
+    n, act, dev = shape[-1], DTYPE_CODE[x.dtype], x.device.index
+    dense = contiguous_strides(shape)
+    strides = [tuple(x.stride())]
+    if add:
+        strides += [tuple(residual.stride()), dense if residual_out is None else tuple(residual_out.stride())]
+    # more than three unmergeable leading dims: the rows are gathered, and written back
+    layouts = plan_rows(shape, strides) if n and math.prod(lead) else None
+    staged = layouts is None
+    if staged:
+        layouts = [bytes(FdRows(1, 1, math.prod(lead), 0, 0, n, 1, n))] * len(strides)
+    name = "fd_" + op
+    call = getattr(native(), op)
+    wcode, wstride = (DTYPE_CODE[weight.dtype], int(weight.stride(0)) if n > 1 else 1) if norm else (act, 1)
+
+    def run(x, w, r, out, scale_out, residual_out):
+        c = torch.empty(shape, dtype=FP8_DTYPE, device=device) if out is None else out
+        s = torch.empty(lead, dtype=torch.float32, device=device) if scale_out is None else scale_out
+        if staged:
+            x = x.contiguous()
+        if not add:
+            if norm:
+                status = _on(dev, call, c.data_ptr(), s.data_ptr(), x.data_ptr(), w.data_ptr(), wcode, wstride,
+                             layouts[0], eps, act)
+            else:
+                status = _on(dev, call, c.data_ptr(), s.data_ptr(), x.data_ptr(), layouts[0], act)
+            if status:
+                fail(name, status)
+            return c if out is None else _written(out), s if scale_out is None else _written(scale_out)
+        ro = torch.empty(shape, dtype=x.dtype, device=device) if residual_out is None or staged else residual_out
+        if staged:
+            r = r.contiguous()
+        status = _on(dev, call, c.data_ptr(), s.data_ptr(), ro.data_ptr(), x.data_ptr(), r.data_ptr(), w.data_ptr(),
+                     wcode, wstride, layouts[0], layouts[1], layouts[2], eps, act)
+        if status:
+            fail(name, status)
+        if residual_out is not None:
+            ro = residual_out.copy_(ro) if staged else _written(residual_out)
+        return c if out is None else _written(out), s if scale_out is None else _written(scale_out), ro
+
+    if math.prod(lead) == 0 or n == 0:  # no value to compute: a row of none has scale 1
+        def empty(x, w, r, out, scale_out, residual_out):
+            c = torch.empty(shape, dtype=FP8_DTYPE, device=device) if out is None else out
+            s = torch.ones(lead, dtype=torch.float32, device=device) if scale_out is None else scale_out.fill_(1.0)
+            return (c, s, torch.empty_like(x) if residual_out is None else residual_out) if add else (c, s)
+        return empty
+    return run
+
+
+# ------------------------------------------------------------------ products of codes
+
+
+def linear_w8a8(
+    x: torch.Tensor,
+    x_scale: torch.Tensor,
+    weight: torch.Tensor,
+    scale: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    *,
+    activation: str | None = None,
+    row_add: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """``act(dequantised x @ dequantised weight.T (+ bias)) (+ row_add)`` for E4M3 ``x [..., K]`` with float32
+    ``x_scale [...]`` and E4M3 ``weight [N, K]`` with float32 ``scale [N]``, rounded once to ``dtype`` (float16
+    or bfloat16; ``out``'s where that is given, else bfloat16).
+
+    ``activation`` is None, "relu", "silu", "gelu" (with erf), "gelu_tanh" or "swiglu", which takes gate rows
+    above up rows (``weight [2I, K]``, ``bias [2I]``) and returns ``silu(gate) * up`` ``[..., I]``. ``bias`` and
+    ``row_add`` have any float dtype; ``row_add`` broadcasts to the output and is added after the activation.
+    Any number of rows and any K; rows of codes that are not 16-byte aligned and K that is no multiple of 16
+    take a slower kernel, and codes without unit stride along K are gathered first."""
+    try:
+        if _recorded(x, x_scale, weight, scale, bias, row_add):
+            y = torch.ops.fused_decode.linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add,
+                                                   dtype or (torch.bfloat16 if out is None else out.dtype))
+            return y if out is None else out.copy_(y)
+        key = ("linear_w8a8", x.shape, x.stride(), x.dtype, x.get_device(), _sig(x_scale), _sig(weight), _sig(scale),
+               _sig(bias), activation, _sig(row_add), _sig(out), dtype)
+        plan = _PLANS.get(key)
+    except (AttributeError, TypeError):  # a non-tensor or unhashable argument: checked below
+        key, plan = None, None
+    if plan is None:
+        plan = _remember(key, _plan_linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add, out, dtype))
+    return plan(x, x_scale, weight, scale, bias, row_add, out)
+
+
+def _plan_linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add, out, dtype):
+    """Launch plan of ``linear_w8a8`` for one argument signature."""
+    a = check("linear_w8a8", x=x, x_scale=x_scale, weight=weight, scale=scale, bias=bias, activation=activation,
+              row_add=row_add, out=out, dtype=dtype)
+    dtype, device, dev = a["dtype"], x.device, x.device.index
+    n, k = (int(d) for d in weight.shape)
+    nout = n // 2 if activation == "swiglu" else n
+    m = math.prod(x.shape[:-1])
+    expected = (*x.shape[:-1], nout)
+    ra = None if row_add is None else _row_add_rows(row_add, m, nout, expected)
+    if out is not None:
+        _check_out(out, expected, torch.empty((), dtype=dtype, device=device))
+    if m == 0 or nout == 0:
+        return lambda x, xs, w, ws, b, r, o: torch.empty(expected, dtype=dtype, device=device) if o is None else o
+    xr = _as_rows(x, m)
+    x_copy = xr.flat or (k > 1 and xr.col != 1)
+    w_copy = k > 1 and weight.stride(1) != 1
+    sxm, swn = k if x_copy else xr.row, k if w_copy else int(weight.stride(0))
+    s_copy = not (x_scale.is_contiguous() and scale.is_contiguous())
+    act, code = ACT_CODE[activation], DTYPE_CODE[dtype]
+    bcode, sb = (code, 0) if bias is None else (DTYPE_CODE[bias.dtype], int(bias.stride(0)))
+    rcode = code if row_add is None else DTYPE_CODE[row_add.dtype]
+    srm, srn, r_flat = ra if ra is not None else (0, 0, False)
+    call = native().linear_w8a8
+    with torch.cuda.device(dev):
+        scratch_bytes = _lib.scratch_bytes("fd_linear_w8a8_scratch", m, n, k)
+
+    def run(x, xs, w, ws, b, r, o):
+        y = torch.empty(expected, dtype=dtype, device=device) if o is None else o
+        if x_copy:
+            x = x.reshape(m, k).contiguous()
+        if w_copy:
+            w = w.contiguous()
+        if s_copy:
+            xs, ws = xs.contiguous(), ws.contiguous()
+        if r_flat:
+            r = r.expand(expected).reshape(m, nout)
+        part = torch.empty(scratch_bytes, dtype=torch.uint8, device=device) if scratch_bytes else None
+        args = (x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), None if b is None else b.data_ptr(), bcode, act,
+                None if r is None else r.data_ptr(), rcode, m, n, k, sxm, swn, sb, srm, srn, nout, 1,
+                None if part is None else part.data_ptr(), scratch_bytes, code)
+        status = _on(dev, call, y.data_ptr(), *args)
+        if status == FD_EUNSUPPORTED and o is not None:  # `out` may lie over an operand: write beside it
+            beside = torch.empty(expected, dtype=dtype, device=device)
+            status = _on(dev, call, beside.data_ptr(), *args)
+            if status == 0:
+                return o.copy_(beside)
+        if status:
+            fail("fd_linear_w8a8", status)
+        return y if o is None else _written(o)
+    return run

@@ -42,6 +42,17 @@ enum {
   FD_ELAUNCH = 3      /* the HIP launch itself failed */
 };
 
+/* activations of fd_linear_w8a8's epilogue: GELU is 0.5 v (1 + erf(v / sqrt 2)), GELU_TANH its
+ * tanh approximation, SWIGLU silu(gate) * up over the two halves of the weight's rows */
+enum {
+  FD_ACT_NONE = 0,
+  FD_ACT_RELU = 1,
+  FD_ACT_SILU = 2,
+  FD_ACT_GELU = 3,
+  FD_ACT_GELU_TANH = 4,
+  FD_ACT_SWIGLU = 5
+};
+
 /*
  * A row layout: the tensor is a grid of a*b*c rows of n elements. Row (i,j,l)
  * starts at i*sa + j*sb + l*sc and element t of a row sits at t*col further on.
@@ -417,6 +428,51 @@ int fd_pre_attn_qkv_fp8_sumsq(void* y, const void* hidden, const void* norm_w, i
                               int64_t cs_row_stride, int64_t M, int64_t H, int64_t N,
                               int64_t rope_cols, int64_t head_dim, float eps, int act_dtype,
                               const float* ss_in, int64_t ss_tiles, void* stream);
+
+/*
+ * Rows to OCP E4M3 codes with one float32 scale a row (8-bit activations for
+ * fd_linear_w8a8). With t the row (fd_add_rms_norm_fp8: t = x + residual in float32 and
+ * residual_out = round(t)) and y = t, or t * w * rsqrt(mean(t^2) + eps) in float32 for the
+ * norms:
+ *   scale = max(max|y| / 448, 2^-126) (1 where max|y| is 0), codes = e4m3(y / scale)
+ * y is not rounded to act_dtype before. A row whose max|y| is not finite has a NaN scale and
+ * NaN codes. codes are rows of n bytes, scale one float a row, both dense and in the order
+ * of the row grid; they overlap no input and each other in no byte. residual_out may be x
+ * or residual in the same layout and overlaps them in no other way (else FD_EINVAL).
+ * fd_quantize_rows_fp8's codes are x / scale with the division's own rounding.
+ * No reference counterpart (its activations are fp16/bf16 only).
+ */
+int fd_quantize_rows_fp8(void* codes, float* scale, const void* x, const fd_rows* lx, int act_dtype,
+                         void* stream);
+int fd_rms_norm_fp8(void* codes, float* scale, const void* x, const void* w, int w_dtype,
+                    int64_t w_stride, const fd_rows* lx, float eps, int act_dtype, void* stream);
+int fd_add_rms_norm_fp8(void* codes, float* scale, void* residual_out, const void* x,
+                        const void* residual, const void* w, int w_dtype, int64_t w_stride,
+                        const fd_rows* lx, const fd_rows* lr, const fd_rows* lro, float eps,
+                        int act_dtype, void* stream);
+
+/*
+ * The product of E4M3 activations x8 [M,K] (row stride sxm bytes, one float32 scale a row)
+ * and E4M3 weights w8 [N,K] (row stride swn, one float32 scale a row), any M, N and K:
+ *   v[m,n] = x_scale[m] * w_scale[n] * sum_k x8[m,k] * w8[n,k] + bias[n]
+ *   y[m,n] = round(act(v[m,n]) + row_add[m,n])
+ * With FD_ACT_SWIGLU w8 holds gate rows above up rows (N = 2I) and y is [M,I]:
+ *   y[m,j] = round(silu(v[m,j]) * v[m,I+j] + row_add[m,j])
+ * Sums and the epilogue are float32 with one rounding. bias (N values at stride sb) and
+ * row_add (strides srm, srn; 0 broadcasts) have any of the three dtypes and may be NULL; y has
+ * act_dtype. Rows that are not 16-byte aligned, or K % 16 != 0, take a slower kernel. Few
+ * output tiles split K over workgroups whose float32 sums go through `scratch` (16-byte
+ * aligned, caller-owned, not shared with a call that may overlap) and are added in a fixed
+ * order; fd_linear_w8a8_scratch gives the bytes of the preferred split (0: none), less lowers
+ * it, down to none with scratch NULL. y may be row_add element for element and overlaps no
+ * operand otherwise (FD_EUNSUPPORTED). No reference counterpart.
+ */
+int fd_linear_w8a8(void* y, const void* x8, const float* x_scale, const void* w8,
+                   const float* w_scale, const void* bias, int bias_dtype, int activation,
+                   const void* row_add, int row_dtype, int64_t M, int64_t N, int64_t K, int64_t sxm,
+                   int64_t swn, int64_t sb, int64_t srm, int64_t srn, int64_t sym, int64_t syn,
+                   float* scratch, int64_t scratch_bytes, int act_dtype, void* stream);
+int fd_linear_w8a8_scratch(int64_t M, int64_t N, int64_t K, int64_t* bytes);
 
 /*
  * Bandwidth roofs. dst = src over `bytes` bytes (any size; 16-byte aligned
