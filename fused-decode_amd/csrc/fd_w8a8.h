@@ -33,19 +33,19 @@ __device__ __forceinline__ f32x4 mfma_e4m3(const u32x4& a0, const u32x4& a1, con
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
 }
 
-// One 16-byte-per-lane DMA into LDS at byte address `lds` (wave-uniform; lane L lands at
-// 16 L). The s_nop is the wait state a load that reads m0 needs after the write of m0. (m0
-// is a reserved register, which the compiler warns of; the clobber still keeps it from
+// One 16-byte-per-lane DMA from base + off into LDS at byte address `lds` (wave-uniform; lane L
+// lands at 16 L). The s_nop is the wait state a load that reads m0 needs after the write of
+// m0. (m0 is a reserved register, which the compiler warns of; the clobber still keeps it from
 // reusing a value of its own across the asm.)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 template <bool NT>
-__device__ __forceinline__ void dma16(const void* src, unsigned lds) {
+__device__ __forceinline__ void dma16(const uint8_t* base, unsigned off, unsigned lds) {
   if constexpr (NT)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds), "v"(src)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base)
                  : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
                  : "memory", "m0");
 }
 #pragma clang diagnostic pop
@@ -67,17 +67,29 @@ struct W8Epi {
   int64_t srm, srn;
 };
 
-// GELU through erfc, which keeps its relative accuracy where 1 + erf cancels.
-__device__ __forceinline__ float activate(float v, int act) {
-  switch (act) {
-    case FD_ACT_RELU: return v < 0.f ? 0.f : v;
-    case FD_ACT_SILU: return silu_stable(v);
-    case FD_ACT_GELU: return 0.5f * v * erfcf(v * -0.70710678118654752f);
-    case FD_ACT_GELU_TANH: {  // 0.5 (1 + tanh(u)) = sigmoid(2 u)
-      const float u = 1.5957691216057308f * (v + 0.044715f * v * v * v), e = __expf(-fabsf(u));
-      return v * (u >= 0.f ? 1.f / (1.f + e) : e / (1.f + e));
-    }
-    default: return v;
+// v sigmoid(u), the sigmoid from one reciprocal: exp(-u) past float32's range leaves 0.
+__device__ __forceinline__ float times_sigmoid(float v, float u) {
+  return v * __builtin_amdgcn_rcpf(1.f + __expf(-u));
+}
+
+// Eight values at once, so that the choice is made once. GELU goes through erfc, which keeps its
+// relative accuracy where 1 + erf cancels; 0.5 (1 + tanh(u)) is sigmoid(2 u).
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int act) {
+  if (act == FD_ACT_NONE) return;
+  if (act == FD_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = times_sigmoid(v[i], v[i]);
+  } else if (act == FD_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];
+  } else if (act == FD_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * erfcf(v[i] * -0.70710678118654752f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = times_sigmoid(v[i], 1.5957691216057308f * (v[i] + 0.044715f * v[i] * v[i] * v[i]));
   }
 }
 
@@ -90,10 +102,13 @@ template <bool SWIGLU>
 __device__ __forceinline__ float w8_out(const W8Epi& e, float acc, float up, int64_t m, int64_t n, int64_t half) {
   const float xs = e.xs[m];
   float v = acc * xs * e.ws[n] + w8_bias(e, n);
-  if constexpr (SWIGLU)
-    v = silu_stable(v) * (up * xs * e.ws[n + half] + w8_bias(e, n + half));
-  else
-    v = activate(v, e.act);
+  if constexpr (SWIGLU) {
+    v = times_sigmoid(v, v) * (up * xs * e.ws[n + half] + w8_bias(e, n + half));
+  } else {
+    float one[1] = {v};
+    activate(one, e.act);
+    v = one[0];
+  }
   if (e.row) v += load_any(e.row, e.row_dtype, m * e.srm + n * e.srn);
   return v;
 }

@@ -2,28 +2,81 @@
 // activation rows (fd_w8a8.h has the mathematics).
 //
 // A workgroup of WN x WM waves owns BN weight rows x BM activation rows and walks K in stages
-// of 128. Both tiles of a stage go to LDS, D - 1 stages ahead of the one being multiplied, one
-// barrier a stage: by DMA (global_load_lds_dwordx4) where rows are 16-byte aligned and K % 16
-// == 0, else through registers with 16-byte loads at any address (bytes for the piece that
-// crosses K). The DMAs are inline assembly, so the compiler sees plain LDS reads and schedules
-// and waits for those itself; the vmcnt waits are explicit.
+// of 128. Both tiles of a stage go to LDS in a ring of D stages: by DMA (global_load_lds_dwordx4)
+// where rows are 16-byte aligned and K % 16 == 0, else through registers with 16-byte loads at
+// any address (bytes where a piece crosses K). The DMAs are inline assembly, so the compiler sees
+// plain LDS reads and schedules and waits for those itself; the vmcnt waits are explicit.
+//
+// The matrix cores are fed from registers that hold the whole stage: weight tile n's registers
+// are refilled with the next stage's once row n of the wave's tiles is multiplied, the
+// activations' during the last row. So no MFMA waits for the LDS read in front of it, the LDS
+// reads lie evenly between the MFMAs, a buffer is free for the DMAs of stage s + D as soon as
+// stage s begins, and one barrier a stage is enough. It stands behind the first row's MFMAs,
+// which run on while the waves meet.
 //
 // LDS layout: a tile row is 8 chunks of 16 bytes, chunk c at slot c ^ (row mod 8), so the 8
 // lanes of a read (8 rows, one chunk) hit distinct bank groups and a DMA instruction still fills
-// 1 KiB in lane order. The weight rows of a wave lie in LDS in the order that gives a lane
-// consecutive outputs: lane group g's sums are outputs 4 NT g .. 4 NT g + 4 NT - 1 of the wave
-// (SWIGLU: gate and up rows in turn, so that a lane holds both of an output), and leave in
-// 16-byte pieces along a row without another pass through LDS.
+// 1 KiB in lane order. At the end each wave's sums go through LDS and leave along the rows in
+// 16-byte nontemporal stores. SWIGLU: gate and up tiles of 16 rows in turn, so that a lane finds
+// both of an output.
 //
-// Where the output has fewer tiles than the GPU has CUs, K is split over workgroups whose
+// Where the output has fewer tiles than the GPU has room for, K is split over workgroups whose
 // float32 sums go through scratch and are added in split order by a second launch.
 #include <type_traits>
+#include <utility>
 
 #include "fd_w8a8.h"
 
 namespace fd {
 
 template <int BN, int BM> constexpr int kStageBytes = (BN + BM) * kStep;
+
+// 16-row tiles of a wave's sums that fit the LDS at once.
+template <int NW, int NT, int MT, int kLimit>
+constexpr int epi_tiles() {
+  int em = MT;
+  while (em > 1 && (MT % em != 0 || (size_t)NW * em * 16 * (NT * 16 + 4) * 4 + NW * MT * 64 > (size_t)kLimit)) --em;
+  return em;
+}
+template <int NW, int NT, int MT, int kLimit>
+constexpr size_t epi_bytes() { return (size_t)NW * epi_tiles<NW, NT, MT, kLimit>() * 16 * (NT * 16 + 4) * 4 + NW * MT * 64; }
+
+template <typename F, int... I>
+__device__ __forceinline__ void each_part(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
+// Elements n .. n + 7 of p (at n * stride + shift * stride) in float32: one or two loads where they lie together,
+// the last element again past cols; zeros of no p.
+__device__ __forceinline__ void load8_vec(const void* p, int dtype, int n, int64_t stride, int cols, float (&f)[8],
+                                          int shift = 0) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = 0.f;
+  } else if (stride == 1 && n + 8 <= cols) {
+    const char* q = static_cast<const char*>(p) + (int64_t)(n + shift) * (dtype == FD_F32 ? 4 : 2);
+    const u32x4 lo = *reinterpret_cast<const u32x4_any*>(q);
+    if (dtype == FD_F32) {
+      const u32x4 hi = *reinterpret_cast<const u32x4_any*>(q + 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[i] = __builtin_bit_cast(float, (uint32_t)lo[i]);
+        f[i + 4] = __builtin_bit_cast(float, (uint32_t)hi[i]);
+      }
+    } else if (dtype == FD_F16) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = to_f32(__builtin_bit_cast(f16x8, lo)[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = to_f32(__builtin_bit_cast(bf16x8, lo)[i]);
+    }
+  } else {
+    for (int i = 0; i < 8; ++i) {
+      const int c = n + i < cols ? n + i : cols - 1;
+      f[i] = load_any(p, dtype, (int64_t)(c + shift) * stride);
+    }
+  }
+}
 
 enum W8Form { W8_OUT = 0, W8_PART = 1 };
 
@@ -37,6 +90,10 @@ __device__ __forceinline__ u32x4 load16_any(const uint8_t* row, int k, int K) {
   return v;
 }
 
+// Tiles of a group of row blocks: an XCD's workgroups share the activations of kGroup row blocks
+// and walk the weights (8192 x 28672 x 4096: 4, 8, 16 row blocks 750, 746, 781 us).
+constexpr int kGroup = 8;
+
 template <typename T, int WN, int WM, int NT, int MT, int D, bool SWIGLU, int FORM, bool DMA>
 __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float* part, const uint8_t* x,
                                                                     const uint8_t* w, int M, int N, int K, int64_t sxm,
@@ -46,7 +103,8 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
   constexpr int NW = WN * WM, BN = WN * NT * 16, BM = WM * MT * 16;
   constexpr int AOPS = BN / 8 / NW, BOPS = BM / 8 / NW, OPS = AOPS + BOPS;
   static_assert(AOPS * 8 * NW == BN && BOPS * 8 * NW == BM, "the waves share a stage evenly");
-  static_assert(!SWIGLU || NT % 2 == 0, "gate and up tiles in turn");
+  static_assert(NT > 1 && (!SWIGLU || NT % 2 == 0), "gate and up tiles in turn");
+  static_assert(D >= 2 && (DMA || D == 2), "the register path holds one stage");
   extern __shared__ __align__(16) u32x4 w8_smem[];
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -67,56 +125,86 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
       tile = xcd * q + (xcd < rem ? xcd : rem) + (b >> 3);
     }
   }
-  const int ntile = tile / mtiles, m0 = (tile - ntile * mtiles) * BM;
+  int ntile, mtile;
+  {
+    const int ntiles = (int)gridDim.x / splits / mtiles;
+    const int G = kGroup, per = G * ntiles, gi = tile / per, rem = tile - gi * per;
+    const int gs = mtiles - gi * G < G ? mtiles - gi * G : G;
+    ntile = rem / gs;
+    mtile = gi * G + rem - ntile * gs;
+  }
+  const int m0 = mtile * BM;
   const int half = N / 2, cols = SWIGLU ? half : N;
-  constexpr int OUT = SWIGLU ? BN / 2 : BN, LANE = SWIGLU ? NT * 2 : NT * 4;  // outputs of a tile, of a lane
+  constexpr int OUT = SWIGLU ? BN / 2 : BN, WOUT = OUT / WN;  // output columns of a tile, of a wave
   const int stages_all = (K + kStep - 1) / kStep;
   const int s0 = (int)((int64_t)stages_all * split / splits);
   const int ns = (int)((int64_t)stages_all * (split + 1) / splits) - s0;
 
-  // weight row at LDS row t of the tile (past the last: one that exists, never stored)
+  // weight row at LDS row t of the tile (past the last: one that exists, never stored); SWIGLU:
+  // a wave's 16-row tiles are gate and up rows in turn
   auto wrow = [&](int t) -> int64_t {
-    const int wv = t / (NT * 16), f = t / 16 % NT, i = t & 15;
     if constexpr (SWIGLU) {
-      const int n = ntile * OUT + wv * (NT * 8) + (i >> 2) * LANE + (f >> 1) * 4 + (i & 3);
+      const int f = t / 16, n = ntile * OUT + (f >> 1) * 16 + (t & 15);
       return (n < half ? n : half - 1) + (int64_t)((f & 1) ? half : 0);
     } else {
-      const int n = ntile * OUT + wv * (NT * 16) + (i >> 2) * LANE + f * 4 + (i & 3);
+      const int n = ntile * OUT + t;
       return n < N ? n : N - 1;
     }
   };
 
   const unsigned lds0 = lds_addr(w8_smem);
   constexpr unsigned kStage = (unsigned)kStageBytes<BN, BM>;
-  const uint8_t* src[OPS];
+  // DMA: a scalar base for the tile's weight rows (SWIGLU: and its up rows) and activation rows, and a
+  // 32-bit offset a lane; else pointers
+  const int64_t n_first = (int64_t)ntile * OUT < cols ? (int64_t)ntile * OUT : cols - 1;
+  const uint8_t* const wbase = w + n_first * swn;
+  const uint8_t* const ubase = SWIGLU ? wbase + (int64_t)half * swn : wbase;
+  const uint8_t* const xbase = x + (int64_t)m0 * sxm;
+  const uint8_t* src[DMA ? 1 : OPS];
+  unsigned voff[DMA ? OPS : 1];
   int off[OPS];
 #pragma unroll
   for (int i = 0; i < OPS; ++i) {
     const bool wt = i < AOPS;
     const int t = (wt ? wave * AOPS + i : wave * BOPS + i - AOPS) * 8 + lane / 8;
     const int m = m0 + t;
-    src[i] = wt ? w + wrow(t) * swn : x + (int64_t)(m < M ? m : M - 1) * sxm;
+    const int64_t row = wt ? wrow(t) : (m < M ? m : M - 1);
     off[i] = ((lane & 7) ^ (t & 7)) * 16;
+    if constexpr (DMA)
+      voff[i] = (unsigned)(wt ? (row - n_first - (SWIGLU && ((t >> 4) & 1) ? half : 0)) * swn : (row - m0) * sxm) + off[i];
+    else
+      src[i] = wt ? w + row * swn : x + row * sxm;
   }
   auto place = [&](int i) {  // byte address in a stage of this wave's i-th KiB
     return (unsigned)(i < AOPS ? wave * AOPS + i : BN / 8 + wave * BOPS + i - AOPS) * 1024u;
   };
-  auto issue = [&](int s) {
-    const unsigned base = lds0 + (unsigned)(s % D) * kStage;
-#pragma unroll
-    for (int i = 0; i < OPS; ++i) {
-      const int k = (s0 + s) * kStep + off[i];
-      dma16<false>(src[i] + (k < K ? k : 0), base + place(i));
-    }
+  auto issue_one = [&](int s, int i) {
+    const int k0 = (s0 + s) * kStep;
+    const bool up = SWIGLU && (((wave * AOPS + i) >> 1) & 1);  // 8 rows of an up tile
+    const uint8_t* base = i < AOPS ? (up ? ubase : wbase) : xbase;
+    const unsigned to = lds0 + (unsigned)(s % D) * kStage + place(i), o = voff[DMA ? i : 0];
+    if (k0 + kStep <= K)
+      dma16<false>(base + k0, o, to);
+    else  // pieces past K: the row's start
+      dma16<false>(base, k0 + off[i] < K ? o + (unsigned)k0 : o - (unsigned)off[i], to);
   };
   u32x4 held[DMA ? 1 : OPS];
-  auto fetch = [&](int s) {
+  auto fetch = [&](int s) {  // stage s into registers
+    const int k0 = (s0 + s) * kStep;
 #pragma unroll
-    for (int i = 0; i < OPS; ++i) held[DMA ? 0 : i] = load16_any(src[i], (s0 + s) * kStep + off[i], K);
+    for (int i = 0; i < OPS; ++i) held[DMA ? 0 : i] = load16_any(src[DMA ? 0 : i], k0 + off[i], K);
   };
-  auto put = [&](int s) {
+  auto put = [&](int s) {  // and on into LDS
 #pragma unroll
     for (int i = 0; i < OPS; ++i) w8_smem[((s % D) * kStage + place(i)) / 16 + lane] = held[DMA ? 0 : i];
+  };
+  auto zero_tail = [&](int s) {  // DMA past K brought the row's start: the activations there become zero
+    const int k0 = (s0 + s) * kStep;
+    if (k0 + kStep > K) {
+#pragma unroll
+      for (int i = AOPS; i < OPS; ++i)
+        if (k0 + off[i] >= K) ds_zero16(lds0 + (unsigned)(s % D) * kStage + place(i) + (unsigned)lane * 16u);
+    }
   };
 
   f32x4 acc[NT][MT];
@@ -128,55 +216,89 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
   // this lane's two chunks of a tile row (u32x4 entries): row r of a 16-row tile, r mod 8 is
   // every tile's swizzle
   const int c0 = g ^ (r & 7), c1 = (4 + g) ^ (r & 7);
-  auto multiply = [&](int s) {
-    const u32x4* st = w8_smem + (size_t)(s % D) * (kStage / 16);
-    u32x4 b0[MT], b1[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const u32x4* p = st + BN * 8 + ((wm * MT + m) * 16 + r) * 8;
-      b0[m] = p[c0];
-      b1[m] = p[c1];
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const u32x4* p = st + ((wn * NT + n) * 16 + r) * 8;
-      const u32x4 a0 = p[c0], a1 = p[c1];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) acc[n][m] = mfma_e4m3(a0, a1, b0[m], b1[m], acc[n][m]);
-    }
+  u32x4 a0[NT], a1[NT], b0[MT], b1[MT];
+  auto load_a = [&](int s, int n) {
+    const u32x4* p = w8_smem + (s % D) * (kStage / 16) + ((wn * NT + n) * 16 + r) * 8;
+    a0[n] = p[c0];
+    a1[n] = p[c1];
   };
-
-  if constexpr (DMA) {
-    const int pre = ns < D - 1 ? ns : D - 1;
-    for (int s = 0; s < pre; ++s) issue(s);
-    for (int s = 0; s < ns; ++s) {
-      // stages issued so far end at s + D - 2: D - 2 of them may stay in flight
-      if (s + D - 2 < ns)
+  auto load_b = [&](int s, int m) {
+    const u32x4* p = w8_smem + (s % D) * (kStage / 16) + (BN + (wm * MT + m) * 16 + r) * 8;
+    b0[m] = p[c0];
+    b1[m] = p[c1];
+  };
+  if (ns > 0) {
+    if constexpr (DMA) {
+      const int pre = ns < D ? ns : D;
+      for (int s = 0; s < pre; ++s)
+#pragma unroll
+        for (int i = 0; i < OPS; ++i) issue_one(s, i);
+      if (ns >= D)
+        wait_vm<OPS*(D - 1)>();
+      else
+        wait_vm<0>();
+      zero_tail(0);
+    } else {
+      fetch(0);
+      put(0);
+      if (ns > 1) {
+        fetch(1);
+        put(1);
+      }
+    }
+    lds_barrier();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) load_a(0, n);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) load_b(0, m);
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0), so that the loop's waits count its own reads alone
+  }
+  for (int s = 0; s < ns; ++s) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[0][m] = mfma_e4m3(a0[0], a1[0], b0[m], b1[m], acc[0][m]);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (DMA) {
+      // issued so far: to stage s + D - 1; the next stage has to be there
+      if (s + D <= ns)
         wait_vm<OPS*(D - 2)>();
       else
         wait_vm<0>();
-      if ((s0 + s + 1) * kStep > K) {  // K tail: activations past K are zero
-#pragma unroll
-        for (int i = AOPS; i < OPS; ++i)
-          if ((s0 + s) * kStep + off[i] >= K)
-            ds_zero16(lds0 + (unsigned)(s % D) * kStage + place(i) + (unsigned)lane * 16u);
-      }
-      lds_barrier();  // stage s has landed everywhere; every wave is done with stage s - 1
-      if (s + D - 1 < ns) issue(s + D - 1);
-      multiply(s);
+      if (s + 1 < ns) zero_tail(s + 1);
     }
-  } else {
-    if (ns > 0) fetch(0);
-    for (int s = 0; s < ns; ++s) {
-      put(s);  // D = 2: the other half may still be read
-      lds_barrier();
-      if (s + 1 < ns) fetch(s + 1);
-      multiply(s);
+    lds_barrier();  // stage s is in every wave's registers, stage s + 1 in LDS
+    const bool more = s + D < ns;
+    if constexpr (!DMA) {
+      if (more) fetch(s + 2);
+    }
+    // (past the last stage the registers are refilled with what the ring holds, and not used)
+#pragma unroll
+    for (int n = 1; n < NT; ++n) {
+      load_a(s + 1, n - 1);
+      if constexpr (DMA) {
+        if (more) {
+#pragma unroll
+          for (int i = OPS * (n - 1) / (NT - 1); i < OPS * n / (NT - 1); ++i) issue_one(s + D, i);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        acc[n][m] = mfma_e4m3(a0[n], a1[n], b0[m], b1[m], acc[n][m]);
+        if (n == NT - 1) {
+          __builtin_amdgcn_sched_barrier(0);
+          load_b(s + 1, m);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    load_a(s + 1, NT - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!DMA) {
+      if (more) put(s + 2);
     }
   }
 
-  const int n0 = ntile * OUT + wn * (OUT / WN) + g * LANE;  // this lane's first output column
-  if (n0 >= cols) return;
+  const int n0 = ntile * OUT + wn * WOUT;  // this wave's first output column
   if constexpr (FORM == W8_PART) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -185,7 +307,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
       float* to = part + ((int64_t)split * M + row) * N;
 #pragma unroll
       for (int f = 0; f < NT; ++f) {
-        const int n = n0 + (SWIGLU ? f >> 1 : f) * 4, at = n + (SWIGLU && (f & 1) ? half : 0);
+        const int n = n0 + (SWIGLU ? f >> 1 : f) * 16 + g * 4, at = n + (SWIGLU && (f & 1) ? half : 0);
         if (n + 4 <= cols && N % 4 == 0 && (!SWIGLU || half % 4 == 0)) {
           *reinterpret_cast<f32x4*>(to + at) = acc[f][m];
         } else {
@@ -196,51 +318,105 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
       }
     }
   } else {
-    const bool wide = syn == 1 && sym % 8 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
-    // eight outputs at a time: their scales and bias once for all of this lane's rows
-#pragma unroll
-    for (int q = 0; q < LANE / 8; ++q) {
-      const int n = n0 + q * 8;
-      if (n >= cols) break;
-      float s1[8], b1[8], s2[SWIGLU ? 8 : 1], b2[SWIGLU ? 8 : 1];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int c = n + i < cols ? n + i : cols - 1;
-        s1[i] = e.ws[c];
-        b1[i] = w8_bias(e, c);
-        if constexpr (SWIGLU) {
-          s2[i] = e.ws[half + c];
-          b2[i] = w8_bias(e, (int64_t)half + c);
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int row = m0 + (wm * MT + m) * 16 + r;
-        if (row >= M) continue;
-        const float xs = e.xs[row];
-        V8 o;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float v;
-          if constexpr (SWIGLU) {
-            const int f = (q * 2 + i / 4) * 2;
-            v = silu_stable(acc[f][m][i % 4] * xs * s1[i] + b1[i]) * (acc[f + 1][m][i % 4] * xs * s2[i] + b2[i]);
-          } else {
-            v = activate(acc[q * 2 + i / 4][m][i % 4] * xs * s1[i] + b1[i], e.act);
-          }
-          if (e.row && n + i < cols) v += load_any(e.row, e.row_dtype, row * e.srm + (n + i) * e.srn);
-          o[i] = from_f32<T>(v);
-        }
-        T* to = y + (int64_t)row * sym + n * syn;
-        if (wide && n + 8 <= cols) {
-          store8<T>(to, o);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (n + i < cols) to[i * syn] = o[i];
-        }
-      }
+    // Each wave's sums go through LDS of its own, EM tiles of 16 activation rows at a time, and
+    // leave along the rows: a lane has the same eight output columns of every row it writes.
+    constexpr int EM = epi_tiles<NW, NT, MT, (int)(kStageBytes<BN, BM> * D)>(), PITCH = NT * 16 + 4, TPR = WOUT / 8,
+                  RPP = kWave / TPR, U = EM * 16 >= RPP * 2 ? 2 : 1;
+    static_assert(EM * 16 % (RPP * U) == 0, "whole passes");
+    float* sums = reinterpret_cast<float*>(w8_smem) + wave * (EM * 16 * PITCH);
+    float* xsl = reinterpret_cast<float*>(w8_smem) + NW * (EM * 16 * PITCH) + wave * (MT * 16);
+    const int oc = lane % TPR * 8, n = n0 + oc, rr = lane / TPR;
+    const int sc = SWIGLU ? (oc >> 4) * 32 + (oc & 15) : oc;  // its column of the sums; SWIGLU: up 16 further
+    const int mrow = m0 + wm * MT * 16;
+    float s1[8], b1[8], s2[SWIGLU ? 8 : 1], b2[SWIGLU ? 8 : 1];
+    load8_vec(e.ws, FD_F32, n, 1, cols, s1);
+    load8_vec(e.bias, e.bias_dtype, n, e.sb, cols, b1);
+    if constexpr (SWIGLU) {
+      load8_vec(e.ws + half, FD_F32, n, 1, cols, s2);
+      load8_vec(e.bias, e.bias_dtype, n, e.sb, cols, b2, half);
     }
+    float xv[(MT * 16 + kWave - 1) / kWave];
+#pragma unroll
+    for (int i = 0; i < MT * 16; i += kWave) {
+      const int row = mrow + i + lane;
+      xv[i / kWave] = e.xs[row < M ? row : M - 1];
+    }
+    const bool whole = n + 8 <= cols, wide = whole && syn == 1;
+    const int add_dtype = e.row_dtype, add = !e.row ? 0 : e.srn != 1 ? 3 : add_dtype == FD_F32 ? 2 : 1;
+    lds_barrier();  // the last stage has been read everywhere
+#pragma unroll
+    for (int i = 0; i < MT * 16; i += kWave)
+      if (i + lane < MT * 16) xsl[i + lane] = xv[i / kWave];
+    auto part_of = [&](auto part) {
+      constexpr int h = decltype(part)::value;
+#pragma unroll
+      for (int m = 0; m < EM; ++m)
+#pragma unroll
+        for (int f = 0; f < NT; ++f)
+          *reinterpret_cast<f32x4*>(sums + (m * 16 + r) * PITCH + f * 16 + g * 4) = acc[f][h * EM + m];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 1
+      for (int t0 = rr; t0 < EM * 16; t0 += RPP * U) {
+        u32x4 lo[U], hi[U];
+        if (whole && (add == 1 || add == 2)) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int row = mrow + h * EM * 16 + t0 + u * RPP;
+            const int64_t at = (row < M ? row : M - 1) * e.srm + n;
+            const char* p = static_cast<const char*>(e.row) + at * (add == 2 ? 4 : 2);
+            lo[u] = *reinterpret_cast<const u32x4_any*>(p);
+            if (add == 2) hi[u] = *reinterpret_cast<const u32x4_any*>(p + 16);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int t = t0 + u * RPP, row = mrow + h * EM * 16 + t;
+          const float xs = xsl[h * EM * 16 + t];
+          const float* p = sums + t * PITCH + sc;
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = p[i] * xs * s1[i] + b1[i];
+          if constexpr (SWIGLU) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = times_sigmoid(v[i], v[i]) * (p[16 + i] * xs * s2[i] + b2[i]);
+          } else {
+            activate(v, e.act);
+          }
+          if (row >= M || n >= cols) continue;
+          if (add) {
+            if (!whole || add == 3) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (n + i < cols) v[i] += load_any(e.row, add_dtype, row * e.srm + (n + i) * e.srn);
+            } else if (add == 2) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                v[i] += __builtin_bit_cast(float, (uint32_t)lo[u][i]);
+                v[i + 4] += __builtin_bit_cast(float, (uint32_t)hi[u][i]);
+              }
+            } else if (add_dtype == FD_F16) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] += to_f32(__builtin_bit_cast(f16x8, lo[u])[i]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] += to_f32(__builtin_bit_cast(bf16x8, lo[u])[i]);
+            }
+          }
+          V8 o;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = from_f32<T>(v[i]);
+          T* to = y + (int64_t)row * sym + n * syn;
+          if (wide) {
+            store8_any<T>(to, o);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (n + i < cols) to[i * syn] = o[i];
+          }
+        }
+      }
+    };
+    each_part(part_of, std::make_integer_sequence<int, MT / EM>{});
   }
 }
 
@@ -268,7 +444,9 @@ namespace {
 template <typename T, int WN, int WM, int NT, int MT, int D, bool SWIGLU, int FORM, bool DMA>
 int tile_launch(const W8Args& a, int splits) {
   constexpr int BN = WN * NT * 16, BM = WM * MT * 16;
-  constexpr size_t lds = (size_t)kStageBytes<BN, BM> * D;
+  constexpr size_t ring = (size_t)kStageBytes<BN, BM> * D;
+  constexpr size_t sums = FORM == W8_OUT ? epi_bytes<WN * WM, NT, MT, (int)ring>() : 0;
+  constexpr size_t lds = ring > sums ? ring : sums;
   static_assert(lds <= kMaxLds, "a launch fits the LDS of a CU");
   const int64_t nt = (a.N + BN - 1) / BN, mt = (a.M + BM - 1) / BM;
   if (nt * mt * splits > 0x7fffffffLL) return set_error(FD_EUNSUPPORTED, "too many tiles");
@@ -280,10 +458,25 @@ int tile_launch(const W8Args& a, int splits) {
   return FD_OK;
 }
 
+// Whether tiles of 256 x 256, one to a CU, take less time than tiles of 128 x 128, two to a CU:
+// rounds of workgroups, each of its stages and what its start and its output cost (us, measured).
+bool w8_large(int64_t M, int64_t N, int64_t K) {
+  auto rounds = [&](int64_t b, int64_t slots) {
+    const int64_t tiles = ((M + b - 1) / b) * ((N + b - 1) / b);
+    return (double)((tiles + slots - 1) / slots);
+  };
+  const double stages = (double)((K + kStep - 1) / kStep);
+  const int cus = device_cus();
+  return rounds(256, cus) * (stages * 1.35 + 9) < rounds(128, 2 * cus) * (stages * 0.95 + 6);
+}
+
 template <typename T, bool SWIGLU, int FORM>
 int pick_tile(const W8Args& a, int splits, bool dma) {
   if (!dma) return tile_launch<T, 2, 2, 4, 4, 2, SWIGLU, FORM, false>(a, splits);
-  return tile_launch<T, 2, 2, 4, 4, 3, SWIGLU, FORM, true>(a, splits);
+  if constexpr (FORM == W8_OUT) {
+    if (w8_large(a.M, a.N, a.K)) return tile_launch<T, 4, 2, 4, 8, 2, SWIGLU, FORM, true>(a, 1);
+  }
+  return tile_launch<T, 2, 2, 4, 4, 2, SWIGLU, FORM, true>(a, splits);
 }
 
 template <typename T, bool SWIGLU>
@@ -366,8 +559,9 @@ extern "C" int fd_linear_w8a8(void* y, const void* x8, const float* x_scale, con
   a.scratch_bytes = scratch ? scratch_bytes : 0;
   a.act_dtype = act_dtype;
   a.st = static_cast<hipStream_t>(stream);
+  // the DMAs' 32-bit offsets reach over a tile's rows
   const bool dma = K % 16 == 0 && aligned16(x8) && aligned16(w8) && (M == 1 || sxm % 16 == 0) &&
-                   (N == 1 || swn % 16 == 0);
+                   (N == 1 || swn % 16 == 0) && sxm < (1 << 23) && swn < (1 << 23);
   int splits = w8_splits(M, N, K);
   while (splits > 1 && a.scratch_bytes < (int64_t)splits * M * N * 4) --splits;
   const int rc = act_dtype == FD_F16 ? (swiglu ? tiles<f16, true>(a, splits, dma) : tiles<f16, false>(a, splits, dma))

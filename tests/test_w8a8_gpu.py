@@ -225,6 +225,24 @@ def test_products_of_small_integers_are_exact(m, n, k, dtype):
     assert torch.equal(fd.linear_w8a8(x.flip(0), xs.flip(0), w, ws, dtype=dtype), v.flip(0).to(dtype))
 
 
+@pytest.mark.parametrize("m,n,k,name", [(4000, 8200, 400, None), (4091, 16390, 272, "swiglu"), (4100, 8195, 129, "relu")])
+def test_products_of_large_tiles(m, n, k, name):
+    """Many rows and columns, neither a multiple of a tile, K no multiple of a step."""
+    import fused_decode as fd
+
+    x, xs, w, ws, bias, _, v = exact_case(m, n, k, m, torch.bfloat16)
+    v = v + bias.double()
+    if name == "swiglu":
+        v, xs, bias = v * 2.0**-6, xs * 2.0**-6, bias * 2.0**-6  # sigmoids that are neither 0 nor 1
+        ref = v[:, : n // 2] * torch.sigmoid(v[:, : n // 2]) * v[:, n // 2:]
+        y = fd.linear_w8a8(x, xs, w, ws, bias, activation=name)
+        # exact arguments: the sigmoid's own float32 evaluation (64 steps of 2^-24) and the output's rounding
+        assert bool(((y.double() - ref).abs() <= (2.0**-18 + 2.0**-8) * ref.abs() + 1e-30).all())
+    else:
+        want = v.clamp_min(0) if name == "relu" else v
+        assert torch.equal(fd.linear_w8a8(x, xs, w, ws, bias, activation=name), want.bfloat16())
+
+
 def act64(v, name):
     if name == "relu":
         return v.clamp_min(0)
