@@ -48,7 +48,31 @@ __device__ __forceinline__ void dma16(const uint8_t* base, unsigned off, unsigne
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
                  : "memory", "m0");
 }
+// The same from a pointer a lane, nontemporal.
+__device__ __forceinline__ void dma16_ptr(const uint8_t* src, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds), "v"(src)
+               : "memory", "m0");
+}
 #pragma clang diagnostic pop
+
+// 16 bytes at any address.
+__device__ __forceinline__ u32x4 load16_any(const uint8_t* p) {
+  typedef u32x4 u32x4_b __attribute__((aligned(1)));
+  return *reinterpret_cast<const u32x4_b*>(p);
+}
+// 16 bytes of a row of K >= 16 at k >= 0; zeros past K. One load wherever k is: the piece that crosses K, and one
+// past it, is the row's last 16 bytes moved down.
+__device__ __forceinline__ u32x4 load16_end(const uint8_t* row, int k, int K) {
+  const int at = k + 16 <= K ? k : K - 16, down = k - at;
+  const u32x4 v = load16_any(row + at);
+  uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+  const int s = (down & 7) * 8;
+  const uint64_t up = s ? hi << (64 - s) : 0;
+  const uint64_t lo1 = lo >> s | up, hi1 = hi >> s;
+  lo = down < 8 ? lo1 : down < 16 ? hi1 : 0;
+  hi = down < 8 ? hi1 : 0;
+  return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+}
 
 // This wave's LDS operations are done, then the workgroup's barrier; nothing moves across.
 __device__ __forceinline__ void lds_barrier() {
@@ -72,8 +96,26 @@ __device__ __forceinline__ float times_sigmoid(float v, float u) {
   return v * __builtin_amdgcn_rcpf(1.f + __expf(-u));
 }
 
-// Eight values at once, so that the choice is made once. GELU goes through erfc, which keeps its
-// relative accuracy where 1 + erf cancels; 0.5 (1 + tanh(u)) is sigmoid(2 u).
+// v (1 + erf(v / sqrt 2)) / 2. The lower tail of the normal distribution at -|v| is exp(-v^2 / 2) t P(t) with
+// t = 1 / (1 + |v| / sqrt 8) and P a polynomial fitted to exp(z^2) erfc(z) / (2 t), z = |v| / sqrt 2, with a relative
+// error below 5e-8 for z <= 13 (past that the exponential is 0): relative accuracy on both sides, no branch and few
+// instructions, where erfc's code alone was most of a kernel.
+__device__ __forceinline__ float gelu(float v) {
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.35355339f * fabsf(v));
+  float p = -0.0296934061f;
+  p = p * t + 0.14306283f;
+  p = p * t - 0.24520494f;
+  p = p * t + 0.140868649f;
+  p = p * t - 0.014575636f;
+  p = p * t + 0.10187684f;
+  p = p * t + 0.121417411f;
+  p = p * t + 0.141206071f;
+  p = p * t + 0.141042158f;
+  const float tail = v * (__expf(-0.5f * v * v) * t * p);
+  return v < 0.f ? tail : v - tail;
+}
+
+// Values at once, so that the choice is made once. 0.5 (1 + tanh(u)) is sigmoid(2 u).
 template <int N>
 __device__ __forceinline__ void activate(float (&v)[N], int act) {
   if (act == FD_ACT_NONE) return;
@@ -85,7 +127,7 @@ __device__ __forceinline__ void activate(float (&v)[N], int act) {
     for (int i = 0; i < N; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];
   } else if (act == FD_ACT_GELU) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * erfcf(v[i] * -0.70710678118654752f);
+    for (int i = 0; i < N; ++i) v[i] = gelu(v[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -119,7 +161,7 @@ struct W8Args {
   const uint8_t *x, *w;
   int M, N, K;  // N: rows of w
   int64_t sxm, swn, sym, syn;
-  bool swiglu;
+  bool swiglu, dma;  // dma: 16-byte aligned rows of whole 16-byte pieces
   W8Epi e;
   float* scratch;
   int64_t scratch_bytes;

@@ -31,15 +31,18 @@ namespace fd {
 
 template <int BN, int BM> constexpr int kStageBytes = (BN + BM) * kStep;
 
-// 16-row tiles of a wave's sums that fit the LDS at once.
-template <int NW, int NT, int MT, int kLimit>
+// 16-row tiles of a wave's sums that its workgroup's LDS holds at once, without a workgroup less on a CU.
+template <int NW, int NT, int MT, int RING>
 constexpr int epi_tiles() {
+  const int limit = (int)kMaxLds / ((int)kMaxLds / RING);
   int em = MT;
-  while (em > 1 && (MT % em != 0 || (size_t)NW * em * 16 * (NT * 16 + 4) * 4 + NW * MT * 64 > (size_t)kLimit)) --em;
+  while (em > 1 && (MT % em != 0 || NW * em * 16 * (NT * 16 + 4) * 4 + NW * MT * 64 > limit)) --em;
   return em;
 }
-template <int NW, int NT, int MT, int kLimit>
-constexpr size_t epi_bytes() { return (size_t)NW * epi_tiles<NW, NT, MT, kLimit>() * 16 * (NT * 16 + 4) * 4 + NW * MT * 64; }
+template <int NW, int NT, int MT, int RING>
+constexpr size_t epi_bytes() {
+  return (size_t)NW * epi_tiles<NW, NT, MT, RING>() * 16 * (NT * 16 + 4) * 4 + NW * MT * 64;
+}
 
 template <typename F, int... I>
 __device__ __forceinline__ void each_part(F&& f, std::integer_sequence<int, I...>) {
@@ -78,37 +81,41 @@ __device__ __forceinline__ void load8_vec(const void* p, int dtype, int n, int64
   }
 }
 
-enum W8Form { W8_OUT = 0, W8_PART = 1 };
-
-// 16 bytes of a row of K at k, any alignment; zeros past K.
-__device__ __forceinline__ u32x4 load16_any(const uint8_t* row, int k, int K) {
-  typedef u32x4 u32x4_b __attribute__((aligned(1)));
-  if (k + 16 <= K) return *reinterpret_cast<const u32x4_b*>(row + k);
-  u32x4 v = {0u, 0u, 0u, 0u};
-  for (int i = 0; i < 16; ++i)
-    if (k + i < K) v[i / 4] |= (uint32_t)row[k + i] << (i % 4 * 8);
-  return v;
+// A K split's sums of columns n .. n + 7 of a row.
+__device__ __forceinline__ void store8_part(float* to, const float (&v)[8], int n, int cols) {
+  if (n + 8 <= cols) {
+    typedef f32x4 f32x4_any __attribute__((aligned(4)));
+    *reinterpret_cast<f32x4_any*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4_any*>(to + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n + i < cols) to[i] = v[i];
+  }
 }
+
+enum W8Form { W8_OUT = 0, W8_PART = 1 };
 
 // Tiles of a group of row blocks: an XCD's workgroups share the activations of kGroup row blocks
 // and walk the weights (8192 x 28672 x 4096: 4, 8, 16 row blocks 750, 746, 781 us).
 constexpr int kGroup = 8;
 
-template <typename T, int WN, int WM, int NT, int MT, int D, bool SWIGLU, int FORM, bool DMA>
-__global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float* part, const uint8_t* x,
+template <typename T, int PW, int WN, int WM, int NT, int MT, int D, bool SWIGLU, int FORM, bool DMA>
+__global__ __launch_bounds__((WN * WM + PW) * kWave) void w8a8_tile_kernel(T* y, float* part, const uint8_t* x,
                                                                     const uint8_t* w, int M, int N, int K, int64_t sxm,
                                                                     int64_t swn, int64_t sym, int64_t syn, W8Epi e,
                                                                     int mtiles, int splits) {
   typedef typename Vec8<T>::type V8;
-  constexpr int NW = WN * WM, BN = WN * NT * 16, BM = WM * MT * 16;
-  constexpr int AOPS = BN / 8 / NW, BOPS = BM / 8 / NW, OPS = AOPS + BOPS;
-  static_assert(AOPS * 8 * NW == BN && BOPS * 8 * NW == BM, "the waves share a stage evenly");
+  constexpr int NW = WN * WM, LW = PW ? PW : NW, BN = WN * NT * 16, BM = WM * MT * 16;
+  constexpr int AOPS = BN / 8 / LW, BOPS = BM / 8 / LW, OPS = AOPS + BOPS;  // of a wave that loads
+  static_assert(AOPS * 8 * LW == BN && BOPS * 8 * LW == BM, "the loading waves share a stage evenly");
   static_assert(NT > 1 && (!SWIGLU || NT % 2 == 0), "gate and up tiles in turn");
-  static_assert(D >= 2 && (DMA || D == 2), "the register path holds one stage");
+  static_assert(D >= 2 && (DMA || (PW > 0 && D == 3)), "the register path has loading waves, two stages each");
   extern __shared__ __align__(16) u32x4 w8_smem[];
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int wm = wave % WM, wn = wave / WM;
+  const int lw = PW ? wave - NW : wave;  // which of the loading waves
   const int r = lane & 15, g = lane >> 4;
 
   // Block -> (tile, K split). Consecutive blocks go to the eight XCDs in turn: each XCD takes
@@ -139,6 +146,14 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
   const int stages_all = (K + kStep - 1) / kStep;
   const int s0 = (int)((int64_t)stages_all * split / splits);
   const int ns = (int)((int64_t)stages_all * (split + 1) / splits) - s0;
+  // With one row block no two workgroups share weights: each starts its K sweep at a stage of its
+  // own, so that they do not all read one line of every weight row at once (120 x 28672 x 4096:
+  // 33.1 -> 28.2 us). With more, workgroups that read the same lines together are faster.
+  const int rot = mtiles == 1 ? (int)((int64_t)(ntile & 31) * ns >> 5) : 0;
+  auto stage_k = [&](int s) {  // first k of this block's s-th stage
+    const int u = s + rot;
+    return (s0 + (u >= ns ? u - ns : u)) * kStep;
+  };
 
   // weight row at LDS row t of the tile (past the last: one that exists, never stored); SWIGLU:
   // a wave's 16-row tiles are gate and up rows in turn
@@ -166,7 +181,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
 #pragma unroll
   for (int i = 0; i < OPS; ++i) {
     const bool wt = i < AOPS;
-    const int t = (wt ? wave * AOPS + i : wave * BOPS + i - AOPS) * 8 + lane / 8;
+    const int t = (wt ? lw * AOPS + i : lw * BOPS + i - AOPS) * 8 + lane / 8;  // its row of the tile
     const int m = m0 + t;
     const int64_t row = wt ? wrow(t) : (m < M ? m : M - 1);
     off[i] = ((lane & 7) ^ (t & 7)) * 16;
@@ -175,12 +190,12 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
     else
       src[i] = wt ? w + row * swn : x + row * sxm;
   }
-  auto place = [&](int i) {  // byte address in a stage of this wave's i-th KiB
-    return (unsigned)(i < AOPS ? wave * AOPS + i : BN / 8 + wave * BOPS + i - AOPS) * 1024u;
+  auto place = [&](int i) {  // byte address in a stage of this wave's i-th KiB: weights, then activations
+    return (unsigned)(i < AOPS ? lw * AOPS + i : BN / 8 + lw * BOPS + i - AOPS) * 1024u;
   };
   auto issue_one = [&](int s, int i) {
-    const int k0 = (s0 + s) * kStep;
-    const bool up = SWIGLU && (((wave * AOPS + i) >> 1) & 1);  // 8 rows of an up tile
+    const int k0 = stage_k(s);
+    const bool up = SWIGLU && (((lw * AOPS + i) >> 1) & 1);  // 8 rows of an up tile
     const uint8_t* base = i < AOPS ? (up ? ubase : wbase) : xbase;
     const unsigned to = lds0 + (unsigned)(s % D) * kStage + place(i), o = voff[DMA ? i : 0];
     if (k0 + kStep <= K)
@@ -188,18 +203,23 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
     else  // pieces past K: the row's start
       dma16<false>(base, k0 + off[i] < K ? o + (unsigned)k0 : o - (unsigned)off[i], to);
   };
-  u32x4 held[DMA ? 1 : OPS];
-  auto fetch = [&](int s) {  // stage s into registers
-    const int k0 = (s0 + s) * kStep;
+  u32x4 held[DMA ? 1 : 2][DMA ? 1 : OPS];
+  auto fetch = [&](int s, auto h) {  // stage s into registers
+    const int k0 = stage_k(s);
+    if (k0 + kStep <= K) {
 #pragma unroll
-    for (int i = 0; i < OPS; ++i) held[DMA ? 0 : i] = load16_any(src[DMA ? 0 : i], k0 + off[i], K);
+      for (int i = 0; i < OPS; ++i) held[h][DMA ? 0 : i] = load16_any(src[DMA ? 0 : i] + k0 + off[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < OPS; ++i) held[h][DMA ? 0 : i] = load16_end(src[DMA ? 0 : i], k0 + off[i], K);
+    }
   };
-  auto put = [&](int s) {  // and on into LDS
+  auto put = [&](int s, auto h) {  // and on into LDS
 #pragma unroll
-    for (int i = 0; i < OPS; ++i) w8_smem[((s % D) * kStage + place(i)) / 16 + lane] = held[DMA ? 0 : i];
+    for (int i = 0; i < OPS; ++i) w8_smem[((s % D) * kStage + place(i)) / 16 + lane] = held[h][DMA ? 0 : i];
   };
   auto zero_tail = [&](int s) {  // DMA past K brought the row's start: the activations there become zero
-    const int k0 = (s0 + s) * kStep;
+    const int k0 = stage_k(s);
     if (k0 + kStep > K) {
 #pragma unroll
       for (int i = AOPS; i < OPS; ++i)
@@ -216,6 +236,72 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
   // this lane's two chunks of a tile row (u32x4 entries): row r of a 16-row tile, r mod 8 is
   // every tile's swizzle
   const int c0 = g ^ (r & 7), c1 = (4 + g) ^ (r & 7);
+  // The loads of a stage and its waits, by the waves that load: all of them, or PW of their own
+  // whose DMAs, each of which holds its wave for over a hundred cycles, then hold no MFMA.
+  auto load_first = [&]() {
+    if constexpr (DMA) {
+      const int pre = ns < D ? ns : D;
+      for (int s = 0; s < pre; ++s)
+#pragma unroll
+        for (int i = 0; i < OPS; ++i) issue_one(s, i);
+      if (ns >= D)
+        wait_vm<OPS*(D - 1)>();
+      else
+        wait_vm<0>();
+      zero_tail(0);
+    }
+  };
+  auto wait_next = [&](int s) {  // stage s + 1 has landed
+    if constexpr (DMA) {
+      if (s + D <= ns)  // issued so far: to stage s + D - 1
+        wait_vm<OPS*(D - 2)>();
+      else
+        wait_vm<0>();
+      if (s + 1 < ns) zero_tail(s + 1);
+    }
+  };
+  if constexpr (PW > 0) {
+    if (wave >= NW) {
+      if constexpr (DMA) {
+        if (ns > 0) {
+          load_first();
+          lds_barrier();
+        }
+        for (int s = 0; s < ns; ++s) {
+          wait_next(s);
+          lds_barrier();
+          if (s + D < ns) {
+#pragma unroll
+            for (int i = 0; i < OPS; ++i) issue_one(s + D, i);
+          }
+        }
+      } else if (ns > 0) {
+        // stages go into LDS as their buffers come free, two ahead of that in registers
+        const std::integral_constant<int, 0> even{};
+        const std::integral_constant<int, 1> odd{};
+        fetch(0, even);
+        if (ns > 1) fetch(1, odd);
+        put(0, even);
+        if (ns > 2) fetch(2, even);
+        if (ns > 1) put(1, odd);
+        if (ns > 3) fetch(3, odd);
+        if (ns > 2) put(2, even);
+        if (ns > 4) fetch(4, even);
+        lds_barrier();
+        auto step = [&](int s, auto h) {  // of stage s: s + 3 into its buffer
+          lds_barrier();
+          if (s + 3 < ns) put(s + 3, h);
+          if (s + 5 < ns) fetch(s + 5, h);
+        };
+        for (int s = 0; s < ns; s += 2) {
+          step(s, odd);
+          if (s + 1 < ns) step(s + 1, even);
+        }
+      }
+      return;  // a wave that has ended is not waited for at a barrier
+    }
+  }
+
   u32x4 a0[NT], a1[NT], b0[MT], b1[MT];
   auto load_a = [&](int s, int n) {
     const u32x4* p = w8_smem + (s % D) * (kStage / 16) + ((wn * NT + n) * 16 + r) * 8;
@@ -228,24 +314,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
     b1[m] = p[c1];
   };
   if (ns > 0) {
-    if constexpr (DMA) {
-      const int pre = ns < D ? ns : D;
-      for (int s = 0; s < pre; ++s)
-#pragma unroll
-        for (int i = 0; i < OPS; ++i) issue_one(s, i);
-      if (ns >= D)
-        wait_vm<OPS*(D - 1)>();
-      else
-        wait_vm<0>();
-      zero_tail(0);
-    } else {
-      fetch(0);
-      put(0);
-      if (ns > 1) {
-        fetch(1);
-        put(1);
-      }
-    }
+    if constexpr (PW == 0) load_first();
     lds_barrier();
 #pragma unroll
     for (int n = 0; n < NT; ++n) load_a(0, n);
@@ -257,24 +326,14 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[0][m] = mfma_e4m3(a0[0], a1[0], b0[m], b1[m], acc[0][m]);
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (DMA) {
-      // issued so far: to stage s + D - 1; the next stage has to be there
-      if (s + D <= ns)
-        wait_vm<OPS*(D - 2)>();
-      else
-        wait_vm<0>();
-      if (s + 1 < ns) zero_tail(s + 1);
-    }
+    if constexpr (PW == 0) wait_next(s);
     lds_barrier();  // stage s is in every wave's registers, stage s + 1 in LDS
-    const bool more = s + D < ns;
-    if constexpr (!DMA) {
-      if (more) fetch(s + 2);
-    }
+    const bool more = PW == 0 && s + D < ns;
     // (past the last stage the registers are refilled with what the ring holds, and not used)
 #pragma unroll
     for (int n = 1; n < NT; ++n) {
       load_a(s + 1, n - 1);
-      if constexpr (DMA) {
+      if constexpr (PW == 0) {
         if (more) {
 #pragma unroll
           for (int i = OPS * (n - 1) / (NT - 1); i < OPS * n / (NT - 1); ++i) issue_one(s + D, i);
@@ -293,95 +352,87 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
     }
     load_a(s + 1, NT - 1);
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (!DMA) {
-      if (more) put(s + 2);
-    }
   }
 
+  // The sums go through LDS, EM tiles of 16 activation rows of a wave at a time, and leave along the
+  // rows: a lane has the same eight output columns of every row it writes.
+  constexpr int EM = epi_tiles<NW, NT, MT, (int)(kStageBytes<BN, BM> * D)>(), PITCH = NT * 16 + 4, TPR = WOUT / 8,
+                RPP = kWave / TPR, U = EM * 16 >= RPP * 2 ? 2 : 1;
+  static_assert(EM * 16 % (RPP * U) == 0, "whole passes");
   const int n0 = ntile * OUT + wn * WOUT;  // this wave's first output column
-  if constexpr (FORM == W8_PART) {
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int row = m0 + (wm * MT + m) * 16 + r;
-      if (row >= M) continue;
-      float* to = part + ((int64_t)split * M + row) * N;
-#pragma unroll
-      for (int f = 0; f < NT; ++f) {
-        const int n = n0 + (SWIGLU ? f >> 1 : f) * 16 + g * 4, at = n + (SWIGLU && (f & 1) ? half : 0);
-        if (n + 4 <= cols && N % 4 == 0 && (!SWIGLU || half % 4 == 0)) {
-          *reinterpret_cast<f32x4*>(to + at) = acc[f][m];
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (n + i < cols) to[at + i] = acc[f][m][i];
-        }
-      }
-    }
-  } else {
-    // Each wave's sums go through LDS of its own, EM tiles of 16 activation rows at a time, and
-    // leave along the rows: a lane has the same eight output columns of every row it writes.
-    constexpr int EM = epi_tiles<NW, NT, MT, (int)(kStageBytes<BN, BM> * D)>(), PITCH = NT * 16 + 4, TPR = WOUT / 8,
-                  RPP = kWave / TPR, U = EM * 16 >= RPP * 2 ? 2 : 1;
-    static_assert(EM * 16 % (RPP * U) == 0, "whole passes");
-    float* sums = reinterpret_cast<float*>(w8_smem) + wave * (EM * 16 * PITCH);
-    float* xsl = reinterpret_cast<float*>(w8_smem) + NW * (EM * 16 * PITCH) + wave * (MT * 16);
-    const int oc = lane % TPR * 8, n = n0 + oc, rr = lane / TPR;
-    const int sc = SWIGLU ? (oc >> 4) * 32 + (oc & 15) : oc;  // its column of the sums; SWIGLU: up 16 further
-    const int mrow = m0 + wm * MT * 16;
-    float s1[8], b1[8], s2[SWIGLU ? 8 : 1], b2[SWIGLU ? 8 : 1];
-    load8_vec(e.ws, FD_F32, n, 1, cols, s1);
-    load8_vec(e.bias, e.bias_dtype, n, e.sb, cols, b1);
+  float* const all = reinterpret_cast<float*>(w8_smem);
+  float* const sums = all + wave * (EM * 16 * PITCH);
+  float* const xsl = all + NW * (EM * 16 * PITCH) + wave * (MT * 16);
+  const int oc = lane % TPR * 8, n = n0 + oc, rr = lane / TPR;
+  const int sc = SWIGLU ? (oc >> 4) * 32 + (oc & 15) : oc;  // its column of the sums; SWIGLU: up 16 further
+  const int mrow = m0 + wm * MT * 16;
+  const bool whole = n + 8 <= cols, wide = whole && syn == 1;
+  const int add_dtype = e.row_dtype, add = !e.row ? 0 : e.srn != 1 ? 3 : add_dtype == FD_F32 ? 2 : 1;
+  float scale1[8], bias1[8], scale2[SWIGLU ? 8 : 1], bias2[SWIGLU ? 8 : 1], xv[(MT * 16 + kWave - 1) / kWave];
+  if constexpr (FORM == W8_OUT) {
+    load8_vec(e.ws, FD_F32, n, 1, cols, scale1);
+    load8_vec(e.bias, e.bias_dtype, n, e.sb, cols, bias1);
     if constexpr (SWIGLU) {
-      load8_vec(e.ws + half, FD_F32, n, 1, cols, s2);
-      load8_vec(e.bias, e.bias_dtype, n, e.sb, cols, b2, half);
+      load8_vec(e.ws + half, FD_F32, n, 1, cols, scale2);
+      load8_vec(e.bias, e.bias_dtype, n, e.sb, cols, bias2, half);
     }
-    float xv[(MT * 16 + kWave - 1) / kWave];
 #pragma unroll
     for (int i = 0; i < MT * 16; i += kWave) {
       const int row = mrow + i + lane;
       xv[i / kWave] = e.xs[row < M ? row : M - 1];
     }
-    const bool whole = n + 8 <= cols, wide = whole && syn == 1;
-    const int add_dtype = e.row_dtype, add = !e.row ? 0 : e.srn != 1 ? 3 : add_dtype == FD_F32 ? 2 : 1;
-    lds_barrier();  // the last stage has been read everywhere
+  }
+  auto part_of = [&](auto which) {
+    constexpr int h = decltype(which)::value;
+    if constexpr (h == 0) lds_barrier();  // the last stage has been read everywhere
+    if constexpr (FORM == W8_OUT && h == 0) {
 #pragma unroll
-    for (int i = 0; i < MT * 16; i += kWave)
-      if (i + lane < MT * 16) xsl[i + lane] = xv[i / kWave];
-    auto part_of = [&](auto part) {
-      constexpr int h = decltype(part)::value;
+      for (int i = 0; i < MT * 16; i += kWave)
+        if (i + lane < MT * 16) xsl[i + lane] = xv[i / kWave];
+    }
 #pragma unroll
-      for (int m = 0; m < EM; ++m)
+    for (int m = 0; m < EM; ++m)
 #pragma unroll
-        for (int f = 0; f < NT; ++f)
-          *reinterpret_cast<f32x4*>(sums + (m * 16 + r) * PITCH + f * 16 + g * 4) = acc[f][h * EM + m];
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      for (int f = 0; f < NT; ++f)
+        *reinterpret_cast<f32x4*>(sums + (m * 16 + r) * PITCH + f * 16 + g * 4) = acc[f][h * EM + m];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll 1
-      for (int t0 = rr; t0 < EM * 16; t0 += RPP * U) {
-        u32x4 lo[U], hi[U];
-        if (whole && (add == 1 || add == 2)) {
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int row = mrow + h * EM * 16 + t0 + u * RPP;
-            const int64_t at = (row < M ? row : M - 1) * e.srm + n;
-            const char* p = static_cast<const char*>(e.row) + at * (add == 2 ? 4 : 2);
-            lo[u] = *reinterpret_cast<const u32x4_any*>(p);
-            if (add == 2) hi[u] = *reinterpret_cast<const u32x4_any*>(p + 16);
-          }
-        }
+    for (int t0 = rr; t0 < EM * 16; t0 += RPP * U) {
+      u32x4 lo[U], hi[U];
+      if (FORM == W8_OUT && whole && (add == 1 || add == 2)) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int t = t0 + u * RPP, row = mrow + h * EM * 16 + t;
-          const float xs = xsl[h * EM * 16 + t];
-          const float* p = sums + t * PITCH + sc;
-          float v[8];
+          const int row = mrow + h * EM * 16 + t0 + u * RPP;
+          const int64_t at = (row < M ? row : M - 1) * e.srm + n;
+          const char* p = static_cast<const char*>(e.row) + at * (add == 2 ? 4 : 2);
+          lo[u] = *reinterpret_cast<const u32x4_any*>(p);
+          if (add == 2) hi[u] = *reinterpret_cast<const u32x4_any*>(p + 16);
+        }
+      }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = p[i] * xs * s1[i] + b1[i];
-          if constexpr (SWIGLU) {
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * RPP, row = mrow + h * EM * 16 + t;
+        const float* p = sums + t * PITCH + sc;
+        float v[8], up[SWIGLU ? 8 : 1];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = times_sigmoid(v[i], v[i]) * (p[16 + i] * xs * s2[i] + b2[i]);
-          } else {
-            activate(v, e.act);
+        for (int i = 0; i < 8; ++i) {
+          v[i] = p[i];
+          if constexpr (SWIGLU) up[i] = p[16 + i];
+        }
+        if constexpr (FORM == W8_PART) {
+          if (row < M) {
+            float* const to = part + ((int64_t)split * M + row) * N + n;
+            store8_part(to, v, n, cols);
+            if constexpr (SWIGLU) store8_part(to + half, up, n, cols);
           }
+        } else {
+          const float xs = xsl[h * EM * 16 + t];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            v[i] = v[i] * xs * scale1[i] + bias1[i];
+            if constexpr (SWIGLU) v[i] = times_sigmoid(v[i], v[i]) * (up[i] * xs * scale2[i] + bias2[i]);
+          }
+          if constexpr (!SWIGLU) activate(v, e.act);
           if (row >= M || n >= cols) continue;
           if (add) {
             if (!whole || add == 3) {
@@ -415,88 +466,173 @@ __global__ __launch_bounds__(WN * WM * kWave) void w8a8_tile_kernel(T* y, float*
           }
         }
       }
-    };
-    each_part(part_of, std::make_integer_sequence<int, MT / EM>{});
-  }
+    }
+  };
+  each_part(part_of, std::make_integer_sequence<int, MT / EM>{});
 }
 
-// The K splits' sums, added in split order, then the epilogue: a thread per output.
+// The K splits' sums, added in split order, then the epilogue: a thread per four columns of a
+// row, with four splits' sums on the way at once.
 template <typename T, bool SWIGLU>
 __global__ __launch_bounds__(256) void w8a8_sum_kernel(T* y, const float* part, int M, int N, int splits, int64_t sym,
-                                                       int64_t syn, W8Epi e, FastDiv cols, uint32_t total) {
+                                                       int64_t syn, W8Epi e, FastDiv quads, uint32_t total) {
   const uint32_t v = blockIdx.x * 256 + threadIdx.x;
   if (v >= total) return;
-  uint32_t c;
-  const uint32_t m = cols.divmod(v, c);
-  const int half = N / 2;
+  uint32_t q;
+  const uint32_t m = quads.divmod(v, q);
+  const int c = (int)q * 4, half = N / 2, cols = SWIGLU ? half : N;
   const float* p = part + (int64_t)m * N + c;
   const int64_t step = (int64_t)M * N;
-  float a = 0.f, u = 0.f;
-  for (int i = 0; i < splits; ++i) {
-    a += p[i * step];
-    if constexpr (SWIGLU) u += p[i * step + half];
+  f32x4 a = {0.f, 0.f, 0.f, 0.f}, u = a;
+  if (N % 4 == 0 && (!SWIGLU || half % 4 == 0)) {
+    for (int i = 0; i < splits; i += 4) {
+      f32x4 t[4], w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float* at = p + (i + j < splits ? i + j : splits - 1) * step;
+        t[j] = *reinterpret_cast<const f32x4*>(at);
+        if constexpr (SWIGLU) w[j] = *reinterpret_cast<const f32x4*>(at + half);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j < splits) {
+          a += t[j];
+          if constexpr (SWIGLU) u += w[j];
+        }
+    }
+  } else {
+    for (int i = 0; i < splits; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < cols) {
+          a[j] += p[i * step + j];
+          if constexpr (SWIGLU) u[j] += p[i * step + half + j];
+        }
   }
-  y[(int64_t)m * sym + c * syn] = from_f32<T>(w8_out<SWIGLU>(e, a, u, m, c, half));
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (c + j < cols)
+      y[(int64_t)m * sym + (c + j) * syn] = from_f32<T>(w8_out<SWIGLU>(e, a[j], u[j], m, c + j, half));
 }
 
 namespace {
 
-template <typename T, int WN, int WM, int NT, int MT, int D, bool SWIGLU, int FORM, bool DMA>
+template <typename T, int PW, int WN, int WM, int NT, int MT, int D, bool SWIGLU, int FORM, bool DMA>
 int tile_launch(const W8Args& a, int splits) {
   constexpr int BN = WN * NT * 16, BM = WM * MT * 16;
   constexpr size_t ring = (size_t)kStageBytes<BN, BM> * D;
-  constexpr size_t sums = FORM == W8_OUT ? epi_bytes<WN * WM, NT, MT, (int)ring>() : 0;
+  constexpr size_t sums = epi_bytes<WN * WM, NT, MT, (int)ring>();
   constexpr size_t lds = ring > sums ? ring : sums;
   static_assert(lds <= kMaxLds, "a launch fits the LDS of a CU");
   const int64_t nt = (a.N + BN - 1) / BN, mt = (a.M + BM - 1) / BM;
   if (nt * mt * splits > 0x7fffffffLL) return set_error(FD_EUNSUPPORTED, "too many tiles");
-  auto kernel = w8a8_tile_kernel<T, WN, WM, NT, MT, D, SWIGLU, FORM, DMA>;
+  auto kernel = w8a8_tile_kernel<T, PW, WN, WM, NT, MT, D, SWIGLU, FORM, DMA>;
   if (!allow_lds(kernel, lds)) return set_error(FD_ELAUNCH, "cannot raise the LDS limit to %zu bytes", lds);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(nt * mt * splits)), dim3(WN * WM * kWave), lds, a.st,
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(nt * mt * splits)), dim3((WN * WM + PW) * kWave), lds, a.st,
                      static_cast<T*>(a.y), a.scratch, a.x, a.w, a.M, a.N, a.K, a.sxm, a.swn, a.sym, a.syn, a.e, (int)mt,
                      splits);
   return FD_OK;
 }
 
-// Whether tiles of 256 x 256, one to a CU, take less time than tiles of 128 x 128, two to a CU:
-// rounds of workgroups, each of its stages and what its start and its output cost (us, measured).
-bool w8_large(int64_t M, int64_t N, int64_t K) {
-  auto rounds = [&](int64_t b, int64_t slots) {
-    const int64_t tiles = ((M + b - 1) / b) * ((N + b - 1) / b);
-    return (double)((tiles + slots - 1) / slots);
-  };
-  const double stages = (double)((K + kStep - 1) / kStep);
-  const int cus = device_cus();
-  return rounds(256, cus) * (stages * 1.35 + 9) < rounds(128, 2 * cus) * (stages * 0.95 + 6);
+// The forms of a tile launch: output columns (weight rows) and activation rows of a tile, workgroups
+// that a CU holds, and microseconds that a stage of all of them takes and a round of them besides (its start, its
+// output), measured.
+struct TileForm {
+  int bn, bm, per_cu;
+  float stage, round;
+};
+enum { T_256 = 0, T_256x128, T_128, T_64x128, T_64, T_128x32, T_UNALIGNED, T_FORMS };
+constexpr TileForm kTiles[T_FORMS] = {{256, 256, 1, 1.40f, 9.f},  {256, 128, 1, 0.80f, 6.f}, {128, 128, 1, 0.58f, 5.f},
+                                      {64, 128, 1, 0.37f, 5.f},   {64, 64, 1, 0.29f, 4.5f},  {128, 32, 1, 0.33f, 4.f},
+                                      {128, 256, 1, 1.20f, 8.f}};
+
+struct TilePlan {
+  int form, splits;
+};
+
+// The form and the K splits (as many as give every CU one workgroup, each with at least six stages) that take the
+// least time by that table. Adding the splits' sums is a launch, and their floats go to memory and back.
+TilePlan tile_plan(int64_t M, int64_t N, int64_t K, bool dma) {
+  const int64_t stages = (K + kStep - 1) / kStep, cus = device_cus();
+  TilePlan best{T_UNALIGNED, 1};
+  float least = INFINITY;
+  for (int f = 0; f < T_FORMS; ++f) {
+    if (dma == (f == T_UNALIGNED)) continue;
+    const TileForm& t = kTiles[f];
+    const int64_t tiles = ((N + t.bn - 1) / t.bn) * ((M + t.bm - 1) / t.bm);
+    int64_t most = cus / (tiles < cus ? tiles : cus);
+    if (most > stages / 6) most = stages / 6;
+    for (int64_t s = 1; s == 1 || s <= most; ++s) {
+      const int64_t rounds = (tiles * s + cus * t.per_cu - 1) / (cus * t.per_cu);
+      const float sum = s > 1 ? 4.f + (float)(s * M * N) * 8e-6f / 4.f : 0.f;  // 4 TB/s there and back
+      const float us = (float)rounds * ((float)((stages + s - 1) / s) * t.stage + t.round) + sum;
+      if (us < least) {
+        least = us;
+        best = TilePlan{f, (int)s};
+      }
+    }
+  }
+  return best;
 }
 
 template <typename T, bool SWIGLU, int FORM>
-int pick_tile(const W8Args& a, int splits, bool dma) {
-  if (!dma) return tile_launch<T, 2, 2, 4, 4, 2, SWIGLU, FORM, false>(a, splits);
-  if constexpr (FORM == W8_OUT) {
-    if (w8_large(a.M, a.N, a.K)) return tile_launch<T, 4, 2, 4, 8, 2, SWIGLU, FORM, true>(a, 1);
+int pick_tile(const W8Args& a, TilePlan p) {
+  switch (p.form) {
+    case T_256: return tile_launch<T, 0, 4, 2, 4, 8, 2, SWIGLU, FORM, true>(a, p.splits);
+    case T_256x128: return tile_launch<T, 4, 4, 2, 4, 4, 3, SWIGLU, FORM, true>(a, p.splits);
+    case T_128: return tile_launch<T, 0, 2, 4, 4, 2, 4, SWIGLU, FORM, true>(a, p.splits);
+    case T_64x128: return tile_launch<T, 0, 2, 4, 2, 2, 4, SWIGLU, FORM, true>(a, p.splits);
+    case T_64: return tile_launch<T, 4, 2, 2, 2, 2, 4, SWIGLU, FORM, true>(a, p.splits);
+    case T_128x32: return tile_launch<T, 0, 4, 1, 2, 2, 4, SWIGLU, FORM, true>(a, p.splits);
+    default: return tile_launch<T, 4, 2, 4, 4, 4, 3, SWIGLU, FORM, false>(a, p.splits);
   }
-  return tile_launch<T, 2, 2, 4, 4, 2, SWIGLU, FORM, true>(a, splits);
 }
 
 template <typename T, bool SWIGLU>
-int tiles(const W8Args& a, int splits, bool dma) {
-  if (splits == 1) return pick_tile<T, SWIGLU, W8_OUT>(a, 1, dma);
-  const int rc = pick_tile<T, SWIGLU, W8_PART>(a, splits, dma);
+int tiles(const W8Args& a, TilePlan p) {
+  if (p.splits == 1) return pick_tile<T, SWIGLU, W8_OUT>(a, p);
+  const int rc = pick_tile<T, SWIGLU, W8_PART>(a, p);
   if (rc != FD_OK) return rc;
-  const int cols = SWIGLU ? a.N / 2 : a.N;
-  const uint32_t total = (uint32_t)a.M * (uint32_t)cols;  // splits > 1: few tiles, so M * N is small
+  const int quads = ((SWIGLU ? a.N / 2 : a.N) + 3) / 4;
+  const uint32_t total = (uint32_t)a.M * (uint32_t)quads;  // splits > 1: few tiles, so M * N is small
   hipLaunchKernelGGL((w8a8_sum_kernel<T, SWIGLU>), dim3((total + 255) / 256), dim3(256), 0, a.st, static_cast<T*>(a.y),
-                     a.scratch, a.M, a.N, splits, a.sym, a.syn, a.e, FastDiv((uint32_t)cols), total);
+                     a.scratch, a.M, a.N, p.splits, a.sym, a.syn, a.e, FastDiv((uint32_t)quads), total);
   return FD_OK;
 }
 
-// K splits of a product: enough for one workgroup on every CU, each with at least four stages.
-int w8_splits(int64_t M, int64_t N, int64_t K) {
-  const int64_t tiles = ((N + 127) / 128) * ((M + 127) / 128), stages = (K + kStep - 1) / kStep;
-  int64_t s = device_cus() / tiles;
-  if (s > stages / 4) s = stages / 4;
-  return s < 1 ? 1 : (int)s;
+// K below one 16-byte piece, none included: a thread per output.
+template <typename T, bool SWIGLU>
+__global__ __launch_bounds__(256) void w8a8_short_kernel(T* y, const uint8_t* x, const uint8_t* w, int M, int N, int K,
+                                                         int64_t sxm, int64_t swn, int64_t sym, int64_t syn, W8Epi e,
+                                                         int64_t total) {
+  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (v >= total) return;
+  const int cols = SWIGLU ? N / 2 : N, m = (int)(v / cols), c = (int)(v - (int64_t)m * cols);
+  float a = 0.f, u = 0.f;
+  for (int k = 0; k < K; ++k) {
+    const float xv = __builtin_amdgcn_cvt_f32_fp8(x[m * sxm + k], 0);
+    a += xv * __builtin_amdgcn_cvt_f32_fp8(w[c * swn + k], 0);
+    if constexpr (SWIGLU) u += xv * __builtin_amdgcn_cvt_f32_fp8(w[(c + (int64_t)cols) * swn + k], 0);
+  }
+  y[m * sym + c * syn] = from_f32<T>(w8_out<SWIGLU>(e, a, u, m, c, cols));
+}
+
+template <typename T, bool SWIGLU>
+int short_launch(const W8Args& a) {
+  const int64_t total = (int64_t)a.M * (SWIGLU ? a.N / 2 : a.N), blocks = (total + 255) / 256;
+  if (blocks > 0x7fffffffLL) return set_error(FD_EUNSUPPORTED, "too large");
+  hipLaunchKernelGGL((w8a8_short_kernel<T, SWIGLU>), dim3((unsigned)blocks), dim3(256), 0, a.st, static_cast<T*>(a.y),
+                     a.x, a.w, a.M, a.N, a.K, a.sxm, a.swn, a.sym, a.syn, a.e, total);
+  return FD_OK;
+}
+
+template <typename T, bool SWIGLU>
+int product(const W8Args& a) {
+  if (a.K < 16) return short_launch<T, SWIGLU>(a);
+  if (w8_few_fits(a)) return w8_few_launch(a);
+  TilePlan p = tile_plan(a.M, a.N, a.K, a.dma);
+  while (p.splits > 1 && a.scratch_bytes < (int64_t)p.splits * a.M * a.N * 4) --p.splits;
+  return tiles<T, SWIGLU>(a, p);
 }
 
 constexpr int64_t kMostIndex = 0x7fffffffLL - 512;  // indexes run to the end of the last tile and stage
@@ -510,8 +646,14 @@ extern "C" int fd_linear_w8a8_scratch(int64_t M, int64_t N, int64_t K, int64_t* 
   if (M < 0 || N < 0 || K < 0) return set_error(FD_EINVAL, "negative size");
   if (!bytes) return set_error(FD_EINVAL, "null pointer argument");
   *bytes = 0;
-  if (M == 0 || N == 0 || M > kMostIndex || N > kMostIndex || K > kMostIndex) return FD_OK;
-  const int s = w8_splits(M, N, K);
+  if (M == 0 || N == 0 || K < 16 || M > kMostIndex || N > kMostIndex || K > kMostIndex) return FD_OK;
+  W8Args a{};
+  a.M = (int)M;
+  a.N = (int)N;
+  a.K = (int)K;
+  a.dma = K % 16 == 0;
+  if (w8_few_fits(a)) return FD_OK;
+  const int s = tile_plan(M, N, K, a.dma).splits;
   if (s > 1) *bytes = (int64_t)s * M * N * 4;
   return FD_OK;
 }
@@ -560,12 +702,10 @@ extern "C" int fd_linear_w8a8(void* y, const void* x8, const float* x_scale, con
   a.act_dtype = act_dtype;
   a.st = static_cast<hipStream_t>(stream);
   // the DMAs' 32-bit offsets reach over a tile's rows
-  const bool dma = K % 16 == 0 && aligned16(x8) && aligned16(w8) && (M == 1 || sxm % 16 == 0) &&
-                   (N == 1 || swn % 16 == 0) && sxm < (1 << 23) && swn < (1 << 23);
-  int splits = w8_splits(M, N, K);
-  while (splits > 1 && a.scratch_bytes < (int64_t)splits * M * N * 4) --splits;
-  const int rc = act_dtype == FD_F16 ? (swiglu ? tiles<f16, true>(a, splits, dma) : tiles<f16, false>(a, splits, dma))
-                                     : (swiglu ? tiles<bf16, true>(a, splits, dma) : tiles<bf16, false>(a, splits, dma));
+  a.dma = K % 16 == 0 && aligned16(x8) && aligned16(w8) && (M == 1 || sxm % 16 == 0) && (N == 1 || swn % 16 == 0) &&
+          sxm < (1 << 23) && swn < (1 << 23);
+  const int rc = act_dtype == FD_F16 ? (swiglu ? product<f16, true>(a) : product<f16, false>(a))
+                                     : (swiglu ? product<bf16, true>(a) : product<bf16, false>(a));
   if (rc != FD_OK) return rc;
   return check_launch();
 }

@@ -211,7 +211,8 @@ SIZES = [(1, 1, 1), (1, 16, 128), (1, 33, 4096), (2, 130, 272), (3, 4, 16), (7, 
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("m,n,k", SIZES + [(5, 40, 131), (70, 140, 1023), (130, 300, 257), (9, 24, 15)])
+@pytest.mark.parametrize("m,n,k", SIZES + [(5, 40, 131), (70, 140, 1023), (130, 300, 257), (9, 24, 15), (1, 520, 4097),
+                                           (20, 100, 2051), (3, 70, 8191), (40, 33, 8200), (12, 9, 17), (2, 300, 13)])
 def test_products_of_small_integers_are_exact(m, n, k, dtype):
     import fused_decode as fd
 
