@@ -155,13 +155,13 @@ __device__ __forceinline__ float w8_out(const W8Epi& e, float acc, float up, int
   return v;
 }
 
-// A checked product, as the launchers take it.
+// A checked product, as the launchers take it: 16-byte aligned rows of whole 16-byte pieces but for K < 16.
 struct W8Args {
   void* y;
   const uint8_t *x, *w;
   int M, N, K;  // N: rows of w
   int64_t sxm, swn, sym, syn;
-  bool swiglu, dma;  // dma: 16-byte aligned rows of whole 16-byte pieces
+  bool swiglu;
   W8Epi e;
   float* scratch;
   int64_t scratch_bytes;
@@ -170,7 +170,7 @@ struct W8Args {
 };
 
 // Few rows (w8a8_few.hip): whether a product fits, and its launch.
-bool w8_few_fits(const W8Args& a);
+bool w8_few_fits(int64_t M, int64_t K);
 int w8_few_launch(const W8Args& a);
 
 }  // namespace fd

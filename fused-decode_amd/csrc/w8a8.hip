@@ -2,10 +2,10 @@
 // activation rows (fd_w8a8.h has the mathematics).
 //
 // A workgroup of WN x WM waves owns BN weight rows x BM activation rows and walks K in stages
-// of 128. Both tiles of a stage go to LDS in a ring of D stages: by DMA (global_load_lds_dwordx4)
-// where rows are 16-byte aligned and K % 16 == 0, else through registers with 16-byte loads at
-// any address (bytes where a piece crosses K). The DMAs are inline assembly, so the compiler sees
-// plain LDS reads and schedules and waits for those itself; the vmcnt waits are explicit.
+// of 128. Both tiles of a stage go to LDS in a ring of D stages by DMA (global_load_lds_dwordx4), so
+// rows have to be 16-byte aligned: others are copied into scratch first (w8a8_align_kernel). The
+// DMAs are inline assembly, so the compiler sees plain LDS reads and schedules and waits for those
+// itself; the vmcnt waits are explicit.
 //
 // The matrix cores are fed from registers that hold the whole stage: weight tile n's registers
 // are refilled with the next stage's once row n of the wave's tiles is multiplied, the
@@ -100,7 +100,7 @@ enum W8Form { W8_OUT = 0, W8_PART = 1 };
 // and walk the weights (8192 x 28672 x 4096: 4, 8, 16 row blocks 750, 746, 781 us).
 constexpr int kGroup = 8;
 
-template <typename T, int PW, int WN, int WM, int NT, int MT, int D, bool SWIGLU, int FORM, bool DMA>
+template <typename T, int PW, int WN, int WM, int NT, int MT, int D, bool SWIGLU, int FORM>
 __global__ __launch_bounds__((WN * WM + PW) * kWave) void w8a8_tile_kernel(T* y, float* part, const uint8_t* x,
                                                                     const uint8_t* w, int M, int N, int K, int64_t sxm,
                                                                     int64_t swn, int64_t sym, int64_t syn, W8Epi e,
@@ -110,7 +110,6 @@ __global__ __launch_bounds__((WN * WM + PW) * kWave) void w8a8_tile_kernel(T* y,
   constexpr int AOPS = BN / 8 / LW, BOPS = BM / 8 / LW, OPS = AOPS + BOPS;  // of a wave that loads
   static_assert(AOPS * 8 * LW == BN && BOPS * 8 * LW == BM, "the loading waves share a stage evenly");
   static_assert(NT > 1 && (!SWIGLU || NT % 2 == 0), "gate and up tiles in turn");
-  static_assert(D >= 2 && (DMA || (PW > 0 && D == 3)), "the register path has loading waves, two stages each");
   extern __shared__ __align__(16) u32x4 w8_smem[];
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -169,14 +168,13 @@ __global__ __launch_bounds__((WN * WM + PW) * kWave) void w8a8_tile_kernel(T* y,
 
   const unsigned lds0 = lds_addr(w8_smem);
   constexpr unsigned kStage = (unsigned)kStageBytes<BN, BM>;
-  // DMA: a scalar base for the tile's weight rows (SWIGLU: and its up rows) and activation rows, and a
-  // 32-bit offset a lane; else pointers
+  // a scalar base for the tile's weight rows (SWIGLU: and its up rows) and activation rows, and a 32-bit
+  // offset a lane
   const int64_t n_first = (int64_t)ntile * OUT < cols ? (int64_t)ntile * OUT : cols - 1;
   const uint8_t* const wbase = w + n_first * swn;
   const uint8_t* const ubase = SWIGLU ? wbase + (int64_t)half * swn : wbase;
   const uint8_t* const xbase = x + (int64_t)m0 * sxm;
-  const uint8_t* src[DMA ? 1 : OPS];
-  unsigned voff[DMA ? OPS : 1];
+  unsigned voff[OPS];
   int off[OPS];
 #pragma unroll
   for (int i = 0; i < OPS; ++i) {
@@ -185,10 +183,7 @@ __global__ __launch_bounds__((WN * WM + PW) * kWave) void w8a8_tile_kernel(T* y,
     const int m = m0 + t;
     const int64_t row = wt ? wrow(t) : (m < M ? m : M - 1);
     off[i] = ((lane & 7) ^ (t & 7)) * 16;
-    if constexpr (DMA)
-      voff[i] = (unsigned)(wt ? (row - n_first - (SWIGLU && ((t >> 4) & 1) ? half : 0)) * swn : (row - m0) * sxm) + off[i];
-    else
-      src[i] = wt ? w + row * swn : x + row * sxm;
+    voff[i] = (unsigned)(wt ? (row - n_first - (SWIGLU && ((t >> 4) & 1) ? half : 0)) * swn : (row - m0) * sxm) + off[i];
   }
   auto place = [&](int i) {  // byte address in a stage of this wave's i-th KiB: weights, then activations
     return (unsigned)(i < AOPS ? lw * AOPS + i : BN / 8 + lw * BOPS + i - AOPS) * 1024u;
@@ -197,26 +192,11 @@ __global__ __launch_bounds__((WN * WM + PW) * kWave) void w8a8_tile_kernel(T* y,
     const int k0 = stage_k(s);
     const bool up = SWIGLU && (((lw * AOPS + i) >> 1) & 1);  // 8 rows of an up tile
     const uint8_t* base = i < AOPS ? (up ? ubase : wbase) : xbase;
-    const unsigned to = lds0 + (unsigned)(s % D) * kStage + place(i), o = voff[DMA ? i : 0];
+    const unsigned to = lds0 + (unsigned)(s % D) * kStage + place(i), o = voff[i];
     if (k0 + kStep <= K)
       dma16<false>(base + k0, o, to);
     else  // pieces past K: the row's start
       dma16<false>(base, k0 + off[i] < K ? o + (unsigned)k0 : o - (unsigned)off[i], to);
-  };
-  u32x4 held[DMA ? 1 : 2][DMA ? 1 : OPS];
-  auto fetch = [&](int s, auto h) {  // stage s into registers
-    const int k0 = stage_k(s);
-    if (k0 + kStep <= K) {
-#pragma unroll
-      for (int i = 0; i < OPS; ++i) held[h][DMA ? 0 : i] = load16_any(src[DMA ? 0 : i] + k0 + off[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < OPS; ++i) held[h][DMA ? 0 : i] = load16_end(src[DMA ? 0 : i], k0 + off[i], K);
-    }
-  };
-  auto put = [&](int s, auto h) {  // and on into LDS
-#pragma unroll
-    for (int i = 0; i < OPS; ++i) w8_smem[((s % D) * kStage + place(i)) / 16 + lane] = held[h][DMA ? 0 : i];
   };
   auto zero_tail = [&](int s) {  // DMA past K brought the row's start: the activations there become zero
     const int k0 = stage_k(s);
@@ -239,63 +219,35 @@ __global__ __launch_bounds__((WN * WM + PW) * kWave) void w8a8_tile_kernel(T* y,
   // The loads of a stage and its waits, by the waves that load: all of them, or PW of their own
   // whose DMAs, each of which holds its wave for over a hundred cycles, then hold no MFMA.
   auto load_first = [&]() {
-    if constexpr (DMA) {
-      const int pre = ns < D ? ns : D;
-      for (int s = 0; s < pre; ++s)
+    const int pre = ns < D ? ns : D;
+    for (int s = 0; s < pre; ++s)
 #pragma unroll
-        for (int i = 0; i < OPS; ++i) issue_one(s, i);
-      if (ns >= D)
-        wait_vm<OPS*(D - 1)>();
-      else
-        wait_vm<0>();
-      zero_tail(0);
-    }
+      for (int i = 0; i < OPS; ++i) issue_one(s, i);
+    if (ns >= D)
+      wait_vm<OPS*(D - 1)>();
+    else
+      wait_vm<0>();
+    zero_tail(0);
   };
   auto wait_next = [&](int s) {  // stage s + 1 has landed
-    if constexpr (DMA) {
-      if (s + D <= ns)  // issued so far: to stage s + D - 1
-        wait_vm<OPS*(D - 2)>();
-      else
-        wait_vm<0>();
-      if (s + 1 < ns) zero_tail(s + 1);
-    }
+    if (s + D <= ns)             // issued so far: to stage s + D - 1
+      wait_vm<OPS*(D - 2)>();
+    else
+      wait_vm<0>();
+    if (s + 1 < ns) zero_tail(s + 1);
   };
   if constexpr (PW > 0) {
     if (wave >= NW) {
-      if constexpr (DMA) {
-        if (ns > 0) {
-          load_first();
-          lds_barrier();
-        }
-        for (int s = 0; s < ns; ++s) {
-          wait_next(s);
-          lds_barrier();
-          if (s + D < ns) {
-#pragma unroll
-            for (int i = 0; i < OPS; ++i) issue_one(s + D, i);
-          }
-        }
-      } else if (ns > 0) {
-        // stages go into LDS as their buffers come free, two ahead of that in registers
-        const std::integral_constant<int, 0> even{};
-        const std::integral_constant<int, 1> odd{};
-        fetch(0, even);
-        if (ns > 1) fetch(1, odd);
-        put(0, even);
-        if (ns > 2) fetch(2, even);
-        if (ns > 1) put(1, odd);
-        if (ns > 3) fetch(3, odd);
-        if (ns > 2) put(2, even);
-        if (ns > 4) fetch(4, even);
+      if (ns > 0) {
+        load_first();
         lds_barrier();
-        auto step = [&](int s, auto h) {  // of stage s: s + 3 into its buffer
-          lds_barrier();
-          if (s + 3 < ns) put(s + 3, h);
-          if (s + 5 < ns) fetch(s + 5, h);
-        };
-        for (int s = 0; s < ns; s += 2) {
-          step(s, odd);
-          if (s + 1 < ns) step(s + 1, even);
+      }
+      for (int s = 0; s < ns; ++s) {
+        wait_next(s);
+        lds_barrier();
+        if (s + D < ns) {
+#pragma unroll
+          for (int i = 0; i < OPS; ++i) issue_one(s + D, i);
         }
       }
       return;  // a wave that has ended is not waited for at a barrier
@@ -517,7 +469,10 @@ __global__ __launch_bounds__(256) void w8a8_sum_kernel(T* y, const float* part, 
 
 namespace {
 
-template <typename T, int PW, int WN, int WM, int NT, int MT, int D, bool SWIGLU, int FORM, bool DMA>
+constexpr int64_t kMostIndex = 0x7fffffffLL - 512;  // indexes run to the end of the last tile and stage
+constexpr int64_t kMostStride = 1 << 23;            // 256 rows of it, and a row, are below 2^32 bytes
+
+template <typename T, int PW, int WN, int WM, int NT, int MT, int D, bool SWIGLU, int FORM>
 int tile_launch(const W8Args& a, int splits) {
   constexpr int BN = WN * NT * 16, BM = WM * MT * 16;
   constexpr size_t ring = (size_t)kStageBytes<BN, BM> * D;
@@ -526,7 +481,7 @@ int tile_launch(const W8Args& a, int splits) {
   static_assert(lds <= kMaxLds, "a launch fits the LDS of a CU");
   const int64_t nt = (a.N + BN - 1) / BN, mt = (a.M + BM - 1) / BM;
   if (nt * mt * splits > 0x7fffffffLL) return set_error(FD_EUNSUPPORTED, "too many tiles");
-  auto kernel = w8a8_tile_kernel<T, PW, WN, WM, NT, MT, D, SWIGLU, FORM, DMA>;
+  auto kernel = w8a8_tile_kernel<T, PW, WN, WM, NT, MT, D, SWIGLU, FORM>;
   if (!allow_lds(kernel, lds)) return set_error(FD_ELAUNCH, "cannot raise the LDS limit to %zu bytes", lds);
   hipLaunchKernelGGL(kernel, dim3((unsigned)(nt * mt * splits)), dim3((WN * WM + PW) * kWave), lds, a.st,
                      static_cast<T*>(a.y), a.scratch, a.x, a.w, a.M, a.N, a.K, a.sxm, a.swn, a.sym, a.syn, a.e, (int)mt,
@@ -541,10 +496,9 @@ struct TileForm {
   int bn, bm, per_cu;
   float stage, round;
 };
-enum { T_256 = 0, T_256x128, T_128, T_64x128, T_64, T_128x32, T_UNALIGNED, T_FORMS };
+enum { T_256 = 0, T_256x128, T_128, T_64x128, T_64, T_128x32, T_FORMS };
 constexpr TileForm kTiles[T_FORMS] = {{256, 256, 1, 1.40f, 9.f},  {256, 128, 1, 0.80f, 6.f}, {128, 128, 1, 0.58f, 5.f},
-                                      {64, 128, 1, 0.37f, 5.f},   {64, 64, 1, 0.29f, 4.5f},  {128, 32, 1, 0.33f, 4.f},
-                                      {128, 256, 1, 1.20f, 8.f}};
+                                      {64, 128, 1, 0.37f, 5.f},   {64, 64, 1, 0.29f, 4.5f},  {128, 32, 1, 0.33f, 4.f}};
 
 struct TilePlan {
   int form, splits;
@@ -552,12 +506,11 @@ struct TilePlan {
 
 // The form and the K splits (as many as give every CU one workgroup, each with at least six stages) that take the
 // least time by that table. Adding the splits' sums is a launch, and their floats go to memory and back.
-TilePlan tile_plan(int64_t M, int64_t N, int64_t K, bool dma) {
+TilePlan tile_plan(int64_t M, int64_t N, int64_t K) {
   const int64_t stages = (K + kStep - 1) / kStep, cus = device_cus();
-  TilePlan best{T_UNALIGNED, 1};
+  TilePlan best{T_128, 1};
   float least = INFINITY;
   for (int f = 0; f < T_FORMS; ++f) {
-    if (dma == (f == T_UNALIGNED)) continue;
     const TileForm& t = kTiles[f];
     const int64_t tiles = ((N + t.bn - 1) / t.bn) * ((M + t.bm - 1) / t.bm);
     int64_t most = cus / (tiles < cus ? tiles : cus);
@@ -578,13 +531,12 @@ TilePlan tile_plan(int64_t M, int64_t N, int64_t K, bool dma) {
 template <typename T, bool SWIGLU, int FORM>
 int pick_tile(const W8Args& a, TilePlan p) {
   switch (p.form) {
-    case T_256: return tile_launch<T, 0, 4, 2, 4, 8, 2, SWIGLU, FORM, true>(a, p.splits);
-    case T_256x128: return tile_launch<T, 4, 4, 2, 4, 4, 3, SWIGLU, FORM, true>(a, p.splits);
-    case T_128: return tile_launch<T, 0, 2, 4, 4, 2, 4, SWIGLU, FORM, true>(a, p.splits);
-    case T_64x128: return tile_launch<T, 0, 2, 4, 2, 2, 4, SWIGLU, FORM, true>(a, p.splits);
-    case T_64: return tile_launch<T, 4, 2, 2, 2, 2, 4, SWIGLU, FORM, true>(a, p.splits);
-    case T_128x32: return tile_launch<T, 0, 4, 1, 2, 2, 4, SWIGLU, FORM, true>(a, p.splits);
-    default: return tile_launch<T, 4, 2, 4, 4, 4, 3, SWIGLU, FORM, false>(a, p.splits);
+    case T_256: return tile_launch<T, 0, 4, 2, 4, 8, 2, SWIGLU, FORM>(a, p.splits);
+    case T_256x128: return tile_launch<T, 4, 4, 2, 4, 4, 3, SWIGLU, FORM>(a, p.splits);
+    case T_128: return tile_launch<T, 0, 2, 4, 4, 2, 4, SWIGLU, FORM>(a, p.splits);
+    case T_64x128: return tile_launch<T, 0, 2, 4, 2, 2, 4, SWIGLU, FORM>(a, p.splits);
+    case T_64: return tile_launch<T, 4, 2, 2, 2, 2, 4, SWIGLU, FORM>(a, p.splits);
+    default: return tile_launch<T, 0, 4, 1, 2, 2, 4, SWIGLU, FORM>(a, p.splits);
   }
 }
 
@@ -626,35 +578,61 @@ int short_launch(const W8Args& a) {
   return FD_OK;
 }
 
+// The rows of both operands, at any address, to rows of K rounded up to 16 bytes, dense and padded with zeros, the
+// activations' first: a thread per 16 bytes (777 x 2051 and 5003 x 2051: 6 us, where tiles loaded through registers
+// from rows off alignment took 14 more than aligned ones).
+__global__ __launch_bounds__(256) void w8a8_align_kernel(u32x4* to, const uint8_t* x, const uint8_t* w, uint32_t M,
+                                                         int64_t sxm, int64_t swn, int K, FastDiv pieces,
+                                                         uint32_t total) {
+  const uint32_t v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= total) return;
+  uint32_t piece;
+  const uint32_t row = pieces.divmod(v, piece);
+  to[v] = load16_end(row < M ? x + row * sxm : w + (row - M) * swn, (int)piece * 16, K);
+}
+
+// Copies the operands' rows into the scratch of `a`, which then starts behind them.
+int align_rows(W8Args& a) {
+  const int64_t pieces = ((int64_t)a.K + 15) / 16, total = ((int64_t)a.M + a.N) * pieces;
+  if (pieces * 16 >= kMostStride || total > 0xffffff00LL) return set_error(FD_EUNSUPPORTED, "too large to align");
+  if (a.scratch_bytes < total * 16) return set_error(FD_EUNSUPPORTED, "rows off 16-byte alignment need scratch");
+  uint8_t* const to = reinterpret_cast<uint8_t*>(a.scratch);
+  hipLaunchKernelGGL(w8a8_align_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, a.st,
+                     reinterpret_cast<u32x4*>(to), a.x, a.w, (uint32_t)a.M, a.sxm, a.swn, a.K, FastDiv((uint32_t)pieces),
+                     (uint32_t)total);
+  a.K = (int)(pieces * 16);
+  a.sxm = a.swn = a.K;
+  a.x = to;
+  a.w = to + (int64_t)a.M * a.K;
+  a.scratch += total * 4;
+  a.scratch_bytes -= total * 16;
+  return FD_OK;
+}
+
 template <typename T, bool SWIGLU>
 int product(const W8Args& a) {
   if (a.K < 16) return short_launch<T, SWIGLU>(a);
-  if (w8_few_fits(a)) return w8_few_launch(a);
-  TilePlan p = tile_plan(a.M, a.N, a.K, a.dma);
+  if (w8_few_fits(a.M, a.K)) return w8_few_launch(a);
+  TilePlan p = tile_plan(a.M, a.N, a.K);
   while (p.splits > 1 && a.scratch_bytes < (int64_t)p.splits * a.M * a.N * 4) --p.splits;
   return tiles<T, SWIGLU>(a, p);
 }
-
-constexpr int64_t kMostIndex = 0x7fffffffLL - 512;  // indexes run to the end of the last tile and stage
 
 }  // namespace
 }  // namespace fd
 
 using namespace fd;
 
-extern "C" int fd_linear_w8a8_scratch(int64_t M, int64_t N, int64_t K, int64_t* bytes) {
+extern "C" int fd_linear_w8a8_scratch(int64_t M, int64_t N, int64_t K, int aligned, int64_t* bytes) {
   if (M < 0 || N < 0 || K < 0) return set_error(FD_EINVAL, "negative size");
   if (!bytes) return set_error(FD_EINVAL, "null pointer argument");
   *bytes = 0;
   if (M == 0 || N == 0 || K < 16 || M > kMostIndex || N > kMostIndex || K > kMostIndex) return FD_OK;
-  W8Args a{};
-  a.M = (int)M;
-  a.N = (int)N;
-  a.K = (int)K;
-  a.dma = K % 16 == 0;
-  if (w8_few_fits(a)) return FD_OK;
-  const int s = tile_plan(M, N, K, a.dma).splits;
-  if (s > 1) *bytes = (int64_t)s * M * N * 4;
+  const int64_t Kp = (K + 15) / 16 * 16;
+  if (!aligned || K != Kp) *bytes = (M + N) * Kp;
+  if (w8_few_fits(M, Kp)) return FD_OK;
+  const int s = tile_plan(M, N, Kp).splits;
+  if (s > 1) *bytes += (int64_t)s * M * N * 4;
   return FD_OK;
 }
 
@@ -701,9 +679,11 @@ extern "C" int fd_linear_w8a8(void* y, const void* x8, const float* x_scale, con
   a.scratch_bytes = scratch ? scratch_bytes : 0;
   a.act_dtype = act_dtype;
   a.st = static_cast<hipStream_t>(stream);
-  // the DMAs' 32-bit offsets reach over a tile's rows
-  a.dma = K % 16 == 0 && aligned16(x8) && aligned16(w8) && (M == 1 || sxm % 16 == 0) && (N == 1 || swn % 16 == 0) &&
-          sxm < (1 << 23) && swn < (1 << 23);
+  // The DMAs take 16-byte pieces, and their 32-bit offsets reach over a tile's rows: other rows are copied first.
+  auto fits = [&](const void* p, int64_t rows, int64_t stride) {
+    return K % 16 == 0 && aligned16(p) && (rows == 1 || (stride % 16 == 0 && stride < kMostStride));
+  };
+  if (K >= 16 && !(fits(x8, M, sxm) && fits(w8, N, swn)) && align_rows(a) != FD_OK) return FD_EUNSUPPORTED;
   const int rc = act_dtype == FD_F16 ? (swiglu ? product<f16, true>(a) : product<f16, false>(a))
                                      : (swiglu ? product<bf16, true>(a) : product<bf16, false>(a));
   if (rc != FD_OK) return rc;

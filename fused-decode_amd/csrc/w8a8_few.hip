@@ -14,12 +14,7 @@
 // The run of a workgroup is N / CUs rows, to the row; a last tile shorter than 16 rows reads
 // its last row again in the lanes past it.
 //
-// Rows that are not 16-byte aligned (D = 0) have no ring: a lane loads its fragments of a tile with 16-byte loads at
-// any address, four steps at a time and two such groups ahead.
-//
 // Slot layout: 16 rows of 8 chunks of 16 bytes, chunk c at c ^ (row mod 8).
-#include <type_traits>
-
 #include "fd_w8a8.h"
 
 namespace fd {
@@ -27,7 +22,7 @@ namespace fd {
 constexpr int kFewWaves = 8;
 constexpr int kFewTiles = 16;  // tiles of a workgroup whose sums its LDS holds
 
-template <int MF, int D>  // D: 0 without a ring
+template <int MF, int D>
 constexpr size_t few_lds() {
   return (size_t)kFewWaves * D * 2048 + (size_t)2 * kFewWaves * MF * 1024 + (size_t)kFewTiles * MF * 1024;
 }
@@ -72,27 +67,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void w8a8_few_kernel(T* y, const
       ++it;
     }
   };
-  if constexpr (D > 0)
-    for (int u = 0; u < (units < D - 1 ? units : D - 1); ++u) issue(u);
-
-  // without a ring: this wave's fragments of four steps of a tile, two such groups held and on the way
-  constexpr int G = S / 4;  // groups of a tile
-  u32x4 h0[D ? 1 : 2][D ? 1 : 4], h1[D ? 1 : 2][D ? 1 : 4];
-  auto fetch = [&](int t, int group, auto h) {
-    const int q = t * Q + (SWIGLU ? r & 7 : r), o = o0 + q < o1 ? o0 + q : o1 - 1;
-    const uint8_t* p = w + (o + (int64_t)(SWIGLU && r >= 8 ? half : 0)) * swn;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int step = (group * 4 + s) * NW + wave, k = step * kStep + g * 16;
-      if ((step + 1) * kStep <= K) {
-        h0[h][D ? 0 : s] = load16_any(p + k);
-        h1[h][D ? 0 : s] = load16_any(p + k + 64);
-      } else {
-        h0[h][D ? 0 : s] = load16_end(p, k, K);
-        h1[h][D ? 0 : s] = load16_end(p, k + 64, K);
-      }
-    }
-  };
+  for (int u = 0; u < (units < D - 1 ? units : D - 1); ++u) issue(u);
 
   // this wave's activations: step s, rows r of each 16, the two 16-byte pieces of group g
   u32x4 b0[MF][S], b1[MF][S];
@@ -104,63 +79,36 @@ __global__ __launch_bounds__(kFewWaves * kWave) void w8a8_few_kernel(T* y, const
     for (int s = 0; s < S; ++s) {
       const int k = (s * NW + wave) * kStep + g * 16;
       const u32x4 z = {0u, 0u, 0u, 0u};
-      if constexpr (D > 0) {
-        b0[f][s] = k < K ? *reinterpret_cast<const u32x4*>(p + k) : z;
-        b1[f][s] = k + 64 < K ? *reinterpret_cast<const u32x4*>(p + k + 64) : z;
-      } else if ((s * NW + wave + 1) * kStep <= K) {
-        b0[f][s] = load16_any(p + k);
-        b1[f][s] = load16_any(p + k + 64);
-      } else {
-        b0[f][s] = load16_end(p, k, K);
-        b1[f][s] = load16_end(p, k + 64, K);
-      }
+      b0[f][s] = k < K ? *reinterpret_cast<const u32x4*>(p + k) : z;
+      b1[f][s] = k + 64 < K ? *reinterpret_cast<const u32x4*>(p + k + 64) : z;
     }
   }
   // all of it has landed here (the first units' weights with it), so that no wait of the compiler's
   // for an activation stands in the loop
-  if constexpr (D > 0) __builtin_amdgcn_s_waitcnt(0x0f70);
+  __builtin_amdgcn_s_waitcnt(0x0f70);
 
   const int c0 = r * 8 + (g ^ (r & 7)), c1 = r * 8 + ((4 + g) ^ (r & 7));
   int u = 0, slot = 0;
-  auto tile = [&](int t, auto h) {
+  for (int t = 0; t < tiles; ++t) {
     f32x4 acc[MF];
 #pragma unroll
     for (int f = 0; f < MF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if constexpr (D == 0) {
-      auto group = [&](auto gi) {
-        const std::integral_constant<int, G == 1 ? decltype(h)::value : decltype(gi)::value & 1> b{};
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < S; ++s) {
+      if (s < sn) {
+        if (u + D - 1 <= units)
+          wait_vm<2 * (D - 2)>();
+        else
+          wait_vm<0>();
+        const u32x4* p = ring + slot * 128;
+        const u32x4 a0 = p[c0], a1 = p[c1];
 #pragma unroll
-          for (int f = 0; f < MF; ++f)
-            acc[f] = mfma_e4m3(h0[b][s], h1[b][s], b0[f][gi * 4 + s], b1[f][gi * 4 + s], acc[f]);
-        const int next = gi + 2;
-        if (t + next / G < tiles) fetch(t + next / G, next % G, b);
-      };
-      group(std::integral_constant<int, 0>{});
-      if constexpr (G >= 2) group(std::integral_constant<int, 1>{});
-      if constexpr (G == 4) {
-        group(std::integral_constant<int, 2>{});
-        group(std::integral_constant<int, 3>{});
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        if (s < sn) {
-          if (u + D - 1 <= units)
-            wait_vm<2 * (D > 0 ? D - 2 : 0)>();
-          else
-            wait_vm<0>();
-          const u32x4* p = ring + slot * 128;
-          const u32x4 a0 = p[c0], a1 = p[c1];
-#pragma unroll
-          for (int f = 0; f < MF; ++f) acc[f] = mfma_e4m3(a0, a1, b0[f][s], b1[f][s], acc[f]);
-          // the unit before this one has been read: its slot takes the next
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          if (u + D - 1 < units) issue(slot == 0 ? D - 1 : slot - 1);
-          ++u;
-          slot = slot == D - 1 ? 0 : slot + 1;
-        }
+        for (int f = 0; f < MF; ++f) acc[f] = mfma_e4m3(a0, a1, b0[f][s], b1[f][s], acc[f]);
+        // the unit before this one has been read: its slot takes the next
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (u + D - 1 < units) issue(slot == 0 ? D - 1 : slot - 1);
+        ++u;
+        slot = slot == D - 1 ? 0 : slot + 1;
       }
     }
     f32x4* pp = parts + ((t & 1) * NW + wave) * MF * kWave + lane;
@@ -177,16 +125,6 @@ __global__ __launch_bounds__(kFewWaves * kWave) void w8a8_few_kernel(T* y, const
         done[(t * MF + f) * kWave + lane] = v;
       }
     }
-  };
-  const std::integral_constant<int, 0> even{};
-  const std::integral_constant<int, 1> odd{};
-  if constexpr (D == 0) {
-    fetch(0, 0, even);
-    if (G > 1 || tiles > 1) fetch(G > 1 ? 0 : 1, G > 1 ? 1 : 0, odd);
-  }
-  for (int t = 0; t < tiles; t += 2) {
-    tile(t, even);
-    if (t + 1 < tiles) tile(t + 1, odd);
   }
   lds_barrier();
   // sum of weight row `row` of tile t and activation row m
@@ -218,36 +156,28 @@ int few_go(const W8Args& a) {
   return FD_OK;
 }
 
-int few_steps(int K) { return ((K + kStep - 1) / kStep + kFewWaves - 1) / kFewWaves; }  // of a wave
+int few_steps(int64_t K) { return (int)(((K + kStep - 1) / kStep + kFewWaves - 1) / kFewWaves); }  // of a wave
 
-template <typename T, bool SWIGLU, bool DMA>
+template <typename T, bool SWIGLU>
 int few_pick(const W8Args& a) {
-  constexpr int D1 = DMA ? 7 : 0, D2 = DMA ? 6 : 0;
   const int s = few_steps(a.K);
   if (a.M <= 16) {
-    if (s <= 4) return few_go<T, 1, 4, D1, SWIGLU>(a);
-    if (!DMA || s <= 8) return few_go<T, 1, 8, D1, SWIGLU>(a);
-    return few_go<T, 1, DMA ? 16 : 8, D1, SWIGLU>(a);
+    if (s <= 4) return few_go<T, 1, 4, 7, SWIGLU>(a);
+    if (s <= 8) return few_go<T, 1, 8, 7, SWIGLU>(a);
+    return few_go<T, 1, 16, 7, SWIGLU>(a);
   }
-  if (!DMA || s <= 4) return few_go<T, 2, 4, D2, SWIGLU>(a);
-  return few_go<T, 2, DMA ? 8 : 4, D2, SWIGLU>(a);
-}
-
-template <typename T>
-int few_form(const W8Args& a) {
-  if (a.dma) return a.swiglu ? few_pick<T, true, true>(a) : few_pick<T, false, true>(a);
-  return a.swiglu ? few_pick<T, true, false>(a) : few_pick<T, false, false>(a);
+  if (s <= 4) return few_go<T, 2, 4, 6, SWIGLU>(a);
+  return few_go<T, 2, 8, 6, SWIGLU>(a);
 }
 
 }  // namespace
 
-bool w8_few_fits(const W8Args& a) {
-  // the activations' registers, and without a ring the weights'
-  return a.M <= 16 ? few_steps(a.K) <= (a.dma ? 16 : 8) : a.M <= 32 && few_steps(a.K) <= (a.dma ? 8 : 4);
-}
+// Whether the activations fit the registers.
+bool w8_few_fits(int64_t M, int64_t K) { return M <= 16 ? few_steps(K) <= 16 : M <= 32 && few_steps(K) <= 8; }
 
 int w8_few_launch(const W8Args& a) {
-  return a.act_dtype == FD_F16 ? few_form<f16>(a) : few_form<bf16>(a);
+  if (a.act_dtype == FD_F16) return a.swiglu ? few_pick<f16, true>(a) : few_pick<f16, false>(a);
+  return a.swiglu ? few_pick<bf16, true>(a) : few_pick<bf16, false>(a);
 }
 
 }  // namespace fd

@@ -99,7 +99,7 @@ SIGNATURES: dict[str, list] = {
     "fd_rms_norm_fp8": [_p, _p, _p, _p, _i, _l, _rows, _f, _i, _p],
     "fd_add_rms_norm_fp8": [_p, _p, _p, _p, _p, _p, _i, _l, _rows, _rows, _rows, _f, _i, _p],
     "fd_linear_w8a8": [_p, _p, _p, _p, _p, _p, _i, _i, _p, _i, _l, _l, _l, _l, _l, _l, _l, _l, _l, _l, _p, _l, _i, _p],
-    "fd_linear_w8a8_scratch": [_l, _l, _l, ctypes.POINTER(_l)],
+    "fd_linear_w8a8_scratch": [_l, _l, _l, _i, ctypes.POINTER(_l)],
     "fd_copy": [_p, _p, _l, _p],
     "fd_copy_persistent": [_p, _p, _l, _i, _p],
     "fd_clock_probe": [_p, _i, ctypes.POINTER(ctypes.c_int), _p],
@@ -188,10 +188,11 @@ def fail(func: str, status: int) -> None:
     raise FusedDecodeError(func, status, native().last_error())
 
 
-def scratch_bytes(func: str, m: int, n: int, k: int) -> int:
-    """Bytes of scratch the preferred K split of an [M, N, K] product takes (``func``: a *_scratch entry point)."""
+def scratch_bytes(func: str, m: int, n: int, k: int, *more: int) -> int:
+    """Bytes of scratch that an [M, N, K] product prefers (``func``: a *_scratch entry point, ``more`` its further
+    arguments)."""
     out = ctypes.c_int64(0)
-    check(func, getattr(lib(), func)(m, n, k, ctypes.byref(out)))
+    check(func, getattr(lib(), func)(m, n, k, *more, ctypes.byref(out)))
     return out.value
 
 

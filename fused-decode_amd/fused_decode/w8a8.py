@@ -49,23 +49,18 @@ __all__ = ["add_rms_norm_fp8", "linear_w8a8", "quantize_rows_fp8", "rms_norm_fp8
 
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else (lambda: -1)
 _grad = torch.is_grad_enabled
+_MOST_STRIDE = 1 << 23  # bytes between rows that the product's kernels take as they are; others are copied
 
 
-def _recorded(*tensors) -> bool:
-    """Whether something records or transforms a call on these tensors (None: absent), which a launch
-    on their pointers would be missing from."""
-    if (torch.compiler.is_compiling() or forward_ad._current_level >= 0 or _transform() is not None or _is_tracing()
-            or _dispatch_modes() or (_function_modes() and _function_modes_watch())):
-        return True
-    return _grad() and any(t is not None and t.requires_grad for t in tensors)
+def _watched() -> bool:
+    """Whether something would record or transform a call, which a launch on bare pointers would be missing from."""
+    return bool(torch.compiler.is_compiling() or forward_ad._current_level >= 0 or _transform() is not None
+                or _is_tracing() or _dispatch_modes() or (_function_modes() and _function_modes_watch()))
 
 
-def _on(dev: int, call, *args) -> int:
-    """``call(*args, stream)`` with ``dev`` current: a launch on the default stream goes to the current device."""
-    if _current_device() == dev:
-        return call(*args, _raw_stream(dev))
-    with torch.cuda.device(dev):
-        return call(*args, _raw_stream(dev))
+def _like(shape: tuple, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """What ``torch.empty_like`` makes a contiguous ``shape`` of, in the least host time: one element, expanded."""
+    return torch.empty((), dtype=dtype, device=device).expand(shape)
 
 
 # ------------------------------------------------------------------ rows to codes
@@ -79,7 +74,17 @@ def quantize_rows_fp8(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """E4M3 codes of ``x``'s rows (its last dimension) and their float32 scales ``x.shape[:-1]``, in one
     launch. For finite rows the codes and scales that ``quantize_fp8`` gives the same rows."""
-    return _rows("quantize_rows_fp8", x, None, None, 0.0, out, scale_out, None)
+    try:
+        if _watched() or (_grad() and x.requires_grad):
+            return _copied(torch.ops.fused_decode.quantize_rows_fp8(x), out, scale_out)
+        key = ("quantize_rows_fp8", x.shape, x.stride(), x.dtype, x.get_device(), None if out is None else _sig(out),
+               None if scale_out is None else _sig(scale_out))
+        plan = _PLANS.get(key)
+    except AttributeError:  # not a tensor: let the contract say so
+        key, plan = None, None
+    if plan is None:
+        plan = _remember(key, _plan_rows_fp8("quantize_rows_fp8", x, None, None, 0.0, out, scale_out, None))
+    return plan(x, None, None, out, scale_out, None)
 
 
 def rms_norm_fp8(
@@ -92,7 +97,18 @@ def rms_norm_fp8(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """``rms_norm`` with E4M3 codes and float32 row scales for its result. ``weight`` is ``(N,)``
     (float16, bfloat16 or float32)."""
-    return _rows("rms_norm_fp8", x, weight, None, eps, out, scale_out, None)
+    try:
+        if _watched() or (_grad() and (x.requires_grad or weight.requires_grad)):
+            return _copied(torch.ops.fused_decode.rms_norm_fp8(x, weight, eps), out, scale_out)
+        key = ("rms_norm_fp8", x.shape, x.stride(), x.dtype, x.get_device(), weight.shape, weight.stride(), weight.dtype,
+               weight.get_device(), eps, None if out is None else _sig(out),
+               None if scale_out is None else _sig(scale_out))
+        plan = _PLANS.get(key)
+    except (AttributeError, TypeError):  # a non-tensor or unhashable argument: checked below
+        key, plan = None, None
+    if plan is None:
+        plan = _remember(key, _plan_rows_fp8("rms_norm_fp8", x, weight, None, eps, out, scale_out, None))
+    return plan(x, weight, None, out, scale_out, None)
 
 
 def add_rms_norm_fp8(
@@ -107,34 +123,29 @@ def add_rms_norm_fp8(
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``add_rms_norm`` with E4M3 codes and float32 row scales for the norm of the float32 sum:
     ``(codes, scale, residual_out)``. ``residual_out=residual`` updates the residual stream in place."""
-    return _rows("add_rms_norm_fp8", x, weight, residual, eps, out, scale_out, residual_out)
-
-
-def _rows(op, x, weight, residual, eps, out, scale_out, residual_out):
     try:
-        if _recorded(x, weight, residual):
-            return _rows_op(op, x, weight, residual, eps, out, scale_out, residual_out)
-        key = (op, x.shape, x.stride(), x.dtype, x.get_device(), _sig(weight), _sig(residual), eps, _sig(out),
-               _sig(scale_out), _sig(residual_out))
+        if _watched() or (_grad() and (x.requires_grad or residual.requires_grad or weight.requires_grad)):
+            return _copied(torch.ops.fused_decode.add_rms_norm_fp8(x, residual, weight, eps), out, scale_out, residual_out)
+        key = ("add_rms_norm_fp8", x.shape, x.stride(), x.dtype, x.get_device(), residual.shape, residual.stride(),
+               residual.dtype, residual.get_device(), weight.shape, weight.stride(), weight.dtype, weight.get_device(),
+               eps, None if out is None else _sig(out), None if scale_out is None else _sig(scale_out),
+               None if residual_out is None else _sig(residual_out))
         plan = _PLANS.get(key)
-    except (AttributeError, TypeError):  # a non-tensor or unhashable argument: checked below
+    except (AttributeError, TypeError):
         key, plan = None, None
     if plan is None:
-        plan = _remember(key, _plan_rows_fp8(op, x, weight, residual, eps, out, scale_out, residual_out))
+        plan = _remember(key, _plan_rows_fp8("add_rms_norm_fp8", x, weight, residual, eps, out, scale_out, residual_out))
     return plan(x, weight, residual, out, scale_out, residual_out)
 
 
-def _rows_op(op, x, weight, residual, eps, out, scale_out, residual_out):
-    """The custom op of the same name, its results copied where outputs are given."""
-    f = getattr(torch.ops.fused_decode, op)
-    got = (f(x) if op == "quantize_rows_fp8" else f(x, weight, eps) if op == "rms_norm_fp8" else
-           f(x, residual, weight, eps))
-    return tuple(v if o is None else o.copy_(v) for v, o in zip(got, (out, scale_out, residual_out)))
+def _copied(got: tuple, *outs) -> tuple:
+    """A custom op's results, copied where outputs are given."""
+    return tuple(v if o is None else o.copy_(v) for v, o in zip(got, outs))
 
 
 def _plan_rows_fp8(op, x, weight, residual, eps, out, scale_out, residual_out):
     """Launch plan of a row operator for one argument signature."""
-    add, norm = residual is not None or op == "add_rms_norm_fp8", op != "quantize_rows_fp8"
+    add, norm = op == "add_rms_norm_fp8", op != "quantize_rows_fp8"
     args = dict(x=x, out=out, scale_out=scale_out)
     if norm:
         args.update(weight=weight, eps=eps)
@@ -142,51 +153,65 @@ def _plan_rows_fp8(op, x, weight, residual, eps, out, scale_out, residual_out):
         args.update(residual=residual, residual_out=residual_out)
     eps = check(op, **args).get("eps", 0.0)
     shape, lead, device = tuple(x.shape), tuple(x.shape[:-1]), x.device
-    n, act, dev = shape[-1], DTYPE_CODE[x.dtype], x.device.index
-    dense = contiguous_strides(shape)
-    strides = [tuple(x.stride())]
-    if add:
-        strides += [tuple(residual.stride()), dense if residual_out is None else tuple(residual_out.stride())]
-    # more than three unmergeable leading dims: the rows are gathered, and written back
-    layouts = plan_rows(shape, strides) if n and math.prod(lead) else None
-    staged = layouts is None
-    if staged:
-        layouts = [bytes(FdRows(1, 1, math.prod(lead), 0, 0, n, 1, n))] * len(strides)
-    name = "fd_" + op
-    call = getattr(native(), op)
-    wcode, wstride = (DTYPE_CODE[weight.dtype], int(weight.stride(0)) if n > 1 else 1) if norm else (act, 1)
-
-    def run(x, w, r, out, scale_out, residual_out):
-        c = torch.empty(shape, dtype=FP8_DTYPE, device=device) if out is None else out
-        s = torch.empty(lead, dtype=torch.float32, device=device) if scale_out is None else scale_out
-        if staged:
-            x = x.contiguous()
-        if not add:
-            if norm:
-                status = _on(dev, call, c.data_ptr(), s.data_ptr(), x.data_ptr(), w.data_ptr(), wcode, wstride,
-                             layouts[0], eps, act)
-            else:
-                status = _on(dev, call, c.data_ptr(), s.data_ptr(), x.data_ptr(), layouts[0], act)
-            if status:
-                fail(name, status)
-            return c if out is None else _written(out), s if scale_out is None else _written(scale_out)
-        ro = torch.empty(shape, dtype=x.dtype, device=device) if residual_out is None or staged else residual_out
-        if staged:
-            r = r.contiguous()
-        status = _on(dev, call, c.data_ptr(), s.data_ptr(), ro.data_ptr(), x.data_ptr(), r.data_ptr(), w.data_ptr(),
-                     wcode, wstride, layouts[0], layouts[1], layouts[2], eps, act)
-        if status:
-            fail(name, status)
-        if residual_out is not None:
-            ro = residual_out.copy_(ro) if staged else _written(residual_out)
-        return c if out is None else _written(out), s if scale_out is None else _written(scale_out), ro
-
-    if math.prod(lead) == 0 or n == 0:  # no value to compute: a row of none has scale 1
+    n, act, dev, rows = shape[-1], DTYPE_CODE[x.dtype], x.device.index, math.prod(lead)
+    if rows == 0 or n == 0:  # no value to compute: a row of none has scale 1
         def empty(x, w, r, out, scale_out, residual_out):
             c = torch.empty(shape, dtype=FP8_DTYPE, device=device) if out is None else out
             s = torch.ones(lead, dtype=torch.float32, device=device) if scale_out is None else scale_out.fill_(1.0)
             return (c, s, torch.empty_like(x) if residual_out is None else residual_out) if add else (c, s)
         return empty
+
+    codes_like, scale_like = _like(shape, FP8_DTYPE, device), _like(lead, torch.float32, device)
+    dense = contiguous_strides(shape)
+    strides = [tuple(x.stride())]
+    if add:
+        strides += [tuple(residual.stride()), dense if residual_out is None else tuple(residual_out.stride())]
+    layouts = plan_rows(shape, strides)
+    staged = layouts is None  # more than three unmergeable leading dims: the rows are gathered, and written back
+    if staged:
+        layouts = [bytes(FdRows(1, 1, rows, 0, 0, n, 1, n))] * len(strides)
+    call = getattr(native(), op)
+    wcode, wstride = (DTYPE_CODE[weight.dtype], int(weight.stride(0)) if n > 1 else 1) if norm else (act, 1)
+    lx = layouts[0]
+
+    if add:
+        lr, lro = layouts[1:]
+        sum_like = _like(shape, x.dtype, device)
+
+        def run_add(x, w, r, out, scale_out, residual_out):
+            if _current_device() != dev:  # a launch on the default stream goes to the current device
+                with torch.cuda.device(dev):
+                    return run_add(x, w, r, out, scale_out, residual_out)
+            c = torch.empty_like(codes_like) if out is None else out
+            s = torch.empty_like(scale_like) if scale_out is None else scale_out
+            ro = torch.empty_like(sum_like) if residual_out is None or staged else residual_out
+            if staged:
+                x, r = x.contiguous(), r.contiguous()
+            status = call(c.data_ptr(), s.data_ptr(), ro.data_ptr(), x.data_ptr(), r.data_ptr(), w.data_ptr(), wcode,
+                          wstride, lx, lr, lro, eps, act, _raw_stream(dev))
+            if status:
+                fail("fd_add_rms_norm_fp8", status)
+            if residual_out is not None:
+                ro = residual_out.copy_(ro) if staged else _written(residual_out)
+            return c if out is None else _written(out), s if scale_out is None else _written(scale_out), ro
+        return run_add
+
+    def run(x, w, r, out, scale_out, residual_out):
+        if _current_device() != dev:
+            with torch.cuda.device(dev):
+                return run(x, w, r, out, scale_out, residual_out)
+        c = torch.empty_like(codes_like) if out is None else out
+        s = torch.empty_like(scale_like) if scale_out is None else scale_out
+        if staged:
+            x = x.contiguous()
+        if norm:
+            status = call(c.data_ptr(), s.data_ptr(), x.data_ptr(), w.data_ptr(), wcode, wstride, lx, eps, act,
+                          _raw_stream(dev))
+        else:
+            status = call(c.data_ptr(), s.data_ptr(), x.data_ptr(), lx, act, _raw_stream(dev))
+        if status:
+            fail("fd_" + op, status)
+        return c if out is None else _written(out), s if scale_out is None else _written(scale_out)
     return run
 
 
@@ -212,15 +237,19 @@ def linear_w8a8(
     ``activation`` is None, "relu", "silu", "gelu" (with erf), "gelu_tanh" or "swiglu", which takes gate rows
     above up rows (``weight [2I, K]``, ``bias [2I]``) and returns ``silu(gate) * up`` ``[..., I]``. ``bias`` and
     ``row_add`` have any float dtype; ``row_add`` broadcasts to the output and is added after the activation.
-    Any number of rows and any K; rows of codes that are not 16-byte aligned and K that is no multiple of 16
-    take a slower kernel, and codes without unit stride along K are gathered first."""
+    Any number of rows and any K; codes whose rows are not 16-byte aligned, whose K is no multiple of 16 or
+    whose stride along K is not 1 are copied first."""
     try:
-        if _recorded(x, x_scale, weight, scale, bias, row_add):
+        if _watched() or (_grad() and (x_scale.requires_grad or scale.requires_grad or x.requires_grad
+                                       or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                       or (row_add is not None and row_add.requires_grad))):
             y = torch.ops.fused_decode.linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add,
                                                    dtype or (torch.bfloat16 if out is None else out.dtype))
             return y if out is None else out.copy_(y)
-        key = ("linear_w8a8", x.shape, x.stride(), x.dtype, x.get_device(), _sig(x_scale), _sig(weight), _sig(scale),
-               _sig(bias), activation, _sig(row_add), _sig(out), dtype)
+        key = ("linear_w8a8", x.shape, x.stride(), x.dtype, x.get_device(), x_scale.shape, x_scale.stride(), x_scale.dtype,
+               x_scale.get_device(), weight.shape, weight.stride(), weight.dtype, weight.get_device(), scale.shape,
+               scale.stride(), scale.dtype, scale.get_device(), None if bias is None else _sig(bias), activation,
+               None if row_add is None else _sig(row_add), None if out is None else _sig(out), dtype)
         plan = _PLANS.get(key)
     except (AttributeError, TypeError):  # a non-tensor or unhashable argument: checked below
         key, plan = None, None
@@ -254,10 +283,18 @@ def _plan_linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add, out,
     srm, srn, r_flat = ra if ra is not None else (0, 0, False)
     call = native().linear_w8a8
     with torch.cuda.device(dev):
-        scratch_bytes = _lib.scratch_bytes("fd_linear_w8a8_scratch", m, n, k)
+        sizes = [_lib.scratch_bytes("fd_linear_w8a8_scratch", m, n, k, aligned) for aligned in (0, 1)]
+    like = _like(expected, dtype, device)
+    # by whether the rows are 16-byte aligned, which the pointers say call by call
+    scratch = [(_like((size // 4,), torch.float32, device), size) if size else (None, 0) for size in sizes]
+    if k % 16 or any(rows > 1 and (step % 16 or step >= _MOST_STRIDE) for rows, step in ((m, sxm), (n, swn))):
+        scratch[1] = scratch[0]
 
     def run(x, xs, w, ws, b, r, o):
-        y = torch.empty(expected, dtype=dtype, device=device) if o is None else o
+        if _current_device() != dev:  # a launch on the default stream goes to the current device
+            with torch.cuda.device(dev):
+                return run(x, xs, w, ws, b, r, o)
+        y = torch.empty_like(like) if o is None else o
         if x_copy:
             x = x.reshape(m, k).contiguous()
         if w_copy:
@@ -266,14 +303,16 @@ def _plan_linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add, out,
             xs, ws = xs.contiguous(), ws.contiguous()
         if r_flat:
             r = r.expand(expected).reshape(m, nout)
-        part = torch.empty(scratch_bytes, dtype=torch.uint8, device=device) if scratch_bytes else None
-        args = (x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), None if b is None else b.data_ptr(), bcode, act,
+        xp, wp = x.data_ptr(), w.data_ptr()
+        part_like, part_bytes = scratch[0 if (xp | wp) & 15 else 1]
+        part = None if part_like is None else torch.empty_like(part_like)
+        args = (xp, xs.data_ptr(), wp, ws.data_ptr(), None if b is None else b.data_ptr(), bcode, act,
                 None if r is None else r.data_ptr(), rcode, m, n, k, sxm, swn, sb, srm, srn, nout, 1,
-                None if part is None else part.data_ptr(), scratch_bytes, code)
-        status = _on(dev, call, y.data_ptr(), *args)
+                None if part is None else part.data_ptr(), part_bytes, code, _raw_stream(dev))
+        status = call(y.data_ptr(), *args)
         if status == FD_EUNSUPPORTED and o is not None:  # `out` may lie over an operand: write beside it
-            beside = torch.empty(expected, dtype=dtype, device=device)
-            status = _on(dev, call, beside.data_ptr(), *args)
+            beside = torch.empty_like(like)
+            status = call(beside.data_ptr(), *args)
             if status == 0:
                 return o.copy_(beside)
         if status:

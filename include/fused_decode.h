@@ -460,19 +460,20 @@ int fd_add_rms_norm_fp8(void* codes, float* scale, void* residual_out, const voi
  *   y[m,j] = round(silu(v[m,j]) * v[m,I+j] + row_add[m,j])
  * Sums and the epilogue are float32 with one rounding. bias (N values at stride sb) and
  * row_add (strides srm, srn; 0 broadcasts) have any of the three dtypes and may be NULL; y has
- * act_dtype. Rows that are not 16-byte aligned, or K % 16 != 0, take a slower kernel. Few
- * output tiles split K over workgroups whose float32 sums go through `scratch` (16-byte
- * aligned, caller-owned, not shared with a call that may overlap) and are added in a fixed
- * order; fd_linear_w8a8_scratch gives the bytes of the preferred split (0: none), less lowers
- * it, down to none with scratch NULL. y may be row_add element for element and overlaps no
- * operand otherwise (FD_EUNSUPPORTED). No reference counterpart.
+ * act_dtype. `scratch` (16-byte aligned, caller-owned, not shared with a call that may
+ * overlap) holds what fd_linear_w8a8_scratch says (0: none; `aligned`: whether the rows of
+ * both operands are 16-byte aligned, as row strides and pointers that are multiples of 16
+ * make them): copies of rows that are not, or whose K is no multiple of 16 (without it
+ * FD_EUNSUPPORTED), and, where there are few output tiles, the float32 sums of K splits, which are added in a
+ * fixed order; less lowers the split, down to none. y may be row_add element for element and
+ * overlaps no operand otherwise (FD_EUNSUPPORTED). No reference counterpart.
  */
 int fd_linear_w8a8(void* y, const void* x8, const float* x_scale, const void* w8,
                    const float* w_scale, const void* bias, int bias_dtype, int activation,
                    const void* row_add, int row_dtype, int64_t M, int64_t N, int64_t K, int64_t sxm,
                    int64_t swn, int64_t sb, int64_t srm, int64_t srn, int64_t sym, int64_t syn,
                    float* scratch, int64_t scratch_bytes, int act_dtype, void* stream);
-int fd_linear_w8a8_scratch(int64_t M, int64_t N, int64_t K, int64_t* bytes);
+int fd_linear_w8a8_scratch(int64_t M, int64_t N, int64_t K, int aligned, int64_t* bytes);
 
 /*
  * Bandwidth roofs. dst = src over `bytes` bytes (any size; 16-byte aligned
