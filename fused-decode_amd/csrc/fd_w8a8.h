@@ -39,14 +39,9 @@ __device__ __forceinline__ f32x4 mfma_e4m3(const u32x4& a0, const u32x4& a1, con
 // reusing a value of its own across the asm.)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-template <bool NT>
 __device__ __forceinline__ void dma16(const uint8_t* base, unsigned off, unsigned lds) {
-  if constexpr (NT)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base)
-                 : "memory", "m0");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
-                 : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
+               : "memory", "m0");
 }
 // The same from a pointer a lane, nontemporal.
 __device__ __forceinline__ void dma16_ptr(const uint8_t* src, unsigned lds) {
@@ -99,9 +94,11 @@ __device__ __forceinline__ float times_sigmoid(float v, float u) {
 // v (1 + erf(v / sqrt 2)) / 2. The lower tail of the normal distribution at -|v| is exp(-v^2 / 2) t P(t) with
 // t = 1 / (1 + |v| / sqrt 8) and P a polynomial fitted to exp(z^2) erfc(z) / (2 t), z = |v| / sqrt 2, with a relative
 // error below 5e-8 for z <= 13 (past that the exponential is 0): relative accuracy on both sides, no branch and few
-// instructions, where erfc's code alone was most of a kernel.
+// instructions, where erfc's code alone was most of a kernel. The tail's |v| stops short of infinity, so that an
+// infinity's is 0.
 __device__ __forceinline__ float gelu(float v) {
-  const float t = __builtin_amdgcn_rcpf(1.f + 0.35355339f * fabsf(v));
+  const float a = fminf(fabsf(v), 1e18f);
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.35355339f * a);
   float p = -0.0296934061f;
   p = p * t + 0.14306283f;
   p = p * t - 0.24520494f;
@@ -111,8 +108,8 @@ __device__ __forceinline__ float gelu(float v) {
   p = p * t + 0.121417411f;
   p = p * t + 0.141206071f;
   p = p * t + 0.141042158f;
-  const float tail = v * (__expf(-0.5f * v * v) * t * p);
-  return v < 0.f ? tail : v - tail;
+  const float tail = a * (__expf(-0.5f * a * a) * t * p);
+  return v < 0.f ? -tail : v - tail;
 }
 
 // Values at once, so that the choice is made once. 0.5 (1 + tanh(u)) is sigmoid(2 u).

@@ -103,12 +103,12 @@ typedef u32x2 u32x2_any __attribute__((aligned(1)));
 template <typename T, typename W, int MODE, int LPR, int VPL>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows_fp8_kernel(
     uint8_t* codes, float* scale, T* ro, const T* x, const T* r, const W* w, RowGrid grid, RowStrides lx, RowStrides lr,
-    RowStrides lro, int n, uint32_t rows, float eps) {
+    RowStrides lro, int n, uint32_t row0, uint32_t rows, float eps) {
   typedef typename Vec8<T>::type V8;
   constexpr int NT = LPR > 256 ? LPR : 256, RPB = NT / LPR, NWAVE = LPR / kWave;
   constexpr bool ADD = MODE == ROWS_ADD, NORM = MODE != ROWS_PLAIN;
   const int l = threadIdx.x % LPR;
-  const uint32_t row = blockIdx.x * RPB + threadIdx.x / LPR;
+  const uint32_t row = row0 + blockIdx.x * RPB + threadIdx.x / LPR;
   const bool live = row < rows;
   const int nv = (n + 7) / 8;
   const RowPos p = row_pos(grid, live ? row : 0);
@@ -202,11 +202,12 @@ template <typename T, int MODE>
 __global__ __launch_bounds__(256) void rows_fp8_gen_kernel(uint8_t* codes, float* scale, T* ro, const T* x, const T* r,
                                                            const void* w, int w_dtype, int64_t w_stride, RowGrid grid,
                                                            RowStrides lx, RowStrides lr, RowStrides lro, int64_t n,
-                                                           float eps) {
+                                                           uint32_t row0, float eps) {
   constexpr bool ADD = MODE == ROWS_ADD, NORM = MODE != ROWS_PLAIN;
   __shared__ float sums[4];
   __shared__ uint32_t tops[4];
-  const RowPos p = row_pos(grid, blockIdx.x);
+  const uint32_t row = row0 + blockIdx.x;
+  const RowPos p = row_pos(grid, row);
   const T* xr = x + row_off(lx, p);
   const T* rr = ADD ? r + row_off(lr, p) : nullptr;
   auto value = [&](int64_t k) {
@@ -233,8 +234,8 @@ __global__ __launch_bounds__(256) void rows_fp8_gen_kernel(uint8_t* codes, float
     mx = tops[i] > mx ? tops[i] : mx;
   }
   const CodeScale q = row_scale(NORM && n ? rsqrtf(ss / (float)n + eps) : 1.f, mx);
-  if (threadIdx.x == 0) scale[blockIdx.x] = q.scale;
-  uint8_t* cr = codes + (int64_t)blockIdx.x * n;
+  if (threadIdx.x == 0) scale[row] = q.scale;
+  uint8_t* cr = codes + (int64_t)row * n;
   T* ror = ADD ? ro + row_off(lro, p) : nullptr;
   for (int64_t k = threadIdx.x; k < n; k += 256) {
     const float f = value(k);
@@ -258,13 +259,25 @@ struct RowsArgs {
   hipStream_t st;
 };
 
+// launch(first row, workgroups) over all rows, `per` a workgroup of `threads`: a launch has fewer than 2^32 threads.
+template <typename F>
+void row_launches(int64_t rows, int per, int threads, F&& launch) {
+  const int64_t most = (int64_t)(0xffffffffu / (unsigned)threads) * per;
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t some = rows - r < most ? rows - r : most;
+    launch((uint32_t)r, dim3((unsigned)((some + per - 1) / per)));
+  }
+}
+
 template <typename T, typename W, int MODE, int LPR, int VPL>
 void launch_rows(const RowsArgs& a) {
   constexpr int NT = LPR > 256 ? LPR : 256, RPB = NT / LPR;
-  hipLaunchKernelGGL((rows_fp8_kernel<T, W, MODE, LPR, VPL>), dim3((unsigned)((a.rows + RPB - 1) / RPB)), dim3(NT), 0,
-                     a.st, static_cast<uint8_t*>(a.codes), a.scale, static_cast<T*>(a.ro), static_cast<const T*>(a.x),
-                     static_cast<const T*>(a.r), static_cast<const W*>(a.w), row_grid(a.lx), row_strides(a.lx),
-                     row_strides(a.lr), row_strides(a.lro), (int)a.lx.n, (uint32_t)a.rows, a.eps);
+  row_launches(a.rows, RPB, NT, [&](uint32_t row0, dim3 blocks) {
+    hipLaunchKernelGGL((rows_fp8_kernel<T, W, MODE, LPR, VPL>), blocks, dim3(NT), 0, a.st,
+                       static_cast<uint8_t*>(a.codes), a.scale, static_cast<T*>(a.ro), static_cast<const T*>(a.x),
+                       static_cast<const T*>(a.r), static_cast<const W*>(a.w), row_grid(a.lx), row_strides(a.lx),
+                       row_strides(a.lr), row_strides(a.lro), (int)a.lx.n, row0, (uint32_t)a.rows, a.eps);
+  });
 }
 
 constexpr int64_t kRowsMaxN = 32768;  // 1024 lanes of four vectors
@@ -299,10 +312,12 @@ int dispatch_rows(const RowsArgs& a) {
   else if (MODE != ROWS_PLAIN && unit && a.lx.n >= 8 && a.lx.n <= kRowsMaxN && a.w_dtype == FD_F32)
     pick_rows<T, typename std::conditional<MODE == ROWS_PLAIN, T, float>::type, MODE>(a);
   else
-    hipLaunchKernelGGL((rows_fp8_gen_kernel<T, MODE>), dim3((unsigned)a.rows), dim3(256), 0, a.st,
-                       static_cast<uint8_t*>(a.codes), a.scale, static_cast<T*>(a.ro), static_cast<const T*>(a.x),
-                       static_cast<const T*>(a.r), a.w, a.w_dtype, a.w_stride, row_grid(a.lx), row_strides(a.lx),
-                       row_strides(a.lr), row_strides(a.lro), a.lx.n, a.eps);
+    row_launches(a.rows, 1, 256, [&](uint32_t row0, dim3 blocks) {
+      hipLaunchKernelGGL((rows_fp8_gen_kernel<T, MODE>), blocks, dim3(256), 0, a.st, static_cast<uint8_t*>(a.codes),
+                         a.scale, static_cast<T*>(a.ro), static_cast<const T*>(a.x), static_cast<const T*>(a.r), a.w,
+                         a.w_dtype, a.w_stride, row_grid(a.lx), row_strides(a.lx), row_strides(a.lr),
+                         row_strides(a.lro), a.lx.n, row0, a.eps);
+    });
   return check_launch();
 }
 

@@ -194,9 +194,9 @@ __global__ __launch_bounds__((WN * WM + PW) * kWave) void w8a8_tile_kernel(T* y,
     const uint8_t* base = i < AOPS ? (up ? ubase : wbase) : xbase;
     const unsigned to = lds0 + (unsigned)(s % D) * kStage + place(i), o = voff[i];
     if (k0 + kStep <= K)
-      dma16<false>(base + k0, o, to);
+      dma16(base + k0, o, to);
     else  // pieces past K: the row's start
-      dma16<false>(base, k0 + off[i] < K ? o + (unsigned)k0 : o - (unsigned)off[i], to);
+      dma16(base, k0 + off[i] < K ? o + (unsigned)k0 : o - (unsigned)off[i], to);
   };
   auto zero_tail = [&](int s) {  // DMA past K brought the row's start: the activations there become zero
     const int k0 = stage_k(s);
@@ -480,7 +480,7 @@ int tile_launch(const W8Args& a, int splits) {
   constexpr size_t lds = ring > sums ? ring : sums;
   static_assert(lds <= kMaxLds, "a launch fits the LDS of a CU");
   const int64_t nt = (a.N + BN - 1) / BN, mt = (a.M + BM - 1) / BM;
-  if (nt * mt * splits > 0x7fffffffLL) return set_error(FD_EUNSUPPORTED, "too many tiles");
+  if (nt * mt * splits * ((WN * WM + PW) * kWave) > 0xffffffffLL) return set_error(FD_EUNSUPPORTED, "too many tiles");
   auto kernel = w8a8_tile_kernel<T, PW, WN, WM, NT, MT, D, SWIGLU, FORM>;
   if (!allow_lds(kernel, lds)) return set_error(FD_ELAUNCH, "cannot raise the LDS limit to %zu bytes", lds);
   hipLaunchKernelGGL(kernel, dim3((unsigned)(nt * mt * splits)), dim3((WN * WM + PW) * kWave), lds, a.st,
@@ -489,16 +489,16 @@ int tile_launch(const W8Args& a, int splits) {
   return FD_OK;
 }
 
-// The forms of a tile launch: output columns (weight rows) and activation rows of a tile, workgroups
-// that a CU holds, and microseconds that a stage of all of them takes and a round of them besides (its start, its
-// output), measured.
+// The forms of a tile launch: output columns (weight rows) and activation rows of a tile, and the microseconds that
+// a stage takes with a workgroup on every CU and a round of them besides (its start, its output). Fitted to products
+// of 64 to 8192 rows, 1024 to 28672 columns and K of 512 to 14336 whose time was measured in every form.
 struct TileForm {
-  int bn, bm, per_cu;
+  int bn, bm;
   float stage, round;
 };
 enum { T_256 = 0, T_256x128, T_128, T_64x128, T_64, T_128x32, T_FORMS };
-constexpr TileForm kTiles[T_FORMS] = {{256, 256, 1, 1.40f, 9.f},  {256, 128, 1, 0.80f, 6.f}, {128, 128, 1, 0.58f, 5.f},
-                                      {64, 128, 1, 0.37f, 5.f},   {64, 64, 1, 0.29f, 4.5f},  {128, 32, 1, 0.33f, 4.f}};
+constexpr TileForm kTiles[T_FORMS] = {{256, 256, 1.40f, 9.f}, {256, 128, 0.80f, 6.f}, {128, 128, 0.58f, 5.f},
+                                      {64, 128, 0.37f, 5.f},  {64, 64, 0.29f, 4.5f},  {128, 32, 0.33f, 4.f}};
 
 struct TilePlan {
   int form, splits;
@@ -516,7 +516,7 @@ TilePlan tile_plan(int64_t M, int64_t N, int64_t K) {
     int64_t most = cus / (tiles < cus ? tiles : cus);
     if (most > stages / 6) most = stages / 6;
     for (int64_t s = 1; s == 1 || s <= most; ++s) {
-      const int64_t rounds = (tiles * s + cus * t.per_cu - 1) / (cus * t.per_cu);
+      const int64_t rounds = (tiles * s + cus - 1) / cus;
       const float sum = s > 1 ? 4.f + (float)(s * M * N) * 8e-6f / 4.f : 0.f;  // 4 TB/s there and back
       const float us = (float)rounds * ((float)((stages + s - 1) / s) * t.stage + t.round) + sum;
       if (us < least) {
@@ -552,27 +552,28 @@ int tiles(const W8Args& a, TilePlan p) {
   return FD_OK;
 }
 
-// K below one 16-byte piece, none included: a thread per output.
+// K below one 16-byte piece, none included: a thread per output, and as many more as the grid leaves it.
 template <typename T, bool SWIGLU>
 __global__ __launch_bounds__(256) void w8a8_short_kernel(T* y, const uint8_t* x, const uint8_t* w, int M, int N, int K,
                                                          int64_t sxm, int64_t swn, int64_t sym, int64_t syn, W8Epi e,
                                                          int64_t total) {
-  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (v >= total) return;
-  const int cols = SWIGLU ? N / 2 : N, m = (int)(v / cols), c = (int)(v - (int64_t)m * cols);
-  float a = 0.f, u = 0.f;
-  for (int k = 0; k < K; ++k) {
-    const float xv = __builtin_amdgcn_cvt_f32_fp8(x[m * sxm + k], 0);
-    a += xv * __builtin_amdgcn_cvt_f32_fp8(w[c * swn + k], 0);
-    if constexpr (SWIGLU) u += xv * __builtin_amdgcn_cvt_f32_fp8(w[(c + (int64_t)cols) * swn + k], 0);
+  const int cols = SWIGLU ? N / 2 : N;
+  for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)gridDim.x * 256) {
+    const int m = (int)(v / cols), c = (int)(v - (int64_t)m * cols);
+    float a = 0.f, u = 0.f;
+    for (int k = 0; k < K; ++k) {
+      const float xv = __builtin_amdgcn_cvt_f32_fp8(x[m * sxm + k], 0);
+      a += xv * __builtin_amdgcn_cvt_f32_fp8(w[c * swn + k], 0);
+      if constexpr (SWIGLU) u += xv * __builtin_amdgcn_cvt_f32_fp8(w[(c + (int64_t)cols) * swn + k], 0);
+    }
+    y[m * sym + c * syn] = from_f32<T>(w8_out<SWIGLU>(e, a, u, m, c, cols));
   }
-  y[m * sym + c * syn] = from_f32<T>(w8_out<SWIGLU>(e, a, u, m, c, cols));
 }
 
 template <typename T, bool SWIGLU>
 int short_launch(const W8Args& a) {
-  const int64_t total = (int64_t)a.M * (SWIGLU ? a.N / 2 : a.N), blocks = (total + 255) / 256;
-  if (blocks > 0x7fffffffLL) return set_error(FD_EUNSUPPORTED, "too large");
+  const int64_t total = (int64_t)a.M * (SWIGLU ? a.N / 2 : a.N), most = 1 << 20;
+  const int64_t blocks = (total + 255) / 256 < most ? (total + 255) / 256 : most;
   hipLaunchKernelGGL((w8a8_short_kernel<T, SWIGLU>), dim3((unsigned)blocks), dim3(256), 0, a.st, static_cast<T*>(a.y),
                      a.x, a.w, a.M, a.N, a.K, a.sxm, a.swn, a.sym, a.syn, a.e, total);
   return FD_OK;

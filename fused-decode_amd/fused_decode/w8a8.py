@@ -53,9 +53,19 @@ _MOST_STRIDE = 1 << 23  # bytes between rows that the product's kernels take as 
 
 
 def _watched() -> bool:
-    """Whether something would record or transform a call, which a launch on bare pointers would be missing from."""
+    """Whether something would record or transform a call, which a launch on bare pointers would be missing from
+    (a tensor whose negation is still to be made takes the same way: the dispatcher makes it)."""
     return bool(torch.compiler.is_compiling() or forward_ad._current_level >= 0 or _transform() is not None
                 or _is_tracing() or _dispatch_modes() or (_function_modes() and _function_modes_watch()))
+
+
+def _out_sig(t: torch.Tensor) -> tuple:
+    """Signature of an output that torch would write in place as well."""
+    if t.requires_grad and _grad():
+        raise RuntimeError("an output that requires a gradient cannot be written in place")
+    if t.is_inference() and not torch.is_inference_mode_enabled():
+        raise RuntimeError("an inference tensor cannot be written outside inference mode")
+    return _sig(t)
 
 
 def _like(shape: tuple, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
@@ -75,10 +85,10 @@ def quantize_rows_fp8(
     """E4M3 codes of ``x``'s rows (its last dimension) and their float32 scales ``x.shape[:-1]``, in one
     launch. For finite rows the codes and scales that ``quantize_fp8`` gives the same rows."""
     try:
-        if _watched() or (_grad() and x.requires_grad):
+        if _watched() or (_grad() and x.requires_grad) or x.is_neg():
             return _copied(torch.ops.fused_decode.quantize_rows_fp8(x), out, scale_out)
-        key = ("quantize_rows_fp8", x.shape, x.stride(), x.dtype, x.get_device(), None if out is None else _sig(out),
-               None if scale_out is None else _sig(scale_out))
+        key = ("quantize_rows_fp8", x.shape, x.stride(), x.dtype, x.get_device(), None if out is None else _out_sig(out),
+               None if scale_out is None else _out_sig(scale_out))
         plan = _PLANS.get(key)
     except AttributeError:  # not a tensor: let the contract say so
         key, plan = None, None
@@ -98,11 +108,12 @@ def rms_norm_fp8(
     """``rms_norm`` with E4M3 codes and float32 row scales for its result. ``weight`` is ``(N,)``
     (float16, bfloat16 or float32)."""
     try:
-        if _watched() or (_grad() and (x.requires_grad or weight.requires_grad)):
+        if (_watched() or (_grad() and (x.requires_grad or weight.requires_grad)) or x.is_neg()
+                or weight.is_neg()):
             return _copied(torch.ops.fused_decode.rms_norm_fp8(x, weight, eps), out, scale_out)
         key = ("rms_norm_fp8", x.shape, x.stride(), x.dtype, x.get_device(), weight.shape, weight.stride(), weight.dtype,
-               weight.get_device(), eps, None if out is None else _sig(out),
-               None if scale_out is None else _sig(scale_out))
+               weight.get_device(), eps, None if out is None else _out_sig(out),
+               None if scale_out is None else _out_sig(scale_out))
         plan = _PLANS.get(key)
     except (AttributeError, TypeError):  # a non-tensor or unhashable argument: checked below
         key, plan = None, None
@@ -124,12 +135,13 @@ def add_rms_norm_fp8(
     """``add_rms_norm`` with E4M3 codes and float32 row scales for the norm of the float32 sum:
     ``(codes, scale, residual_out)``. ``residual_out=residual`` updates the residual stream in place."""
     try:
-        if _watched() or (_grad() and (x.requires_grad or residual.requires_grad or weight.requires_grad)):
+        if (_watched() or (_grad() and (x.requires_grad or residual.requires_grad or weight.requires_grad))
+                or x.is_neg() or residual.is_neg() or weight.is_neg()):
             return _copied(torch.ops.fused_decode.add_rms_norm_fp8(x, residual, weight, eps), out, scale_out, residual_out)
         key = ("add_rms_norm_fp8", x.shape, x.stride(), x.dtype, x.get_device(), residual.shape, residual.stride(),
                residual.dtype, residual.get_device(), weight.shape, weight.stride(), weight.dtype, weight.get_device(),
-               eps, None if out is None else _sig(out), None if scale_out is None else _sig(scale_out),
-               None if residual_out is None else _sig(residual_out))
+               eps, None if out is None else _out_sig(out), None if scale_out is None else _out_sig(scale_out),
+               None if residual_out is None else _out_sig(residual_out))
         plan = _PLANS.get(key)
     except (AttributeError, TypeError):
         key, plan = None, None
@@ -140,6 +152,9 @@ def add_rms_norm_fp8(
 
 def _copied(got: tuple, *outs) -> tuple:
     """A custom op's results, copied where outputs are given."""
+    for v, o in zip(got, outs):
+        if o is not None and (o.shape != v.shape or o.dtype != v.dtype or o.device != v.device):
+            raise ValueError(f"an output must have shape {tuple(v.shape)} and dtype {v.dtype} on {v.device}")
     return tuple(v if o is None else o.copy_(v) for v, o in zip(got, outs))
 
 
@@ -242,14 +257,16 @@ def linear_w8a8(
     try:
         if _watched() or (_grad() and (x_scale.requires_grad or scale.requires_grad or x.requires_grad
                                        or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                       or (row_add is not None and row_add.requires_grad))):
+                                       or (row_add is not None and row_add.requires_grad))) \
+                or x_scale.is_neg() or scale.is_neg() or (bias is not None and bias.is_neg()) \
+                or (row_add is not None and row_add.is_neg()):
             y = torch.ops.fused_decode.linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add,
                                                    dtype or (torch.bfloat16 if out is None else out.dtype))
-            return y if out is None else out.copy_(y)
+            return _copied((y,), out)[0]
         key = ("linear_w8a8", x.shape, x.stride(), x.dtype, x.get_device(), x_scale.shape, x_scale.stride(), x_scale.dtype,
                x_scale.get_device(), weight.shape, weight.stride(), weight.dtype, weight.get_device(), scale.shape,
                scale.stride(), scale.dtype, scale.get_device(), None if bias is None else _sig(bias), activation,
-               None if row_add is None else _sig(row_add), None if out is None else _sig(out), dtype)
+               None if row_add is None else _sig(row_add), None if out is None else _out_sig(out), dtype)
         plan = _PLANS.get(key)
     except (AttributeError, TypeError):  # a non-tensor or unhashable argument: checked below
         key, plan = None, None

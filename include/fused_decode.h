@@ -461,11 +461,11 @@ int fd_add_rms_norm_fp8(void* codes, float* scale, void* residual_out, const voi
  * Sums and the epilogue are float32 with one rounding. bias (N values at stride sb) and
  * row_add (strides srm, srn; 0 broadcasts) have any of the three dtypes and may be NULL; y has
  * act_dtype. `scratch` (16-byte aligned, caller-owned, not shared with a call that may
- * overlap) holds what fd_linear_w8a8_scratch says (0: none; `aligned`: whether the rows of
- * both operands are 16-byte aligned, as row strides and pointers that are multiples of 16
- * make them): copies of rows that are not, or whose K is no multiple of 16 (without it
- * FD_EUNSUPPORTED), and, where there are few output tiles, the float32 sums of K splits, which are added in a
- * fixed order; less lowers the split, down to none. y may be row_add element for element and
+ * overlap) holds what fd_linear_w8a8_scratch says (0: none; `aligned`: whether the pointers and
+ * row strides of both operands are multiples of 16 and the strides below 8 MiB): copies of
+ * rows that are not so, or whose K is no multiple of 16 (without it FD_EUNSUPPORTED), and,
+ * where there are few output tiles, the float32 sums of K splits, which are added in a fixed
+ * order; less lowers the split, down to none. y may be row_add element for element and
  * overlaps no operand otherwise (FD_EUNSUPPORTED). No reference counterpart.
  */
 int fd_linear_w8a8(void* y, const void* x8, const float* x_scale, const void* w8,

@@ -524,3 +524,49 @@ def test_custom_ops_and_gradients():
     out = torch.empty(6, 64, dtype=torch.float16, device=DEV)
     with torch.no_grad():
         assert fd.linear_w8a8(c, s, q, qs, bias, out=out) is out
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("name", ["relu", "silu", "gelu", "gelu_tanh", "swiglu"])
+def test_activations_of_infinities(name, dtype):
+    """A NaN stays one, an infinity gives the activation's limit: itself above, and below nothing but 0 or NaN."""
+    import fused_decode as fd
+
+    k, top = 32, 3e38
+    bias = torch.tensor([top, -top, float("nan"), 0.0], device=DEV)
+    x = torch.ones(2, k, device=DEV).to(E4M3)
+    w = torch.tensor([1.0, -1.0, 0.0, 0.0], device=DEV)[:, None].expand(4, k).contiguous().to(E4M3)
+    xs, ws = torch.full((2,), 2.0**60, device=DEV), torch.full((4,), 2.0**67, device=DEV)  # 2^132: past float32
+    y = fd.linear_w8a8(x, xs, w, ws, bias, activation=None if name == "swiglu" else name, dtype=dtype)
+    if name != "swiglu":
+        assert bool((y[:, 0] == float("inf")).all()) and bool(y[:, 2].isnan().all()) and bool((y[:, 3] == 0).all())
+        assert bool(((y[:, 1] == 0) | y[:, 1].isnan()).all())
+    half = torch.tensor([0.0, 0.0, 2.0, 1.0], device=DEV)
+    gate_up = fd.linear_w8a8(x, xs, w, ws, half, activation="swiglu", dtype=dtype)
+    assert bool((gate_up[:, 0] == float("inf")).all())
+
+
+def test_more_rows_than_one_launch_takes():
+    """Rows past the 2^32 threads of a launch, at a workgroup a row: the last ones are computed like any others."""
+    import fused_decode as fd
+
+    rows, n = 2**24 + 1000, 4
+    x = torch.ones(rows, n, dtype=torch.float16, device=DEV)
+    x[-2000:] = rnd(2000, n, seed=1, dtype=torch.float16)
+    codes, scale = fd.quantize_rows_fp8(x)
+    check_same_codes(codes[-2000:], scale[-2000:], x[-2000:])
+    assert bool((codes[:-2000].view(torch.uint8) == 0x7E).all())  # 448
+    assert torch.equal(scale[:-2000], scale[:1].expand(rows - 2000))
+
+
+def test_a_negation_still_to_be_made():
+    import fused_decode as fd
+
+    x, w = rnd(5, 64, seed=1, dtype=torch.float16), rnd(64, seed=2)
+    for got, want in ((fd.quantize_rows_fp8(torch._neg_view(x)), fd.quantize_rows_fp8(-x)),
+                      (fd.rms_norm_fp8(x, torch._neg_view(w)), fd.rms_norm_fp8(x, -w)),
+                      (fd.add_rms_norm_fp8(x, torch._neg_view(x), w), fd.add_rms_norm_fp8(x, -x, w))):
+        for a, b in zip(got, want):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    c, s = fd.quantize_rows_fp8(x)
+    assert torch.equal(fd.linear_w8a8(c, s, c, s, torch._neg_view(s)), fd.linear_w8a8(c, s, c, s, -s))
