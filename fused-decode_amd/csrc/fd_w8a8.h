@@ -152,7 +152,7 @@ __device__ __forceinline__ float w8_out(const W8Epi& e, float acc, float up, int
   return v;
 }
 
-// A checked product, as the launchers take it: 16-byte aligned rows of whole 16-byte pieces but for K < 16.
+// A checked product, as the launchers take it: 16-byte aligned rows of whole 16-byte pieces but for K < 16 and M = 1.
 struct W8Args {
   void* y;
   const uint8_t *x, *w;
@@ -165,6 +165,9 @@ struct W8Args {
   int act_dtype;
   hipStream_t st;
 };
+
+// One row (w8a8_one.hip): K >= 16, at any alignment.
+int w8_one_launch(const W8Args& a);
 
 // Few rows (w8a8_few.hip): whether a product fits, and its launch.
 bool w8_few_fits(int64_t M, int64_t K);

@@ -183,7 +183,8 @@ __global__ __launch_bounds__((WN * WM + PW) * kWave) void w8a8_tile_kernel(T* y,
     const int m = m0 + t;
     const int64_t row = wt ? wrow(t) : (m < M ? m : M - 1);
     off[i] = ((lane & 7) ^ (t & 7)) * 16;
-    voff[i] = (unsigned)(wt ? (row - n_first - (SWIGLU && ((t >> 4) & 1) ? half : 0)) * swn : (row - m0) * sxm) + off[i];
+    const int64_t first = n_first + (SWIGLU && ((t >> 4) & 1) ? half : 0);
+    voff[i] = (unsigned)(wt ? (row - first) * swn : (row - m0) * sxm) + off[i];
   }
   auto place = [&](int i) {  // byte address in a stage of this wave's i-th KiB: weights, then activations
     return (unsigned)(i < AOPS ? lw * AOPS + i : BN / 8 + lw * BOPS + i - AOPS) * 1024u;
@@ -599,8 +600,8 @@ int align_rows(W8Args& a) {
   if (a.scratch_bytes < total * 16) return set_error(FD_EUNSUPPORTED, "rows off 16-byte alignment need scratch");
   uint8_t* const to = reinterpret_cast<uint8_t*>(a.scratch);
   hipLaunchKernelGGL(w8a8_align_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, a.st,
-                     reinterpret_cast<u32x4*>(to), a.x, a.w, (uint32_t)a.M, a.sxm, a.swn, a.K, FastDiv((uint32_t)pieces),
-                     (uint32_t)total);
+                     reinterpret_cast<u32x4*>(to), a.x, a.w, (uint32_t)a.M, a.sxm, a.swn, a.K,
+                     FastDiv((uint32_t)pieces), (uint32_t)total);
   a.K = (int)(pieces * 16);
   a.sxm = a.swn = a.K;
   a.x = to;
@@ -613,6 +614,10 @@ int align_rows(W8Args& a) {
 template <typename T, bool SWIGLU>
 int product(const W8Args& a) {
   if (a.K < 16) return short_launch<T, SWIGLU>(a);
+  if (a.M == 1) {
+    if (a.K > kMostIndex - (1 << 14)) return set_error(FD_EUNSUPPORTED, "too large");
+    return w8_one_launch(a);
+  }
   if (w8_few_fits(a.M, a.K)) return w8_few_launch(a);
   TilePlan p = tile_plan(a.M, a.N, a.K);
   while (p.splits > 1 && a.scratch_bytes < (int64_t)p.splits * a.M * a.N * 4) --p.splits;
@@ -628,7 +633,7 @@ extern "C" int fd_linear_w8a8_scratch(int64_t M, int64_t N, int64_t K, int align
   if (M < 0 || N < 0 || K < 0) return set_error(FD_EINVAL, "negative size");
   if (!bytes) return set_error(FD_EINVAL, "null pointer argument");
   *bytes = 0;
-  if (M == 0 || N == 0 || K < 16 || M > kMostIndex || N > kMostIndex || K > kMostIndex) return FD_OK;
+  if (M <= 1 || N == 0 || K < 16 || M > kMostIndex || N > kMostIndex || K > kMostIndex) return FD_OK;
   const int64_t Kp = (K + 15) / 16 * 16;
   if (!aligned || K != Kp) *bytes = (M + N) * Kp;
   if (w8_few_fits(M, Kp)) return FD_OK;
@@ -684,7 +689,7 @@ extern "C" int fd_linear_w8a8(void* y, const void* x8, const float* x_scale, con
   auto fits = [&](const void* p, int64_t rows, int64_t stride) {
     return K % 16 == 0 && aligned16(p) && (rows == 1 || (stride % 16 == 0 && stride < kMostStride));
   };
-  if (K >= 16 && !(fits(x8, M, sxm) && fits(w8, N, swn)) && align_rows(a) != FD_OK) return FD_EUNSUPPORTED;
+  if (K >= 16 && M > 1 && !(fits(x8, M, sxm) && fits(w8, N, swn)) && align_rows(a) != FD_OK) return FD_EUNSUPPORTED;
   const int rc = act_dtype == FD_F16 ? (swiglu ? product<f16, true>(a) : product<f16, false>(a))
                                      : (swiglu ? product<bf16, true>(a) : product<bf16, false>(a));
   if (rc != FD_OK) return rc;

@@ -1,4 +1,4 @@
-// Products of E4M3 activations and weights for few activation rows (up to 32): the weights
+// Products of E4M3 activations and weights for few activation rows (2 to 32): the weights
 // stream through LDS once, the activations stay in registers (fd_w8a8.h has the mathematics).
 //
 // A workgroup of eight waves, one to a CU, owns a run of outputs and walks them in tiles of 16
@@ -30,14 +30,16 @@ constexpr size_t few_lds() {
 template <typename T, int MF, int S, int D, bool SWIGLU>
 __global__ __launch_bounds__(kFewWaves * kWave) void w8a8_few_kernel(T* y, const uint8_t* x, const uint8_t* w, int M,
                                                                      int N, int K, int64_t sxm, int64_t swn,
-                                                                     int64_t sym, int64_t syn, W8Epi e) {
+                                                                     int64_t sym, int64_t syn, W8Epi e, int per,
+                                                                     int longer) {
   constexpr int NW = kFewWaves, Q = SWIGLU ? 8 : 16;  // outputs of a tile
   extern __shared__ __align__(16) u32x4 w8_smem[];
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int r = lane & 15, g = lane >> 4;
-  const int half = N / 2, cols = SWIGLU ? half : N;
-  const int o0 = (int)((int64_t)cols * blockIdx.x / gridDim.x), o1 = (int)((int64_t)cols * (blockIdx.x + 1) / gridDim.x);
+  const int half = N / 2;
+  // `per` outputs a workgroup, one more in the first `longer`
+  const int b = (int)blockIdx.x, o0 = b * per + (b < longer ? b : longer), o1 = o0 + per + (b < longer ? 1 : 0);
   const int tiles = (o1 - o0 + Q - 1) / Q;
   const int steps = (K + kStep - 1) / kStep;
   const int sn = (steps - wave + NW - 1) / NW;  // this wave's steps of a tile
@@ -129,7 +131,8 @@ __global__ __launch_bounds__(kFewWaves * kWave) void w8a8_few_kernel(T* y, const
   lds_barrier();
   // sum of weight row `row` of tile t and activation row m
   auto sum = [&](int t, int row, int m) {
-    return reinterpret_cast<const float*>(done)[((t * MF + m / 16) * kWave + (row >> 2) * 16 + (m & 15)) * 4 + (row & 3)];
+    const int lane_of = (t * MF + m / 16) * kWave + (row >> 2) * 16 + (m & 15);
+    return reinterpret_cast<const float*>(done)[lane_of * 4 + (row & 3)];
   };
   const int run = o1 - o0;
   for (int i = tid; i < run * M; i += NW * kWave) {
@@ -152,7 +155,7 @@ int few_go(const W8Args& a) {
   auto kernel = w8a8_few_kernel<T, MF, S, D, SWIGLU>;
   if (!allow_lds(kernel, lds)) return set_error(FD_ELAUNCH, "cannot raise the LDS limit to %zu bytes", lds);
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kFewWaves * kWave), lds, a.st, static_cast<T*>(a.y), a.x, a.w,
-                     a.M, a.N, a.K, a.sxm, a.swn, a.sym, a.syn, a.e);
+                     a.M, a.N, a.K, a.sxm, a.swn, a.sym, a.syn, a.e, cols / grid, cols % grid);
   return FD_OK;
 }
 
