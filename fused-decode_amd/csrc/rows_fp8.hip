@@ -18,6 +18,11 @@
 // max|y| = max|t * w| * rsqrt(...), so the sum of squares and the maximum come from one
 // sweep and one exchange between lanes.
 //
+// Many rows are bound by HBM (8192 x 4096, add and norm: 38.7 us, 6.1 TB/s, half of them
+// writes; 2048 x 14336 quantised: 16.4 us, 5.4 TB/s), few by a launch's start and end (1 x 4096:
+// 2.6 us of device time). Codes are read by the product that follows, not by this kernel: their
+// stores are nontemporal.
+//
 // Two kernels:
 //   rows_fp8_kernel     - unit column stride, rows of any alignment, 8 <= n <= 32768: LPR
 //                         lanes a row (part of a wave, a wave or a workgroup).
@@ -282,24 +287,32 @@ void launch_rows(const RowsArgs& a) {
 
 constexpr int64_t kRowsMaxN = 32768;  // 1024 lanes of four vectors
 
-// Lanes of a row: one vector a lane up to 512 elements; past that a wave, with up to 16 vectors
-// a lane, or a workgroup.
+// Lanes of a row: one vector a lane up to 512 elements, two up to 1024, then a workgroup. Many
+// rows of up to 2048 that are quantised alone, with no second operand on the way, take a wave
+// each. Measured (us, bf16, add and norm / quantise; a workgroup a row, then a wave a row):
+//   rows x n       workgroup        wave
+//   256 x 1024     2.77 / 2.40      2.73 / 2.32
+//   8192 x 1024    13.1 / 8.10      11.1 / 5.31
+//   256 x 2048     2.76 / 2.40      3.41 / 2.64
+//   8192 x 2048    19.4 / 10.6      21.2 / 9.36
+//   256 x 4096     3.44 / 2.92      5.84 / 3.74
+//   8192 x 4096    38.2 / 16.7      43.5 / 17.0
 template <typename T, typename W, int MODE>
 void pick_rows(const RowsArgs& a) {
   const int64_t nv = (a.lx.n + 7) / 8;
-  const bool many = a.rows >= (int64_t)device_cus() * 4;
-  if (nv <= 8) launch_rows<T, W, MODE, 8, 1>(a);
-  else if (nv <= 16) launch_rows<T, W, MODE, 16, 1>(a);
-  else if (nv <= 32) launch_rows<T, W, MODE, 32, 1>(a);
-  else if (nv <= 64) launch_rows<T, W, MODE, 64, 1>(a);
-  else if (many && nv <= 128) launch_rows<T, W, MODE, 64, 2>(a);
-  else if (many && nv <= 256) launch_rows<T, W, MODE, 64, 4>(a);
-  else if (many && nv <= 512) launch_rows<T, W, MODE, 64, 8>(a);
-  else if (nv <= 256) launch_rows<T, W, MODE, 256, 1>(a);
-  else if (nv <= 512) launch_rows<T, W, MODE, 256, 2>(a);
-  else if (nv <= 1024) launch_rows<T, W, MODE, 256, 4>(a);
-  else if (nv <= 2048) launch_rows<T, W, MODE, 256, 8>(a);
-  else launch_rows<T, W, MODE, 1024, 4>(a);
+  if (nv <= 8) return launch_rows<T, W, MODE, 8, 1>(a);
+  if (nv <= 16) return launch_rows<T, W, MODE, 16, 1>(a);
+  if (nv <= 32) return launch_rows<T, W, MODE, 32, 1>(a);
+  if (nv <= 64) return launch_rows<T, W, MODE, 64, 1>(a);
+  if (nv <= 128) return launch_rows<T, W, MODE, 64, 2>(a);
+  if constexpr (MODE == ROWS_PLAIN) {
+    if (nv <= 256 && a.rows >= (int64_t)device_cus() * 4) return launch_rows<T, W, MODE, 64, 4>(a);
+  }
+  if (nv <= 256) return launch_rows<T, W, MODE, 256, 1>(a);
+  if (nv <= 512) return launch_rows<T, W, MODE, 256, 2>(a);
+  if (nv <= 1024) return launch_rows<T, W, MODE, 256, 4>(a);
+  if (nv <= 2048) return launch_rows<T, W, MODE, 256, 8>(a);
+  launch_rows<T, W, MODE, 1024, 4>(a);
 }
 
 template <typename T, int MODE>
