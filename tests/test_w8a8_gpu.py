@@ -604,3 +604,34 @@ def test_one_row(n, k):
             assert torch.equal(y, (v[:, :n].clamp_min(0) + row.double()).float().to(dtype))
             y = fd.linear_w8a8(xp, xs, wp, ws, bias, activation="swiglu", row_add=row, dtype=dtype)
             check_product(y, x, xs, w, ws, bias, "swiglu", row, dtype)
+
+
+def test_captured_as_the_first_call():
+    """A capture that also makes the launch plans: nothing of them belongs to the graph, whose replays and the eager
+    calls after it agree, before and after the graph is gone."""
+    import fused_decode as fd
+    from fused_decode import ops
+
+    ops.clear_plans()
+    x, w = rnd(90, 2048, seed=1, dtype=torch.bfloat16), rnd(2048, seed=2)
+    q, qs = fd.quantize_fp8(rnd(600, 2048, seed=3))
+    odd, odds = fd.quantize_fp8(rnd(70, 2047, seed=4))
+
+    def run():
+        c, s, h = fd.add_rms_norm_fp8(x, x, w)
+        d, t = fd.quantize_rows_fp8(h[:, 1:])
+        return (fd.linear_w8a8(c, s, q, qs, activation="silu"), fd.linear_w8a8(c[:1], s[:1], q, qs),
+                fd.linear_w8a8(c[:9], s[:9], q, qs), fd.linear_w8a8(d, t, odd, odds))
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for _ in range(3):
+        graph.replay()
+        want = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    kept = [t.clone() for t in got]
+    del got, graph
+    assert all(torch.equal(a, b) for a, b in zip(kept, run()))
