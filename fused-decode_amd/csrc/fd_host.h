@@ -56,6 +56,57 @@ inline bool same_grid(const fd_rows& x, const fd_rows& o, const char* what) {
   return true;
 }
 
+// Whether two elements of a layout lie at one address: strides that broadcast, windows that run into each other.
+// Sorted by stride, dimensions that each step past all that the smaller ones reach hold no such two, which is every
+// view that slices and transposes make. For the rest (no more than four, of sizes > 1) it is the question
+// whether some steps, not all zero and less than each size, add up to nothing: answered by search, and by yes where
+// the search is longer than kMeetSearch.
+struct RowDim {
+  int64_t size, step;
+};
+constexpr int kMeetSearch = 1 << 16;
+
+// `at` + steps of dims[0 .. n) = 0, with a step taken somewhere (`moved`: there was one).
+inline bool steps_cancel(const RowDim* dims, int n, int64_t at, bool moved, int& budget) {
+  if (n == 0) return at == 0 && moved;
+  int64_t rest = 0;
+  for (int i = 1; i < n; ++i) rest += (dims[i].size - 1) * dims[i].step;
+  const int64_t step = dims[0].step, most = dims[0].size - 1;
+  for (int64_t k = moved ? -most : 0; k <= most; ++k) {  // the negative of an answer is one: the first step is >= 0
+    const int64_t to = at + k * step;
+    if (to > rest) break;
+    if (to < -rest) {
+      const int64_t skip = (-rest - to + step - 1) / step;
+      k += skip - 1;
+      continue;
+    }
+    if (--budget < 0 || steps_cancel(dims + 1, n - 1, to, moved || k != 0, budget)) return true;
+  }
+  return false;
+}
+
+inline bool rows_meet(const fd_rows& l) {
+  const RowDim all[4] = {{l.a, l.sa}, {l.b, l.sb}, {l.c, l.sc}, {l.n, l.col}};
+  RowDim dims[4];  // by falling stride
+  int n = 0;
+  for (const RowDim& d : all) {
+    if (d.size <= 0) return false;
+    if (d.size == 1) continue;
+    if (d.step == 0) return true;
+    int i = n++;
+    for (; i > 0 && dims[i - 1].step < d.step; --i) dims[i] = dims[i - 1];
+    dims[i] = d;
+  }
+  int64_t reach = 0;
+  bool nested = true;
+  for (int i = n - 1; i >= 0; --i) {
+    nested = nested && dims[i].step > reach;
+    reach += (dims[i].size - 1) * dims[i].step;
+  }
+  int budget = kMeetSearch;
+  return !nested && steps_cancel(dims, n, 0, false, budget);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // True when the byte ranges [a, a + na) and [b, b + nb) share a byte.

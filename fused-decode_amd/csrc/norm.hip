@@ -459,6 +459,8 @@ int rms_common(bool add, void* y, void* ro, const void* x, const void* r, const 
   const int64_t rows = lx->a * lx->b * lx->c;
   if (rows == 0 || lx->n == 0) return FD_OK;
   if (rows > 0x7fffffffLL) return set_error(FD_EUNSUPPORTED, "too many rows (>= 2^31)");
+  // a row may be stored while another is still read
+  if (add && rows_meet(*lro)) return set_error(FD_EINVAL, "residual_out's elements must not share memory");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const fd_rows& LR = add ? *lr : *lx;
   const fd_rows& LRO = add ? *lro : *ly;

@@ -351,6 +351,7 @@ int rows_common(int mode, const RowsArgs& a, int act_dtype) {
   if (a.rows == 0) return FD_OK;
   if (a.rows > 0x7fffffffLL) return set_error(FD_EUNSUPPORTED, "too many rows (>= 2^31)");
   // outputs are stored while other rows are still read
+  if (add && rows_meet(a.lro)) return set_error(FD_EINVAL, "residual_out's elements must not share memory");
   const int64_t nc = a.rows * n, ns = a.rows * 4, nx = layout_bytes(a.lx), nr = add ? layout_bytes(a.lr) : 0,
                 nro = add ? layout_bytes(a.lro) : 0;
   const int64_t nw = norm && n ? ((n - 1) * a.w_stride + 1) * dtype_bytes(a.w_dtype) : 0;

@@ -24,6 +24,8 @@ from typing import Callable
 
 import torch
 
+from ._layout import shares_memory
+
 ACTIVATION = (torch.float16, torch.bfloat16)
 FLOAT = (torch.float16, torch.bfloat16, torch.float32)
 FP8 = torch.float8_e4m3fn
@@ -275,6 +277,18 @@ def output_like(name: str, ref: str) -> Rule:
     return like(name, ref, optional=True)
 
 
+def no_shared_elements(name: str) -> Rule:
+    """An optional output whose elements all lie at addresses of their own: rows are
+    stored while others are still read, and torch would not write it in place either."""
+
+    def rule(a: dict) -> None:
+        t = a[name]
+        if t is not None and shares_memory(t.shape, t.stride()):
+            raise ValueError(f"{name} has elements that share memory: shape {tuple(t.shape)} strides {t.stride()}")
+
+    return rule
+
+
 # ------------------------------------------------- row-sum (sumsq) entry points
 #
 # The row-sum forms call C entry points that take bare pointers with no extents
@@ -494,7 +508,7 @@ CONTRACT: dict[str, tuple[Rule, ...]] = {
     "rms_norm": (tensor_on_gpu("x"), vector_for("weight", "x"), finite_eps(), output_like("out", "x")),
     "add_rms_norm": (tensor_on_gpu("x"), tensor_on_gpu("residual"), like("residual", "x"),
                      vector_for("weight", "x"), finite_eps(), output_like("out", "x"),
-                     output_like("residual_out", "x")),
+                     output_like("residual_out", "x"), no_shared_elements("residual_out")),
     "rope": (tensor_on_gpu("x"), even_last("x"), broadcast_angles("cos", "x"),
              broadcast_angles("sin", "x"), output_like("out", "x")),
     "swiglu": (tensor_on_gpu("gate"), tensor_on_gpu("up"), like("up", "gate"), output_like("out", "gate")),
@@ -526,7 +540,8 @@ CONTRACT.update({
                      scale_of_rows("scale_out", "x", optional=True)),
     "add_rms_norm_fp8": (tensor_on_gpu("x"), has_rows("x"), tensor_on_gpu("residual"), like("residual", "x"),
                          vector_for("weight", "x"), finite_eps(), codes_out("out", "x"),
-                         scale_of_rows("scale_out", "x", optional=True), output_like("residual_out", "x")),
+                         scale_of_rows("scale_out", "x", optional=True), output_like("residual_out", "x"),
+                         no_shared_elements("residual_out")),
     "linear_w8a8": (tensor_on_gpu("x", (FP8,)), has_rows("x"), scale_of_rows("x_scale", "x"),
                     weight_matrix("weight", "x", fp8=True), inner_dim("x", "weight"), row_scales("scale", "weight"),
                     activation_name("activation", "weight"), bias_of("bias", "x", "weight"),

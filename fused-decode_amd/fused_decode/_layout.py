@@ -90,6 +90,44 @@ def _numel(shape) -> int:
     return total
 
 
+_MEET_SEARCH = 1 << 16
+
+
+def shares_memory(shape, strides) -> bool:
+    """Whether two elements of a tensor of ``shape`` and ``strides`` lie at one address: an
+    expanded dim, windows that run into each other. Dims that, sorted by stride, each step past
+    all that the smaller ones reach hold no such two; for others it is the question whether some
+    steps, not all zero and less than each size, add up to nothing, answered by search, and by
+    yes where the search is longer than ``_MEET_SEARCH``."""
+    if 0 in shape:
+        return False
+    dims = sorted(((int(st), int(n)) for n, st in zip(shape, strides) if n != 1), reverse=True)
+    if any(st == 0 for st, _ in dims):
+        return True
+    reach = [0]  # of the dims behind each
+    for st, n in reversed(dims):
+        reach.append(reach[-1] + (n - 1) * st)
+    reach.reverse()
+    if all(st > rest for (st, _), rest in zip(dims, reach[1:])):
+        return False
+    budget = _MEET_SEARCH
+
+    def cancel(i: int, at: int, moved: bool) -> bool:
+        nonlocal budget
+        if i == len(dims):
+            return at == 0 and moved
+        st, n = dims[i]
+        rest = reach[i + 1]
+        first = max(1 - n if moved else 0, -((rest + at) // st))  # the negative of an answer is one
+        for k in range(first, min(n - 1, (rest - at) // st) + 1):
+            budget -= 1
+            if budget < 0 or cancel(i + 1, at + k * st, moved or k != 0):
+                return True
+        return False
+
+    return cancel(0, 0, False)
+
+
 def joint_layout(inputs: list[torch.Tensor], outputs: list[torch.Tensor]) -> tuple[list[Operand], list[Operand]]:
     """Row layouts for operands of one shape (broadcast inputs already expanded)."""
     shape = inputs[0].shape

@@ -40,7 +40,7 @@ from torch.autograd import forward_ad
 from . import _lib
 from ._checks import check
 from ._lib import ACT_CODE, DTYPE_CODE, FD_EUNSUPPORTED, FdRows, fail, native
-from ._layout import contiguous_strides, plan_rows
+from ._layout import contiguous_strides, plan_rows, shares_memory
 from .fp8 import FP8_DTYPE
 from .ops import (_PLANS, _as_rows, _check_out, _dispatch_modes, _function_modes, _function_modes_watch, _is_tracing,
                   _raw_stream, _remember, _row_add_rows, _sig, _transform, _written)
@@ -155,6 +155,8 @@ def _copied(got: tuple, *outs) -> tuple:
     for v, o in zip(got, outs):
         if o is not None and (o.shape != v.shape or o.dtype != v.dtype or o.device != v.device):
             raise ValueError(f"an output must have shape {tuple(v.shape)} and dtype {v.dtype} on {v.device}")
+        if o is not None and shares_memory(o.shape, o.stride()):
+            raise ValueError(f"an output has elements that share memory: shape {tuple(o.shape)} strides {o.stride()}")
     return tuple(v if o is None else o.copy_(v) for v, o in zip(got, outs))
 
 

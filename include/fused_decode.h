@@ -99,7 +99,9 @@ int fd_rms_norm(void* y, const void* x, const void* w, int w_dtype, int64_t w_st
  * s = x + residual in float32; residual_out = round(s);
  * y = round(s * rsqrt(mean(s^2) + eps) * w) - the norm uses the float32 sum.
  * Replaces kernels.py:343-414 (`rms_out` with residual and residual_out),
- * launched from ops.py:91-119 (`add_rms_norm`). residual_out may alias residual.
+ * launched from ops.py:91-119 (`add_rms_norm`). residual_out may alias residual;
+ * no two of its own elements share memory (FD_EINVAL: broadcast strides, windows
+ * that run into each other).
  */
 int fd_add_rms_norm(void* y, void* residual_out, const void* x, const void* residual,
                     const void* w, int w_dtype, int64_t w_stride, const fd_rows* lx,
@@ -438,7 +440,8 @@ int fd_pre_attn_qkv_fp8_sumsq(void* y, const void* hidden, const void* norm_w, i
  * y is not rounded to act_dtype before. A row whose max|y| is not finite has a NaN scale and
  * NaN codes. codes are rows of n bytes, scale one float a row, both dense and in the order
  * of the row grid; they overlap no input and each other in no byte. residual_out may be x
- * or residual in the same layout and overlaps them in no other way (else FD_EINVAL).
+ * or residual in the same layout and overlaps them in no other way, and no two of its own
+ * elements share memory (else FD_EINVAL).
  * fd_quantize_rows_fp8's codes are x / scale with the division's own rounding.
  * No reference counterpart (its activations are fp16/bf16 only).
  */
