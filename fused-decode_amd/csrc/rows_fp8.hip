@@ -14,6 +14,12 @@
 // integer order puts an infinity above every number and a NaN above that. The scale is
 // never subnormal, so its reciprocal is finite.
 //
+// A sum of squares leaves float32's range before its root does: rows of bfloat16 values above about 1e19, and
+// below 1e-14 where eps is as small as their squares. Such a row is read again, an element at a time, with t times a
+// power of two (off_range) that cancels in t * rsqrt(mean(t^2) + eps). That stands behind the stores, which such a
+// row leaves out (its inputs may be its outputs), where no register waits for it: a second sweep of the registers cost
+// every row some (2048 x 14336 norm 16.7 -> 20.8 us), the same code before the stores too (300 x 20000 7.4 -> 8.6).
+//
 // One pass over memory: a row stays in registers, packed, from its loads to its codes.
 // max|y| = max|t * w| * rsqrt(...), so the sum of squares and the maximum come from one
 // sweep and one exchange between lanes.
@@ -69,6 +75,15 @@ __device__ __forceinline__ void lanes_reduce(float& ss, uint32_t& mx) {
 #undef FD_STEP
 }
 
+// The power of two that a row's values take so that the sum of their squares stays in range, 1 where it is. A sum
+// past the top is at least 2^128, 2^-32 with 2^-80 on the values, where squares that then underflow are too small to
+// count. One below 2^-90 matters beside eps only where that is below 2^-60; its values, below 2^-45, take 2^80, and
+// the square of the smallest bfloat16 value becomes 2^-106. NaN and infinite values stay what they are.
+__device__ __forceinline__ float off_range(float ss, float eps) {
+  if (!(ss <= 3.40282347e38f)) return 0x1p-80f;
+  return ss < 0x1p-90f && eps < 0x1p-60f ? 0x1p80f : 1.f;
+}
+
 // What a row's sums make of its values: code = e4m3(v * inv * r), or NaN.
 struct CodeScale {
   float inv, scale, r;
@@ -100,6 +115,47 @@ __device__ __forceinline__ uint32_t pack4(const float (&v)[4], bool bad) {
 __device__ __forceinline__ float quotient(float y, const CodeScale& q) {
   const float a = y * q.r;
   return __builtin_copysignf(__builtin_fmaf(__builtin_fmaf(-a, q.scale, y), q.r, a), y);
+}
+
+// A row an element at a time by LPR lanes, of which this is lane l: the sum of squares and the maximum of its values
+// times `pre`, in every lane. `sums` and `tops` hold a value a wave where a row is a whole workgroup's.
+template <int LPR, bool NORM, typename Value, typename Weight>
+__device__ __forceinline__ void element_sums(Value value, Weight weight, int64_t n, float pre, int l, float& ss,
+                                             uint32_t& mx, float* sums, uint32_t* tops) {
+  ss = 0.f;
+  mx = 0;
+  for (int64_t k = l; k < n; k += LPR) {
+    const float f = value(k) * pre;
+    if constexpr (NORM) ss += f * f;
+    const uint32_t m = mag_bits(NORM ? f * weight(k) : f);
+    mx = m > mx ? m : mx;
+  }
+  lanes_reduce<(LPR > kWave ? kWave : LPR), NORM>(ss, mx);
+  if constexpr (LPR > kWave) {
+    __syncthreads();  // what they held has been read
+    if (l % kWave == 0) {
+      sums[l / kWave] = ss;
+      tops[l / kWave] = mx;
+    }
+    __syncthreads();
+    ss = 0.f;
+    for (int i = 0; i < LPR / kWave; ++i) {
+      ss += sums[i];
+      mx = tops[i] > mx ? tops[i] : mx;
+    }
+  }
+}
+
+// The codes of such a row, and its sum with the residual.
+template <typename T, int MODE, int LPR, typename Value, typename Weight>
+__device__ __forceinline__ void element_codes(uint8_t* codes, T* ro, int64_t ro_col, Value value, Weight weight,
+                                              int64_t n, float pre, int l, const CodeScale& q) {
+  for (int64_t k = l; k < n; k += LPR) {
+    const float f = value(k);
+    if constexpr (MODE == ROWS_ADD) ro[k * ro_col] = from_f32<T>(f);
+    const float v = MODE != ROWS_PLAIN ? f * pre * weight(k) * q.inv * q.r : quotient(f, q);
+    codes[k] = q.bad ? 0x7f : (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false);
+  }
 }
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -158,9 +214,9 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows_fp8_kernel(
     }
   }
   lanes_reduce<(LPR > kWave ? kWave : LPR), NORM>(ss, mx);
+  __shared__ float sums[NWAVE > 1 ? NWAVE : 1];
+  __shared__ uint32_t tops[NWAVE > 1 ? NWAVE : 1];
   if constexpr (NWAVE > 1) {
-    __shared__ float sums[NWAVE];
-    __shared__ uint32_t tops[NWAVE];
     if (threadIdx.x % kWave == 0) {
       sums[threadIdx.x / kWave] = ss;
       tops[threadIdx.x / kWave] = mx;
@@ -173,15 +229,19 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows_fp8_kernel(
       mx = tops[i] > mx ? tops[i] : mx;
     }
   }
+  float pre = NORM ? off_range(ss, eps) : 1.f;  // the same in all of the row's lanes
+  if constexpr (NORM && LPR >= kWave)
+    pre = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, pre)));
   const CodeScale q = row_scale(NORM ? rsqrtf(ss / (float)n + eps) : 1.f, mx);
   if (!live) return;
   if (l == 0) scale[row] = q.scale;
   uint8_t* cr = codes + (int64_t)row * n;
   T* ror = ADD ? ro + row_off(lro, p) : nullptr;
+  const int stored = pre == 1.f ? nv : 0;  // vectors; none of a row out of range, whose inputs may be its outputs
 #pragma unroll
   for (int j = 0; j < VPL; ++j) {
     const int k = first(j * LPR + l);
-    if (j * LPR + l >= nv) continue;
+    if (j * LPR + l >= stored) continue;
     u32x2 o;
     V8 s;
 #pragma unroll
@@ -201,6 +261,24 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rows_fp8_kernel(
     if constexpr (ADD) store8_any<T>(ror + k, s);
     __builtin_nontemporal_store(o, reinterpret_cast<u32x2_any*>(cr + k));
   }
+  if constexpr (NORM) {
+    if (pre != 1.f) {  // in all of the row's lanes, so in every lane that meets at a barrier
+      uint32_t at = row;
+      int lane = l;
+      if constexpr (LPR > kWave) at = __builtin_amdgcn_readfirstlane(at);
+      asm volatile("" : "+v"(lane));  // made here, not ahead in registers that the sweep needs
+      const RowPos p = row_pos(grid, at);
+      const T* xr = x + row_off(lx, p);
+      const T* rr = ADD ? r + row_off(lr, p) : nullptr;
+      auto element = [&](int64_t k) { return ADD ? to_f32(xr[k]) + to_f32(rr[k]) : to_f32(xr[k]); };
+      auto weight = [&](int64_t k) { return to_f32(w[k]); };
+      element_sums<LPR, NORM>(element, weight, n, pre, lane, ss, mx, sums, tops);
+      const CodeScale q = row_scale(rsqrtf(ss / (float)n + eps * pre * pre), mx);
+      if (lane == 0) scale[at] = q.scale;
+      element_codes<T, MODE, LPR>(codes + (int64_t)at * n, ADD ? ro + row_off(lro, p) : nullptr, 1, element, weight, n,
+                                  pre, lane, q);
+    }
+  }
 }
 
 template <typename T, int MODE>
@@ -219,35 +297,18 @@ __global__ __launch_bounds__(256) void rows_fp8_gen_kernel(uint8_t* codes, float
     const float f = to_f32(xr[k * lx.col]);
     return ADD ? f + to_f32(rr[k * lr.col]) : f;
   };
-  float ss = 0.f;
-  uint32_t mx = 0;
-  for (int64_t k = threadIdx.x; k < n; k += 256) {
-    const float f = value(k);
-    if constexpr (NORM) ss += f * f;
-    const uint32_t m = mag_bits(NORM ? f * load_any(w, w_dtype, k * w_stride) : f);
-    mx = m > mx ? m : mx;
+  auto weight = [&](int64_t k) { return load_any(w, w_dtype, k * w_stride); };
+  float ss, pre = 1.f;
+  uint32_t mx;
+  element_sums<256, NORM>(value, weight, n, pre, (int)threadIdx.x, ss, mx, sums, tops);
+  if constexpr (NORM) {
+    pre = off_range(ss, eps);
+    if (pre != 1.f) element_sums<256, NORM>(value, weight, n, pre, (int)threadIdx.x, ss, mx, sums, tops);
   }
-  lanes_reduce<kWave, NORM>(ss, mx);
-  if (threadIdx.x % kWave == 0) {
-    sums[threadIdx.x / kWave] = ss;
-    tops[threadIdx.x / kWave] = mx;
-  }
-  __syncthreads();
-  ss = 0.f;
-  for (int i = 0; i < 4; ++i) {
-    ss += sums[i];
-    mx = tops[i] > mx ? tops[i] : mx;
-  }
-  const CodeScale q = row_scale(NORM && n ? rsqrtf(ss / (float)n + eps) : 1.f, mx);
+  const CodeScale q = row_scale(NORM && n ? rsqrtf(ss / (float)n + eps * pre * pre) : 1.f, mx);
   if (threadIdx.x == 0) scale[row] = q.scale;
-  uint8_t* cr = codes + (int64_t)row * n;
-  T* ror = ADD ? ro + row_off(lro, p) : nullptr;
-  for (int64_t k = threadIdx.x; k < n; k += 256) {
-    const float f = value(k);
-    if constexpr (ADD) ror[k * lro.col] = from_f32<T>(f);
-    const float v = NORM ? f * load_any(w, w_dtype, k * w_stride) * q.inv * q.r : quotient(f, q);
-    cr[k] = q.bad ? 0x7f : (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false);
-  }
+  element_codes<T, MODE, 256>(codes + (int64_t)row * n, ADD ? ro + row_off(lro, p) : nullptr, lro.col, value, weight, n,
+                              pre, (int)threadIdx.x, q);
 }
 
 namespace {
