@@ -39,7 +39,7 @@ from torch.autograd import forward_ad
 
 from . import _lib
 from ._checks import check
-from ._lib import ACT_CODE, DTYPE_CODE, FD_EUNSUPPORTED, FdRows, fail, native
+from ._lib import ACT_CODE, DTYPE_CODE, FD_EINVAL, FD_EUNSUPPORTED, FdRows, FusedDecodeError, fail, native
 from ._layout import contiguous_strides, plan_rows, shares_memory
 from .fp8 import FP8_DTYPE
 from .ops import (_PLANS, _as_rows, _check_out, _dispatch_modes, _function_modes, _function_modes_watch, _is_tracing,
@@ -160,6 +160,12 @@ def _copied(got: tuple, *outs) -> tuple:
     return tuple(v if o is None else o.copy_(v) for v, o in zip(got, outs))
 
 
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the bytes from first to last element of two tensors overlap, as the library asks it."""
+    end = lambda t: t.data_ptr() + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
 def _plan_rows_fp8(op, x, weight, residual, eps, out, scale_out, residual_out):
     """Launch plan of a row operator for one argument signature."""
     add, norm = op == "add_rms_norm_fp8", op != "quantize_rows_fp8"
@@ -203,6 +209,8 @@ def _plan_rows_fp8(op, x, weight, residual, eps, out, scale_out, residual_out):
             s = torch.empty_like(scale_like) if scale_out is None else scale_out
             ro = torch.empty_like(sum_like) if residual_out is None or staged else residual_out
             if staged:
+                if residual_out is not None and any(o is not None and _meet(o, residual_out) for o in (out, scale_out)):
+                    raise FusedDecodeError("fd_add_rms_norm_fp8", FD_EINVAL, "the outputs must not overlap each other")
                 x, r = x.contiguous(), r.contiguous()
             status = call(c.data_ptr(), s.data_ptr(), ro.data_ptr(), x.data_ptr(), r.data_ptr(), w.data_ptr(), wcode,
                           wstride, lx, lr, lro, eps, act, _raw_stream(dev))

@@ -1,0 +1,32 @@
+"""Calls of the operators with 8-bit activations that reach a launch by another way than the plain one, on the CPU with
+the library's calls replaced by ones that only note their names."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from test_w8a8 import E4M3, arguments, calls, cuda  # noqa: F401 (a fixture)
+
+from fused_decode import _lib as L
+from fused_decode import w8a8
+
+
+def unmergeable(dtype):
+    """Rows of 8 in four leading dims of which no two merge."""
+    return torch.zeros(5, 4, 3, 2, 8, dtype=dtype).permute(3, 2, 1, 0, 4)
+
+
+def test_gathered_rows_refuse_outputs_over_each_other(calls):  # noqa: F811
+    """The sums come back by a copy, behind the codes: it must not land on them."""
+    x, r, w = unmergeable(torch.float16), unmergeable(torch.float16), torch.ones(8)
+    memory = torch.zeros(4 * 960, dtype=torch.uint8)
+    residual_out = memory[:1920].view(torch.float16).view(5, 4, 3, 2, 8).permute(3, 2, 1, 0, 4)
+    codes = lambda at: memory[at : at + 960].view(E4M3).view(x.shape)
+    scale = lambda at: memory[at : at + 480].view(torch.float32).view(x.shape[:-1])
+    for out, scale_out in ((codes(0), None), (codes(1919), None), (None, scale(0)), (codes(1920), scale(1916))):
+        with pytest.raises(L.FusedDecodeError, match="overlap"):
+            w8a8.add_rms_norm_fp8(x, r, w, out=out, scale_out=scale_out, residual_out=residual_out)
+    assert calls == []
+    got = w8a8.add_rms_norm_fp8(x, r, w, out=codes(1920), scale_out=scale(2880), residual_out=residual_out)
+    assert got[2] is residual_out and calls == ["add_rms_norm_fp8"]
+    w8a8.add_rms_norm_fp8(x, residual_out, w, residual_out=residual_out)
