@@ -666,8 +666,10 @@ extern "C" int fd_linear_w8a8(void* y, const void* x8, const float* x_scale, con
   if (M == 0 || N == 0) return FD_OK;
   if (!y || !x_scale || !w_scale || (K > 0 && (!x8 || !w8))) return set_error(FD_EINVAL, "null pointer argument");
   if (M > kMostIndex || N > kMostIndex || K > kMostIndex) return set_error(FD_EUNSUPPORTED, "too large");
+  const int64_t cols = swiglu ? N / 2 : N;
+  if (rows_meet(fd_rows{1, 1, M, 0, 0, sym, syn, cols})) return set_error(FD_EINVAL, "y's elements must not share memory");
   // tiles are stored while other workgroups still read their operands
-  const int64_t cols = swiglu ? N / 2 : N, ny = span_bytes(M, cols, sym, syn, 2);
+  const int64_t ny = span_bytes(M, cols, sym, syn, 2);
   if (overlaps(y, ny, x8, span_bytes(M, K, sxm, 1, 1)) || overlaps(y, ny, w8, span_bytes(N, K, swn, 1, 1)) ||
       overlaps(y, ny, x_scale, M * 4) || overlaps(y, ny, w_scale, N * 4) ||
       (bias && overlaps(y, ny, bias, span_bytes(1, N, 0, sb, dtype_bytes(bias_dtype)))) ||

@@ -469,7 +469,8 @@ int fd_add_rms_norm_fp8(void* codes, float* scale, void* residual_out, const voi
  * rows that are not so, or whose K is no multiple of 16 (without it FD_EUNSUPPORTED), and,
  * where there are few output tiles, the float32 sums of K splits, which are added in a fixed
  * order; less lowers the split, down to none. y may be row_add element for element and
- * overlaps no operand otherwise (FD_EUNSUPPORTED). No reference counterpart.
+ * overlaps no operand otherwise (FD_EUNSUPPORTED); no two of its own elements share memory
+ * (FD_EINVAL). No reference counterpart.
  */
 int fd_linear_w8a8(void* y, const void* x8, const float* x_scale, const void* w8,
                    const float* w_scale, const void* bias, int bias_dtype, int activation,

@@ -113,3 +113,18 @@ def test_a_recorded_call_refuses_them():
         w8a8._copied(got, torch.zeros(224).unfold(0, 64, 32), None)
     out = torch.ones(6, 64)
     assert w8a8._copied(got, out, None)[0] is out and bool((out == 0).all())
+
+
+@nogpu
+def test_the_product_refuses_an_output_whose_elements_share_memory():
+    """40 x 64 outputs, 40 x 32 with SwiGLU; a layout that passes is then refused for its overlap with the weights."""
+    def linear(y, sym, syn, act=0, m=40):
+        return L.lib().fd_linear_w8a8(y, X, S, W, S + 0x1000, None, 0, act, None, 0, m, 64, 128, 128, 128, 1, 0, 0, sym, syn,
+                                      None, 0, 0, None)
+
+    for sym, syn in ((0, 1), (63, 1), (64, 0), (1, 39), (128, 4)):
+        assert share(linear(Y, sym, syn)), (sym, syn)
+    assert share(linear(Y, 31, 1, act=5)) and share(linear(Y, 0, 0, m=1))
+    for sym, syn, m in ((64, 1, 40), (70, 1, 40), (1, 40, 40), (128, 2, 40), (0, 1, 1)):
+        assert linear(W, sym, syn, m=m) == L.FD_EUNSUPPORTED and b"overlap" in L.lib().fd_last_error()
+    assert linear(W, 32, 1, act=5) == L.FD_EUNSUPPORTED
