@@ -29,6 +29,7 @@ from __future__ import annotations
 
 import math
 import os
+from numbers import Number
 from typing import Callable, NamedTuple
 
 import torch
@@ -92,8 +93,16 @@ _PLAN_LIMIT = 4096
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _lib.stream_of_device
 
 
+def _by_value(part) -> bool:
+    """Whether a key's part is equal only to parts that say the same: a tensor given as eps is equal to
+    itself whatever it holds by then."""
+    if isinstance(part, tuple):
+        return all(map(_by_value, part))
+    return part is None or isinstance(part, (str, bytes, Number, torch.dtype))
+
+
 def _remember(key, plan: Plan) -> Plan:
-    if key is not None:
+    if key is not None and _by_value(key):
         if len(_PLANS) >= _PLAN_LIMIT:
             _PLANS.clear()
         _PLANS[key] = plan

@@ -8,7 +8,7 @@ import torch
 from test_w8a8 import E4M3, arguments, calls, cuda  # noqa: F401 (a fixture)
 
 from fused_decode import _lib as L
-from fused_decode import w8a8
+from fused_decode import ops, w8a8
 
 
 def unmergeable(dtype):
@@ -30,3 +30,23 @@ def test_gathered_rows_refuse_outputs_over_each_other(calls):  # noqa: F811
     got = w8a8.add_rms_norm_fp8(x, r, w, out=codes(1920), scale_out=scale(2880), residual_out=residual_out)
     assert got[2] is residual_out and calls == ["add_rms_norm_fp8"]
     w8a8.add_rms_norm_fp8(x, residual_out, w, residual_out=residual_out)
+
+
+def test_an_eps_that_changes_is_read_again(calls, monkeypatch):  # noqa: F811
+    """A tensor, or a number of numpy's, given as eps: plans are not kept by the tensor's identity."""
+    import numpy as np
+
+    x, w, q, s = arguments()
+    seen = []
+    monkeypatch.setattr(w8a8, "check", lambda op, **a: {"eps": float(a["eps"])})
+    monkeypatch.setattr(type(calls), "rms_norm_fp8", lambda self, *a: seen.append(a[7]) or L.FD_OK, raising=False)
+    eps = torch.tensor(0.5)
+    w8a8.rms_norm_fp8(x, w, eps)
+    eps.fill_(0.25)
+    w8a8.rms_norm_fp8(x, w, eps)
+    w8a8.rms_norm_fp8(x, w, np.float32(0.125))
+    w8a8.rms_norm_fp8(x, w, 0.125)
+    assert seen == [0.5, 0.25, 0.125, 0.125]
+    assert len(ops._PLANS) == 1
+    ops._remember(("op", x.shape, x.stride(), (torch.float16, None, b"env"), 1e-6, True), lambda: None)
+    assert len(ops._PLANS) == 2
