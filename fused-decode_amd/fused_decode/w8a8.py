@@ -85,13 +85,15 @@ def quantize_rows_fp8(
     """E4M3 codes of ``x``'s rows (its last dimension) and their float32 scales ``x.shape[:-1]``, in one
     launch. For finite rows the codes and scales that ``quantize_fp8`` gives the same rows."""
     try:
-        if _watched() or (_grad() and x.requires_grad) or x.is_neg():
-            return _copied(torch.ops.fused_decode.quantize_rows_fp8(x), out, scale_out)
-        key = ("quantize_rows_fp8", x.shape, x.stride(), x.dtype, x.get_device(), None if out is None else _out_sig(out),
-               None if scale_out is None else _out_sig(scale_out))
-        plan = _PLANS.get(key)
+        recorded = _watched() or (_grad() and x.requires_grad) or x.is_neg()
+        if not recorded:
+            key = ("quantize_rows_fp8", x.shape, x.stride(), x.dtype, x.get_device(),
+                   None if out is None else _out_sig(out), None if scale_out is None else _out_sig(scale_out))
+            plan = _PLANS.get(key)
     except AttributeError:  # not a tensor: let the contract say so
-        key, plan = None, None
+        recorded, key, plan = False, None, None
+    if recorded:
+        return _copied(torch.ops.fused_decode.quantize_rows_fp8(x), out, scale_out)
     if plan is None:
         plan = _remember(key, _plan_rows_fp8("quantize_rows_fp8", x, None, None, 0.0, out, scale_out, None))
     return plan(x, None, None, out, scale_out, None)
@@ -108,15 +110,17 @@ def rms_norm_fp8(
     """``rms_norm`` with E4M3 codes and float32 row scales for its result. ``weight`` is ``(N,)``
     (float16, bfloat16 or float32)."""
     try:
-        if (_watched() or (_grad() and (x.requires_grad or weight.requires_grad)) or x.is_neg()
-                or weight.is_neg()):
-            return _copied(torch.ops.fused_decode.rms_norm_fp8(x, weight, eps), out, scale_out)
-        key = ("rms_norm_fp8", x.shape, x.stride(), x.dtype, x.get_device(), weight.shape, weight.stride(), weight.dtype,
-               weight.get_device(), eps, None if out is None else _out_sig(out),
-               None if scale_out is None else _out_sig(scale_out))
-        plan = _PLANS.get(key)
+        recorded = (_watched() or (_grad() and (x.requires_grad or weight.requires_grad)) or x.is_neg()
+                    or weight.is_neg())
+        if not recorded:
+            key = ("rms_norm_fp8", x.shape, x.stride(), x.dtype, x.get_device(), weight.shape, weight.stride(),
+                   weight.dtype, weight.get_device(), eps, None if out is None else _out_sig(out),
+                   None if scale_out is None else _out_sig(scale_out))
+            plan = _PLANS.get(key)
     except (AttributeError, TypeError):  # a non-tensor or unhashable argument: checked below
-        key, plan = None, None
+        recorded, key, plan = False, None, None
+    if recorded:
+        return _copied(torch.ops.fused_decode.rms_norm_fp8(x, weight, eps), out, scale_out)
     if plan is None:
         plan = _remember(key, _plan_rows_fp8("rms_norm_fp8", x, weight, None, eps, out, scale_out, None))
     return plan(x, weight, None, out, scale_out, None)
@@ -135,16 +139,19 @@ def add_rms_norm_fp8(
     """``add_rms_norm`` with E4M3 codes and float32 row scales for the norm of the float32 sum:
     ``(codes, scale, residual_out)``. ``residual_out=residual`` updates the residual stream in place."""
     try:
-        if (_watched() or (_grad() and (x.requires_grad or residual.requires_grad or weight.requires_grad))
-                or x.is_neg() or residual.is_neg() or weight.is_neg()):
-            return _copied(torch.ops.fused_decode.add_rms_norm_fp8(x, residual, weight, eps), out, scale_out, residual_out)
-        key = ("add_rms_norm_fp8", x.shape, x.stride(), x.dtype, x.get_device(), residual.shape, residual.stride(),
-               residual.dtype, residual.get_device(), weight.shape, weight.stride(), weight.dtype, weight.get_device(),
-               eps, None if out is None else _out_sig(out), None if scale_out is None else _out_sig(scale_out),
-               None if residual_out is None else _out_sig(residual_out))
-        plan = _PLANS.get(key)
+        recorded = (_watched() or (_grad() and (x.requires_grad or residual.requires_grad or weight.requires_grad))
+                    or x.is_neg() or residual.is_neg() or weight.is_neg())
+        if not recorded:
+            key = ("add_rms_norm_fp8", x.shape, x.stride(), x.dtype, x.get_device(), residual.shape, residual.stride(),
+                   residual.dtype, residual.get_device(), weight.shape, weight.stride(), weight.dtype,
+                   weight.get_device(), eps, None if out is None else _out_sig(out),
+                   None if scale_out is None else _out_sig(scale_out),
+                   None if residual_out is None else _out_sig(residual_out))
+            plan = _PLANS.get(key)
     except (AttributeError, TypeError):
-        key, plan = None, None
+        recorded, key, plan = False, None, None
+    if recorded:
+        return _copied(torch.ops.fused_decode.add_rms_norm_fp8(x, residual, weight, eps), out, scale_out, residual_out)
     if plan is None:
         plan = _remember(key, _plan_rows_fp8("add_rms_norm_fp8", x, weight, residual, eps, out, scale_out, residual_out))
     return plan(x, weight, residual, out, scale_out, residual_out)
@@ -153,6 +160,8 @@ def add_rms_norm_fp8(
 def _copied(got: tuple, *outs) -> tuple:
     """A custom op's results, copied where outputs are given."""
     for v, o in zip(got, outs):
+        if o is not None and not isinstance(o, torch.Tensor):
+            raise TypeError(f"an output must be a tensor or None, got {type(o).__name__}")
         if o is not None and (o.shape != v.shape or o.dtype != v.dtype or o.device != v.device):
             raise ValueError(f"an output must have shape {tuple(v.shape)} and dtype {v.dtype} on {v.device}")
         if o is not None and shares_memory(o.shape, o.stride()):
@@ -265,21 +274,23 @@ def linear_w8a8(
     Any number of rows and any K; codes whose rows are not 16-byte aligned, whose K is no multiple of 16 or
     whose stride along K is not 1 are copied first."""
     try:
-        if _watched() or (_grad() and (x_scale.requires_grad or scale.requires_grad or x.requires_grad
-                                       or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                       or (row_add is not None and row_add.requires_grad))) \
-                or x_scale.is_neg() or scale.is_neg() or (bias is not None and bias.is_neg()) \
-                or (row_add is not None and row_add.is_neg()):
-            y = torch.ops.fused_decode.linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add,
-                                                   dtype or (torch.bfloat16 if out is None else out.dtype))
-            return _copied((y,), out)[0]
-        key = ("linear_w8a8", x.shape, x.stride(), x.dtype, x.get_device(), x_scale.shape, x_scale.stride(), x_scale.dtype,
-               x_scale.get_device(), weight.shape, weight.stride(), weight.dtype, weight.get_device(), scale.shape,
-               scale.stride(), scale.dtype, scale.get_device(), None if bias is None else _sig(bias), activation,
-               None if row_add is None else _sig(row_add), None if out is None else _out_sig(out), dtype)
-        plan = _PLANS.get(key)
+        recorded = (_watched() or (_grad() and (x_scale.requires_grad or scale.requires_grad or x.requires_grad
+                                                or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                                or (row_add is not None and row_add.requires_grad)))
+                    or x_scale.is_neg() or scale.is_neg() or (bias is not None and bias.is_neg())
+                    or (row_add is not None and row_add.is_neg()))
+        if not recorded:
+            key = ("linear_w8a8", x.shape, x.stride(), x.dtype, x.get_device(), x_scale.shape, x_scale.stride(),
+                   x_scale.dtype, x_scale.get_device(), weight.shape, weight.stride(), weight.dtype, weight.get_device(),
+                   scale.shape, scale.stride(), scale.dtype, scale.get_device(), None if bias is None else _sig(bias),
+                   activation, None if row_add is None else _sig(row_add), None if out is None else _out_sig(out), dtype)
+            plan = _PLANS.get(key)
     except (AttributeError, TypeError):  # a non-tensor or unhashable argument: checked below
-        key, plan = None, None
+        recorded, key, plan = False, None, None
+    if recorded:
+        y = torch.ops.fused_decode.linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add,
+                                               dtype or getattr(out, "dtype", torch.bfloat16))
+        return _copied((y,), out)[0]
     if plan is None:
         plan = _remember(key, _plan_linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add, out, dtype))
     return plan(x, x_scale, weight, scale, bias, row_add, out)

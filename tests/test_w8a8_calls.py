@@ -50,3 +50,29 @@ def test_an_eps_that_changes_is_read_again(calls, monkeypatch):  # noqa: F811
     assert len(ops._PLANS) == 1
     ops._remember(("op", x.shape, x.stride(), (torch.float16, None, b"env"), 1e-6, True), lambda: None)
     assert len(ops._PLANS) == 2
+
+
+@pytest.mark.parametrize("error", [AttributeError, TypeError, RuntimeError])
+def test_an_error_of_the_custom_op_is_the_calls(calls, monkeypatch, error):  # noqa: F811
+    """What a trace or a transform raises is not taken for a wrong argument, behind which the launch would follow."""
+    x, w, q, s = arguments()
+
+    class Raises:
+        def __getattr__(self, name):
+            def op(*args):
+                raise error(name)
+            return op
+
+    monkeypatch.setattr(torch.ops, "fused_decode", Raises(), raising=False)
+    leaf, c, t = x.clone().requires_grad_(), torch.zeros(3, 64, dtype=E4M3), torch.ones(3)
+    for call in (lambda: w8a8.quantize_rows_fp8(leaf), lambda: w8a8.rms_norm_fp8(leaf, w),
+                 lambda: w8a8.add_rms_norm_fp8(x, leaf, w), lambda: w8a8.linear_w8a8(c, t, q, torch._neg_view(s))):
+        with pytest.raises(error, match="fp8|w8a8"):
+            call()
+    assert calls == []
+
+
+def test_recorded_calls_name_an_output_that_is_no_tensor():
+    x = torch.zeros(3, 64)
+    with pytest.raises(TypeError, match="output"):
+        w8a8._copied((x,), 3)
