@@ -36,6 +36,7 @@ import math
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._checks import check
@@ -48,15 +49,22 @@ from .ops import (_PLANS, _as_rows, _check_out, _dispatch_modes, _function_modes
 __all__ = ["add_rms_norm_fp8", "linear_w8a8", "quantize_rows_fp8", "rms_norm_fp8"]
 
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else (lambda: -1)
-_grad = torch.is_grad_enabled
+_grad, _is_compiling = torch.is_grad_enabled, torch.compiler.is_compiling
 _MOST_STRIDE = 1 << 23  # bytes between rows that the product's kernels take as they are; others are copied
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
 
 
 def _watched() -> bool:
     """Whether something would record or transform a call, which a launch on bare pointers would be missing from
     (a tensor whose negation is still to be made takes the same way: the dispatcher makes it)."""
-    return bool(torch.compiler.is_compiling() or forward_ad._current_level >= 0 or _transform() is not None
-                or _is_tracing() or _dispatch_modes() or (_function_modes() and _function_modes_watch()))
+    return (_is_compiling() or forward_ad._current_level >= 0 or _transform() is not None or _is_tracing()
+            or _dispatch_modes() > 0 or (_function_modes() > 0 and _function_modes_watch()))
+
+
+def _subclasses(*tensors) -> bool:
+    """Whether one of these is of a tensor subclass, whose memory may be another tensor's and which torch's calls let
+    act for itself: the custom op does. (Asked where a class is not in ``_PLAIN``; a list or a number is the contract's.)"""
+    return any(type(t) not in _PLAIN and isinstance(t, torch.Tensor) for t in tensors)
 
 
 def _out_sig(t: torch.Tensor) -> tuple:
@@ -85,7 +93,9 @@ def quantize_rows_fp8(
     """E4M3 codes of ``x``'s rows (its last dimension) and their float32 scales ``x.shape[:-1]``, in one
     launch. For finite rows the codes and scales that ``quantize_fp8`` gives the same rows."""
     try:
-        recorded = _watched() or (_grad() and x.requires_grad) or x.is_neg()
+        recorded = (_watched() or (_grad() and x.requires_grad) or x.is_neg()
+                    or (not (x.__class__ in _PLAIN and out.__class__ in _PLAIN and scale_out.__class__ in _PLAIN)
+                        and _subclasses(x, out, scale_out)))
         if not recorded:
             key = ("quantize_rows_fp8", x.shape, x.stride(), x.dtype, x.get_device(),
                    None if out is None else _out_sig(out), None if scale_out is None else _out_sig(scale_out))
@@ -110,8 +120,9 @@ def rms_norm_fp8(
     """``rms_norm`` with E4M3 codes and float32 row scales for its result. ``weight`` is ``(N,)``
     (float16, bfloat16 or float32)."""
     try:
-        recorded = (_watched() or (_grad() and (x.requires_grad or weight.requires_grad)) or x.is_neg()
-                    or weight.is_neg())
+        recorded = (_watched() or (_grad() and (x.requires_grad or weight.requires_grad)) or x.is_neg() or weight.is_neg()
+                    or (not (x.__class__ in _PLAIN and weight.__class__ in _PLAIN and out.__class__ in _PLAIN
+                             and scale_out.__class__ in _PLAIN) and _subclasses(x, weight, out, scale_out)))
         if not recorded:
             key = ("rms_norm_fp8", x.shape, x.stride(), x.dtype, x.get_device(), weight.shape, weight.stride(),
                    weight.dtype, weight.get_device(), eps, None if out is None else _out_sig(out),
@@ -139,8 +150,13 @@ def add_rms_norm_fp8(
     """``add_rms_norm`` with E4M3 codes and float32 row scales for the norm of the float32 sum:
     ``(codes, scale, residual_out)``. ``residual_out=residual`` updates the residual stream in place."""
     try:
-        recorded = (_watched() or (_grad() and (x.requires_grad or residual.requires_grad or weight.requires_grad))
-                    or x.is_neg() or residual.is_neg() or weight.is_neg())
+        recorded = (_watched()
+                    or (_grad() and (x.requires_grad or residual.requires_grad or weight.requires_grad))
+                    or x.is_neg() or residual.is_neg() or weight.is_neg()
+                    or (not (x.__class__ in _PLAIN and residual.__class__ in _PLAIN and weight.__class__ in _PLAIN
+                             and out.__class__ in _PLAIN and scale_out.__class__ in _PLAIN
+                             and residual_out.__class__ in _PLAIN)
+                        and _subclasses(x, residual, weight, out, scale_out, residual_out)))
         if not recorded:
             key = ("add_rms_norm_fp8", x.shape, x.stride(), x.dtype, x.get_device(), residual.shape, residual.stride(),
                    residual.dtype, residual.get_device(), weight.shape, weight.stride(), weight.dtype,
@@ -225,9 +241,11 @@ def _plan_rows_fp8(op, x, weight, residual, eps, out, scale_out, residual_out):
                           wstride, lx, lr, lro, eps, act, _raw_stream(dev))
             if status:
                 fail("fd_add_rms_norm_fp8", status)
-            if residual_out is not None:
-                ro = residual_out.copy_(ro) if staged else _written(residual_out)
-            return c if out is None else _written(out), s if scale_out is None else _written(scale_out), ro
+            if staged and residual_out is not None:
+                ro = residual_out.copy_(ro)
+            if out is not None or scale_out is not None or residual_out is not None:
+                increment_version([t for t in (out, scale_out, residual_out) if t is not None])
+            return c, s, ro
         return run_add
 
     def run(x, w, r, out, scale_out, residual_out):
@@ -245,7 +263,9 @@ def _plan_rows_fp8(op, x, weight, residual, eps, out, scale_out, residual_out):
             status = call(c.data_ptr(), s.data_ptr(), x.data_ptr(), lx, act, _raw_stream(dev))
         if status:
             fail("fd_" + op, status)
-        return c if out is None else _written(out), s if scale_out is None else _written(scale_out)
+        if out is not None or scale_out is not None:
+            increment_version([t for t in (out, scale_out) if t is not None])
+        return c, s
     return run
 
 
@@ -274,11 +294,16 @@ def linear_w8a8(
     Any number of rows and any K; codes whose rows are not 16-byte aligned, whose K is no multiple of 16 or
     whose stride along K is not 1 are copied first."""
     try:
-        recorded = (_watched() or (_grad() and (x_scale.requires_grad or scale.requires_grad or x.requires_grad
-                                                or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                                or (row_add is not None and row_add.requires_grad)))
+        recorded = (_watched()
+                    or (_grad() and (x_scale.requires_grad or scale.requires_grad or x.requires_grad
+                                     or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                     or (row_add is not None and row_add.requires_grad)))
                     or x_scale.is_neg() or scale.is_neg() or (bias is not None and bias.is_neg())
-                    or (row_add is not None and row_add.is_neg()))
+                    or (row_add is not None and row_add.is_neg())
+                    or (not (x.__class__ in _PLAIN and x_scale.__class__ in _PLAIN and weight.__class__ in _PLAIN
+                             and scale.__class__ in _PLAIN and bias.__class__ in _PLAIN and row_add.__class__ in _PLAIN
+                             and out.__class__ in _PLAIN)
+                        and _subclasses(x, x_scale, weight, scale, bias, row_add, out)))
         if not recorded:
             key = ("linear_w8a8", x.shape, x.stride(), x.dtype, x.get_device(), x_scale.shape, x_scale.stride(),
                    x_scale.dtype, x_scale.get_device(), weight.shape, weight.stride(), weight.dtype, weight.get_device(),

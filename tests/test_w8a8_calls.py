@@ -76,3 +76,73 @@ def test_recorded_calls_name_an_output_that_is_no_tensor():
     x = torch.zeros(3, 64)
     with pytest.raises(TypeError, match="output"):
         w8a8._copied((x,), 3)
+
+
+class Watching(torch.Tensor):
+    """A subclass that notes the functions it meets."""
+
+    seen: list = []
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        cls.seen.append(str(func))
+        return super().__torch_function__(func, types, args, kwargs or {})
+
+
+class Holder(torch.Tensor):
+    """A wrapper without memory of its own: a launch on its pointer would read none of the held tensor's."""
+
+    met: list = []
+
+    @staticmethod
+    def __new__(cls, held):
+        return torch.Tensor._make_wrapper_subclass(cls, held.shape, strides=held.stride(), dtype=held.dtype,
+                                                   device=held.device)
+
+    def __init__(self, held):
+        self.held = held
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        cls.met.append(str(func))
+        return func(*[a.held if isinstance(a, Holder) else a for a in args], **(kwargs or {}))
+
+
+def each_operator():
+    """(name, argument count, call of those tensors) for every operator."""
+    x, w, q, s = arguments()
+    c, t, r = torch.zeros(3, 64, dtype=E4M3), torch.ones(3), torch.zeros(3, 30)
+    return (("quantize_rows_fp8", [x], w8a8.quantize_rows_fp8), ("rms_norm_fp8", [x, w], w8a8.rms_norm_fp8),
+            ("add_rms_norm_fp8", [x, x.clone(), w], w8a8.add_rms_norm_fp8),
+            ("linear_w8a8", [c, t, q, s, s.clone(), r], lambda *a: w8a8.linear_w8a8(*a[:5], row_add=a[5])))
+
+
+def test_subclasses_see_the_call(calls):  # noqa: F811
+    """Each argument in turn; a Parameter is no such subclass."""
+    for name, args, call in each_operator():
+        for i in range(len(args)):
+            given = list(args)
+            Watching.seen.clear()
+            given[i] = args[i].as_subclass(Watching)
+            call(*given)
+            assert any(f"fused_decode.{name}" in f for f in Watching.seen), (name, i)
+            Holder.met.clear()
+            given[i] = Holder(args[i])
+            call(*given)
+            assert any(f.startswith(f"fused_decode.{name}") for f in Holder.met), (name, i)
+            given[i] = torch.nn.Parameter(args[i], requires_grad=False)
+            Watching.seen.clear(), Holder.met.clear()
+            call(*given)
+            assert not Watching.seen and not Holder.met
+
+
+def test_a_subclass_as_output_is_written_by_torch(calls):  # noqa: F811
+    x, w, q, s = arguments()
+    out, t = Holder(torch.empty(3, 30, dtype=torch.bfloat16)), torch.ones(3)
+    Holder.met.clear()
+    assert w8a8.linear_w8a8(torch.zeros(3, 64, dtype=E4M3), t, q, s, out=out) is out
+    assert any("copy_" in f for f in Holder.met)
+    residual_out = Holder(x.clone())
+    Holder.met.clear()
+    assert w8a8.add_rms_norm_fp8(x, x, w, residual_out=residual_out)[2] is residual_out
+    assert any("copy_" in f for f in Holder.met)
