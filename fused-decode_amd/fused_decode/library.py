@@ -150,13 +150,14 @@ def _pre_attn_qkv_fp8_fake(hidden, norm_weight, w_qkv, scale, cos, sin, eps, rop
     return hidden.new_empty((*_lead(hidden), w_qkv.shape[0]))
 
 
-# The implementations run their plans directly: the public w8a8 functions come here when a call is
-# recorded or transformed.
+# The implementations look up and run their plans directly: the public w8a8 functions come here when a
+# call is recorded or transformed.
 
 
 @torch.library.custom_op(f"{_NS}::quantize_rows_fp8", mutates_args=())
 def quantize_rows_fp8(x: Tensor) -> tuple[Tensor, Tensor]:
-    return w8a8._plan_rows_fp8("quantize_rows_fp8", x, None, None, 0.0, None, None, None)(x, None, None, None, None, None)
+    plan = w8a8._planned(w8a8._plan_rows_fp8, "quantize_rows_fp8", x, None, None, 0.0, None, None, None)
+    return plan(x, None, None, None, None, None)
 
 
 def _row_codes(x):
@@ -170,7 +171,8 @@ def _quantize_rows_fp8_fake(x):
 
 @torch.library.custom_op(f"{_NS}::rms_norm_fp8", mutates_args=())
 def rms_norm_fp8(x: Tensor, weight: Tensor, eps: float = 1e-6) -> tuple[Tensor, Tensor]:
-    return w8a8._plan_rows_fp8("rms_norm_fp8", x, weight, None, eps, None, None, None)(x, weight, None, None, None, None)
+    plan = w8a8._planned(w8a8._plan_rows_fp8, "rms_norm_fp8", x, weight, None, eps, None, None, None)
+    return plan(x, weight, None, None, None, None)
 
 
 @rms_norm_fp8.register_fake
@@ -181,8 +183,8 @@ def _rms_norm_fp8_fake(x, weight, eps=1e-6):
 @torch.library.custom_op(f"{_NS}::add_rms_norm_fp8", mutates_args=())
 def add_rms_norm_fp8(x: Tensor, residual: Tensor, weight: Tensor,
                      eps: float = 1e-6) -> tuple[Tensor, Tensor, Tensor]:
-    return w8a8._plan_rows_fp8("add_rms_norm_fp8", x, weight, residual, eps, None, None, None)(x, weight, residual, None,
-                                                                                                None, None)
+    plan = w8a8._planned(w8a8._plan_rows_fp8, "add_rms_norm_fp8", x, weight, residual, eps, None, None, None)
+    return plan(x, weight, residual, None, None, None)
 
 
 @add_rms_norm_fp8.register_fake
@@ -194,8 +196,8 @@ def _add_rms_norm_fp8_fake(x, residual, weight, eps=1e-6):
 def linear_w8a8(x: Tensor, x_scale: Tensor, weight: Tensor, scale: Tensor, bias: Tensor | None = None,
                 activation: str | None = None, row_add: Tensor | None = None,
                 dtype: torch.dtype = torch.bfloat16) -> Tensor:
-    return w8a8._plan_linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add, None, dtype)(
-        x, x_scale, weight, scale, bias, row_add, None)
+    plan = w8a8._planned(w8a8._plan_linear_w8a8, x, x_scale, weight, scale, bias, activation, row_add, None, dtype)
+    return plan(x, x_scale, weight, scale, bias, row_add, None)
 
 
 @linear_w8a8.register_fake

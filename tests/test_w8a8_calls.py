@@ -146,3 +146,18 @@ def test_a_subclass_as_output_is_written_by_torch(calls):  # noqa: F811
     Holder.met.clear()
     assert w8a8.add_rms_norm_fp8(x, x, w, residual_out=residual_out)[2] is residual_out
     assert any("copy_" in f for f in Holder.met)
+
+
+def test_custom_ops_keep_their_plans(calls, monkeypatch):  # noqa: F811
+    """One plan a signature, whatever values the tensors hold; another one for other strides, eps and activations."""
+    plans, check = [], w8a8.check
+    monkeypatch.setattr(w8a8, "check", lambda op, **a: plans.append(op) or check(op, **a))
+    f, (x, w, q, s) = torch.ops.fused_decode, arguments()
+    c, t = torch.zeros(3, 64, dtype=E4M3), torch.ones(3)
+    for _ in range(3):
+        f.quantize_rows_fp8(x.clone()), f.rms_norm_fp8(x, w.clone(), 1e-5), f.add_rms_norm_fp8(x, x.clone(), w, 1e-5)
+        f.linear_w8a8(c, t.clone(), q, s, None, "relu"), f.linear_w8a8(c, t, q, s, None, "silu")
+        f.linear_w8a8(c, t, q, s, s.clone(), None, torch.zeros(30), torch.float16)
+    assert len(calls) == 18 and len(plans) == 6
+    f.rms_norm_fp8(x, w, 1e-6), f.quantize_rows_fp8(x.t().contiguous().t()), f.quantize_rows_fp8(x)
+    assert len(calls) == 21 and len(plans) == 8
