@@ -77,8 +77,12 @@ def _out_sig(t: torch.Tensor) -> tuple:
 
 
 def _like(shape: tuple, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    """What ``torch.empty_like`` makes a contiguous ``shape`` of, in the least host time: one element, expanded."""
-    return torch.empty((), dtype=dtype, device=device).expand(shape)
+    """What ``torch.empty_like`` makes a contiguous ``shape`` of, in the least host time: one element, expanded, and its
+    memory given back (a plan made during a capture would keep the graph's pool with it)."""
+    one = torch.empty((), dtype=dtype, device=device)
+    like = one.expand(shape)
+    one.untyped_storage().resize_(0)
+    return like
 
 
 # ------------------------------------------------------------------ rows to codes

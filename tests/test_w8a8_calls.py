@@ -161,3 +161,14 @@ def test_custom_ops_keep_their_plans(calls, monkeypatch):  # noqa: F811
     assert len(calls) == 18 and len(plans) == 6
     f.rms_norm_fp8(x, w, 1e-6), f.quantize_rows_fp8(x.t().contiguous().t()), f.quantize_rows_fp8(x)
     assert len(calls) == 21 and len(plans) == 8
+
+
+@pytest.mark.parametrize("shape", [(), (0,), (1,), (3, 4), (5, 1, 7), (2, 0, 3)])
+def test_plans_hold_no_memory(shape):
+    """What a plan makes its results of has their shape, and none of the memory that it was made in."""
+    for dtype in (E4M3, torch.float32, torch.bfloat16):
+        like = w8a8._like(shape, dtype, torch.device("cpu"))
+        assert like.untyped_storage().nbytes() == 0
+        made = torch.empty_like(like)
+        assert made.shape == shape and made.dtype == dtype and made.is_contiguous()
+        assert made.zero_().float().sum() == 0
