@@ -216,7 +216,9 @@ def _plan_rows_fp8(op, x, weight, residual, eps, out, scale_out, residual_out):
         def empty(x, w, r, out, scale_out, residual_out):
             c = torch.empty(shape, dtype=FP8_DTYPE, device=device) if out is None else out
             s = torch.ones(lead, dtype=torch.float32, device=device) if scale_out is None else scale_out.fill_(1.0)
-            return (c, s, torch.empty_like(x) if residual_out is None else residual_out) if add else (c, s)
+            if not add:
+                return c, s
+            return c, s, torch.empty(shape, dtype=x.dtype, device=device) if residual_out is None else residual_out
         return empty
 
     codes_like, scale_like = _like(shape, FP8_DTYPE, device), _like(lead, torch.float32, device)

@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 from test_w8a8 import E4M3, arguments, calls, cuda  # noqa: F401 (a fixture)
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from fused_decode import _lib as L
 from fused_decode import ops, w8a8
@@ -172,3 +173,14 @@ def test_plans_hold_no_memory(shape):
         made = torch.empty_like(like)
         assert made.shape == shape and made.dtype == dtype and made.is_contiguous()
         assert made.zero_().float().sum() == 0
+
+
+def test_results_of_no_element_lie_as_the_fake_kernels_say(calls):  # noqa: F811
+    """Contiguous, whatever the strides of a batch of no rows: a compiled graph checks what it was told."""
+    x, w = torch.empty(2, 0, 3, 64, dtype=torch.bfloat16).transpose(1, 2), torch.ones(64)
+    got = w8a8.add_rms_norm_fp8(x, x, w)
+    with FakeTensorMode():
+        fx, fw = cuda(2, 0, 3, 64, dtype=torch.bfloat16).transpose(1, 2), cuda(64)
+        fake = torch.ops.fused_decode.add_rms_norm_fp8(fx, fx, fw)
+    assert [(t.shape, t.stride(), t.dtype) for t in got] == [(t.shape, t.stride(), t.dtype) for t in fake]
+    assert calls == []
