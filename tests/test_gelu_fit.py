@@ -1,9 +1,9 @@
 """The polynomial of the GELU epilogue (csrc/fd_w8a8.h), read from its source and evaluated on the CPU against math.erfc.
 
 The fit's own error is stated there as 9e-8. With u = 2^-24, float32's half step, Horner's eight steps of two roundings are
-off by at most 16 u sum |c_i| t^i, and that sum is at most 2.1 P(t) (checked below): 34 u of P. t carries three
-roundings, in t and, with t P' / P <= 1.25, in P, and three products and the exponential's own step follow:
-34 u + 7 u + 4 u + the fit's 2 u < 64 u = 2^-18. The exponential's argument carries the square's rounding, log2(e)'s and the
+off by at most 16 u sum |c_i| t^i, and that sum is at most 2.16 P(t) (checked below): 35 u of P. t carries three
+roundings, in t and, with t P' / P <= 1.26, in P, and three products and the exponential's own step follow:
+35 u + 7 u + 4 u + the fit's 2 u < 64 u = 2^-18. The exponential's argument carries the square's rounding, log2(e)'s and the
 product's, 3 u of v^2 / 2, below 2^-22 of it."""
 
 from __future__ import annotations
@@ -33,7 +33,7 @@ def test_the_fit():
         t = i / 1000
         terms = [v * t**k for k, v in enumerate(reversed(c))]
         slopes = [k * term for k, term in enumerate(terms)]
-        assert sum(map(abs, terms)) <= 2.1 * sum(terms) and abs(sum(slopes)) <= 1.25 * sum(terms)
+        assert sum(map(abs, terms)) <= 2.16 * sum(terms) and abs(sum(slopes)) <= 1.26 * sum(terms)
     worst = 0.0
     for i in range(1, 13001):
         z = i / 1000
