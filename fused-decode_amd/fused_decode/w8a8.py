@@ -6,9 +6,10 @@
     y = linear_w8a8(codes, scale, q, q_scale, bias, activation="gelu", row_add=r)
 
 A row has one float32 scale, ``max|y| / 448`` for the float32 row ``y`` (never below 2^-126, and 1 for
-a row of zeros), and its codes are ``y / scale`` rounded to the nearest E4M3 value; the norms
-quantise their float32 result, which is never rounded to 16 bits in between. A row whose largest
-magnitude is not finite gets a NaN scale and NaN codes. Weights are those of ``quantize_fp8``
+a row of zeros), and its codes are ``y / scale`` rounded to the nearest E4M3 value: in
+``quantize_rows_fp8`` as a division rounds, in the norms by the scale's reciprocal, which takes one
+code in about 10^6 to its neighbour. The norms quantise their float32 result, which is never rounded
+to 16 bits in between. A row whose largest magnitude is not finite gets a NaN scale and NaN codes. Weights are those of ``quantize_fp8``
 (codes ``[N, K]`` and one scale a row), so that
 
     y[m, n] = round(act(scale[m] * q_scale[n] * sum_k codes[m, k] q[n, k] + bias[n]) + row_add[m, n])
@@ -303,8 +304,8 @@ def linear_w8a8(
     ``activation`` is None, "relu", "silu", "gelu" (with erf), "gelu_tanh" or "swiglu", which takes gate rows
     above up rows (``weight [2I, K]``, ``bias [2I]``) and returns ``silu(gate) * up`` ``[..., I]``. ``bias`` and
     ``row_add`` have any float dtype; ``row_add`` broadcasts to the output and is added after the activation.
-    Any number of rows and any K; codes whose rows are not 16-byte aligned, whose K is no multiple of 16 or
-    whose stride along K is not 1 are copied first."""
+    Any number of rows and any K (below 2^23 for more than one row); codes whose rows are not 16-byte aligned, whose K
+    is no multiple of 16 or whose stride along K is not 1 are copied first."""
     try:
         recorded = (_watched()
                     or (_grad() and (x_scale.requires_grad or scale.requires_grad or x.requires_grad

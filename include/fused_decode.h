@@ -442,7 +442,8 @@ int fd_pre_attn_qkv_fp8_sumsq(void* y, const void* hidden, const void* norm_w, i
  * of the row grid; they overlap no input and each other in no byte. residual_out may be x
  * or residual in the same layout and overlaps them in no other way, and no two of its own
  * elements share memory (else FD_EINVAL).
- * fd_quantize_rows_fp8's codes are x / scale with the division's own rounding.
+ * fd_quantize_rows_fp8's codes are x / scale with the division's own rounding; the norms
+ * multiply by the scale's reciprocal, which takes one code in about 10^6 to its neighbour.
  * No reference counterpart (its activations are fp16/bf16 only).
  */
 int fd_quantize_rows_fp8(void* codes, float* scale, const void* x, const fd_rows* lx, int act_dtype,
@@ -456,7 +457,8 @@ int fd_add_rms_norm_fp8(void* codes, float* scale, void* residual_out, const voi
 
 /*
  * The product of E4M3 activations x8 [M,K] (row stride sxm bytes, one float32 scale a row)
- * and E4M3 weights w8 [N,K] (row stride swn, one float32 scale a row), any M, N and K:
+ * and E4M3 weights w8 [N,K] (row stride swn, one float32 scale a row), M, N and K below
+ * 2^31 - 512, for M > 1 K up to 2^23 - 16 and for M = 1 N up to 2^27 - 8 (else FD_EUNSUPPORTED):
  *   v[m,n] = x_scale[m] * w_scale[n] * sum_k x8[m,k] * w8[n,k] + bias[n]
  *   y[m,n] = round(act(v[m,n]) + row_add[m,n])
  * With FD_ACT_SWIGLU w8 holds gate rows above up rows (N = 2I) and y is [M,I]:
