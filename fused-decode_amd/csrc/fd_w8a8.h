@@ -172,6 +172,7 @@ int w8_one_launch(const W8Args& a);
 
 // Few rows (w8a8_few.hip): whether a product fits, and its launch.
 bool w8_few_fits(int64_t M, int64_t K);
+void w8_few_form(int64_t M, int64_t K, int* groups, int* steps);  // of 16 activation rows; of a wave, at most
 int w8_few_launch(const W8Args& a);
 
 }  // namespace fd

@@ -648,6 +648,31 @@ extern "C" int fd_linear_w8a8_scratch(int64_t M, int64_t N, int64_t K, int align
   return FD_OK;
 }
 
+extern "C" int fd_linear_w8a8_form(int64_t M, int64_t N, int64_t K, int* form) {
+  if (M < 0 || N < 0 || K < 0) return set_error(FD_EINVAL, "negative size");
+  if (!form) return set_error(FD_EINVAL, "null pointer argument");
+  for (int i = 0; i < 4; ++i) form[i] = 0;
+  if (M == 0 || N == 0 || M > kMostIndex || N > kMostIndex || K > kMostIndex) return FD_OK;
+  if (K < 16) {
+    form[0] = FD_W8A8_SHORT;
+  } else if (M == 1) {
+    form[0] = FD_W8A8_ONE;
+  } else {
+    const int64_t Kp = (K + 15) / 16 * 16;
+    if (w8_few_fits(M, Kp)) {
+      form[0] = FD_W8A8_FEW;
+      w8_few_form(M, Kp, &form[1], &form[2]);
+    } else {
+      const TilePlan p = tile_plan(M, N, Kp);
+      form[0] = FD_W8A8_TILES;
+      form[1] = kTiles[p.form].bn;
+      form[2] = kTiles[p.form].bm;
+      form[3] = p.splits;
+    }
+  }
+  return FD_OK;
+}
+
 extern "C" int fd_linear_w8a8(void* y, const void* x8, const float* x_scale, const void* w8, const float* w_scale,
                               const void* bias, int bias_dtype, int activation, const void* row_add, int row_dtype,
                               int64_t M, int64_t N, int64_t K, int64_t sxm, int64_t swn, int64_t sb, int64_t srm,

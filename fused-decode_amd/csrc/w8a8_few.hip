@@ -169,17 +169,24 @@ int few_steps(int64_t K) { return (int)(((K + kStep - 1) / kStep + kFewWaves - 1
 
 template <typename T, bool SWIGLU>
 int few_pick(const W8Args& a) {
-  const int s = few_steps(a.K);
-  if (a.M <= 16) {
-    if (s <= 4) return few_go<T, 1, 4, 7, SWIGLU>(a);
-    if (s <= 8) return few_go<T, 1, 8, 7, SWIGLU>(a);
+  int groups, steps;
+  w8_few_form(a.M, a.K, &groups, &steps);
+  if (groups == 1) {
+    if (steps == 4) return few_go<T, 1, 4, 7, SWIGLU>(a);
+    if (steps == 8) return few_go<T, 1, 8, 7, SWIGLU>(a);
     return few_go<T, 1, 16, 7, SWIGLU>(a);
   }
-  if (s <= 4) return few_go<T, 2, 4, 6, SWIGLU>(a);
+  if (steps == 4) return few_go<T, 2, 4, 6, SWIGLU>(a);
   return few_go<T, 2, 8, 6, SWIGLU>(a);
 }
 
 }  // namespace
+
+void w8_few_form(int64_t M, int64_t K, int* groups, int* steps) {
+  const int s = few_steps(K);
+  *groups = M <= 16 ? 1 : 2;
+  *steps = s <= 4 ? 4 : s <= 8 || *groups == 2 ? 8 : 16;
+}
 
 // Whether the activations fit the registers.
 bool w8_few_fits(int64_t M, int64_t K) { return M <= 16 ? few_steps(K) <= 16 : M <= 32 && few_steps(K) <= 8; }

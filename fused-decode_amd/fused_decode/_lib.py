@@ -100,6 +100,7 @@ SIGNATURES: dict[str, list] = {
     "fd_add_rms_norm_fp8": [_p, _p, _p, _p, _p, _p, _i, _l, _rows, _rows, _rows, _f, _i, _p],
     "fd_linear_w8a8": [_p, _p, _p, _p, _p, _p, _i, _i, _p, _i, _l, _l, _l, _l, _l, _l, _l, _l, _l, _l, _p, _l, _i, _p],
     "fd_linear_w8a8_scratch": [_l, _l, _l, _i, ctypes.POINTER(_l)],
+    "fd_linear_w8a8_form": [_l, _l, _l, ctypes.POINTER(_i)],
     "fd_copy": [_p, _p, _l, _p],
     "fd_copy_persistent": [_p, _p, _l, _i, _p],
     "fd_clock_probe": [_p, _i, ctypes.POINTER(ctypes.c_int), _p],

@@ -482,6 +482,16 @@ int fd_linear_w8a8(void* y, const void* x8, const float* x_scale, const void* w8
 int fd_linear_w8a8_scratch(int64_t M, int64_t N, int64_t K, int aligned, int64_t* bytes);
 
 /*
+ * The kernel that fd_linear_w8a8 takes for a product, given the scratch it asks for, in four
+ * ints (host only; N counts SwiGLU's gate and up rows): form[0] one of FD_W8A8_*, or 0 where
+ * nothing is launched. FD_W8A8_FEW: form[1] groups of 16 activation rows, form[2] the steps of
+ * K a wave keeps. FD_W8A8_TILES: form[1] weight rows and form[2] activation rows of a tile,
+ * form[3] the K splits.
+ */
+enum { FD_W8A8_SHORT = 1, FD_W8A8_ONE = 2, FD_W8A8_FEW = 3, FD_W8A8_TILES = 4 };
+int fd_linear_w8a8_form(int64_t M, int64_t N, int64_t K, int* form);
+
+/*
  * Bandwidth roofs. dst = src over `bytes` bytes (any size; 16-byte aligned
  * pointers take the vector path). c = a + b*scale over n elements of dtype.
  * Replace kernels.py:833-858 (`launch_copy`, `launch_triad`).
