@@ -1,5 +1,5 @@
 """Which kernel fd_linear_w8a8 takes, as its host-only query says (the library's figures are of 256 CUs without a GPU):
-the products of test_w8a8_forms_gpu reach every form of tiles, with and without K splits."""
+the products of test_w8a8_forms_gpu reach every form of tiles, with and without K splits, and every form for few rows."""
 
 from __future__ import annotations
 
@@ -7,7 +7,7 @@ import ctypes
 
 import pytest
 import torch
-from test_w8a8_forms_gpu import TILES, form
+from test_w8a8_forms_gpu import FEW, TILES, form
 
 from fused_decode import _lib as L
 
@@ -36,3 +36,5 @@ def test_every_form_is_among_the_products():
     tiles = {(form(*case[:3])[1:3], form(*case[:3])[3] > 1) for case in TILES}
     sizes = [(256, 256), (256, 128), (128, 128), (64, 128), (64, 64), (128, 32)]
     assert tiles == {(size, split) for size in sizes for split in (False, True)}
+    few = {form(*case)[1:3] for case in FEW}
+    assert few == {(1, 4), (1, 8), (1, 16), (2, 4), (2, 8)}

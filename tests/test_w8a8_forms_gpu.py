@@ -37,6 +37,13 @@ TILES = [
     (1003, 8202, 1040, (256, 256), 1), (779, 10006, 272, (256, 256), 1), (779, 5006, 14352, (256, 256), 3),
 ]
 
+# 2 to 32 rows: both sides of where the kept steps change, one tile a workgroup and several with a short last one, a K
+# that not every wave has a step of, and more outputs than the workgroups of one round hold
+FEW = [(m, 9002, k) for m in (2, 16) for k in (4096, 4112, 8192, 8208, 16384)]
+FEW += [(m, 9002, k) for m in (17, 32) for k in (4096, 4112, 8192)]
+FEW += [(13, 28672, 4096), (16, 16396, 512), (16, 4096, 14336), (31, 9002, 272), (3, 70002, 256), (24, 70002, 144), (5, 300, 16),
+        (32, 514, 8192)]
+
 
 class Case:
     """Operands, and the exact float64 values before an activation."""
@@ -104,6 +111,17 @@ def check_activations(c, n, dtype):
 @pytest.mark.parametrize("m,n,k,tile,splits", TILES)
 def test_tiles(m, n, k, tile, splits):
     assert form(m, n, k) == form(m, n - 1, k) == (4, *tile, splits)
+    dtype = torch.float16 if (m + k // 16) % 2 else torch.bfloat16
+    c = Case(m, n, k, m + n + k, dtype)
+    check_exact(c, n, dtype)
+    check_exact(c, n - 1, dtype)
+    check_activations(c, n - 1, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", FEW)
+def test_few_rows(m, n, k):
+    assert form(m, n, k)[0] == 3
     dtype = torch.float16 if (m + k // 16) % 2 else torch.bfloat16
     c = Case(m, n, k, m + n + k, dtype)
     check_exact(c, n, dtype)
