@@ -191,7 +191,7 @@ def _copied(got: tuple, *outs) -> tuple:
             raise TypeError(f"an output must be a tensor or None, got {type(o).__name__}")
         if o is not None and (o.shape != v.shape or o.dtype != v.dtype or o.device != v.device):
             raise ValueError(f"an output must have shape {tuple(v.shape)} and dtype {v.dtype} on {v.device}")
-        if o is not None and shares_memory(o.shape, o.stride()):
+        if o is not None and not _is_compiling() and shares_memory(o.shape, o.stride()):  # (compiled sizes are symbols)
             raise ValueError(f"an output has elements that share memory: shape {tuple(o.shape)} strides {o.stride()}")
     return tuple(v if o is None else o.copy_(v) for v, o in zip(got, outs))
 

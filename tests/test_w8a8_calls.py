@@ -184,3 +184,25 @@ def test_results_of_no_element_lie_as_the_fake_kernels_say(calls):  # noqa: F811
         fake = torch.ops.fused_decode.add_rms_norm_fp8(fx, fx, fw)
     assert [(t.shape, t.stride(), t.dtype) for t in got] == [(t.shape, t.stride(), t.dtype) for t in fake]
     assert calls == []
+
+
+@pytest.mark.parametrize("dynamic", [False, True])
+def test_a_compiled_call_with_outputs_stays_whole(dynamic):
+    """Sizes that are symbols, outputs given, the residual in place: one graph with the custom op and its copies. (It is run
+    only as far as the op, which refuses the CPU.)"""
+    graphs = []
+
+    def backend(module, inputs):
+        graphs.append([str(n.target) for n in module.graph.nodes if n.op == "call_function"])
+        return module.forward
+
+    x, w, q, s = arguments()
+    torch._dynamo.reset()
+    f = torch.compile(lambda x, r, w, c, t: w8a8.add_rms_norm_fp8(x, r, w, out=c, scale_out=t, residual_out=r),
+                      backend=backend, fullgraph=True, dynamic=dynamic)
+    wide = torch.zeros(3, 128, dtype=torch.float16)
+    for residual in (x.clone(), wide[:, :64]):
+        with pytest.raises(ValueError, match="CUDA"):
+            f(x, residual, w, torch.zeros(3, 64, dtype=E4M3), torch.ones(3))
+    assert graphs and all(sum(t.startswith("fused_decode.add_rms_norm_fp8") for t in g) == 1 for g in graphs)
+    torch._dynamo.reset()
