@@ -20,10 +20,11 @@
 // 16-byte nontemporal stores. SWIGLU: gate and up tiles of 16 rows in turn, so that a lane finds
 // both of an output.
 //
-// Large products are bound by the matrix cores, whose clock falls with their power (8192 x 28672 x
-// 4096 SWIGLU 755 us, 2550 TFLOP/s; MFMA alone on random codes reaches 3500), ordinary ones by the
-// rate at which the L2s feed a CU, 55 to 60 KB a microsecond (2048 x 4096 x 4096 35 us, 1950
-// TFLOP/s), which smaller tiles load more of. Nontemporal stores leave the L2s to the operands
+// Large products run at the clock that their power leaves, with the matrix cores busy 55% of the
+// cycles (8192 x 28672 x 4096 SWIGLU 755 us captured alone, 790 to 830 on a busy card, 2550 to 2320
+// TFLOP/s at 1.98 GHz; MFMA alone on random codes reaches 3500), ordinary ones at the rate at which the
+// L2s feed a CU, 46 KB a microsecond over the whole kernel, 55 to 60 between its start and end (2048 x
+// 4096 x 4096 35 us, 1950 TFLOP/s), which smaller tiles load more of. Nontemporal stores leave the L2s to the operands
 // (825 -> 745 us).
 //
 // Where the output has fewer tiles than the GPU has room for, K is split over workgroups whose
@@ -692,7 +693,8 @@ extern "C" int fd_linear_w8a8(void* y, const void* x8, const float* x_scale, con
   if (!y || !x_scale || !w_scale || (K > 0 && (!x8 || !w8))) return set_error(FD_EINVAL, "null pointer argument");
   if (M > kMostIndex || N > kMostIndex || K > kMostIndex) return set_error(FD_EUNSUPPORTED, "too large");
   const int64_t cols = swiglu ? N / 2 : N;
-  if (rows_meet(fd_rows{1, 1, M, 0, 0, sym, syn, cols})) return set_error(FD_EINVAL, "y's elements must not share memory");
+  if (rows_meet(fd_rows{1, 1, M, 0, 0, sym, syn, cols}))
+    return set_error(FD_EINVAL, "y's elements must not share memory");
   // tiles are stored while other workgroups still read their operands
   const int64_t ny = span_bytes(M, cols, sym, syn, 2);
   if (overlaps(y, ny, x8, span_bytes(M, K, sxm, 1, 1)) || overlaps(y, ny, w8, span_bytes(N, K, swn, 1, 1)) ||

@@ -16,9 +16,10 @@
 //
 // Bound by what a CU takes in a clock, weights and activations, and by a launch's start and end:
 // 13 x 28672 x 4096 SWIGLU 21.5 us (5.5 TB/s of weights), 16 x 4096 x 14336 17.3, 16 x 6144 x 4096
-// 8.8. Activations as the stream's first units, so that nothing waits for all of it, 15.0 against
-// 12.9 (2 x 4096 x 14336: they take the weights' slots); weights straight into registers, in the
-// operand's layout, 20.5 (loads of 64 bytes a row).
+// 8.8; 17 to 32 rows, two groups of 16: 24 x 6144 x 4096 9.6, 32 x 28672 x 4096 SWIGLU 24.1.
+// Activations as the stream's first units, so that nothing waits for all of it, 15.0 against 12.9
+// (2 x 4096 x 14336: they take the weights' slots); weights straight into registers, in the operand's
+// layout, 20.5 (loads of 64 bytes a row).
 //
 // Slot layout: 16 rows of 8 chunks of 16 bytes, chunk c at c ^ (row mod 8).
 #include "fd_w8a8.h"

@@ -9,8 +9,8 @@ A row has one float32 scale, ``max|y| / 448`` for the float32 row ``y`` (never b
 a row of zeros), and its codes are ``y / scale`` rounded to the nearest E4M3 value: in
 ``quantize_rows_fp8`` as a division rounds, in the norms by the scale's reciprocal, which takes one
 code in about 10^6 to its neighbour. The norms quantise their float32 result, which is never rounded
-to 16 bits in between. A row whose largest magnitude is not finite gets a NaN scale and NaN codes. Weights are those of ``quantize_fp8``
-(codes ``[N, K]`` and one scale a row), so that
+to 16 bits in between. A row whose largest magnitude is not finite gets a NaN scale and NaN codes.
+Weights are those of ``quantize_fp8`` (codes ``[N, K]`` and one scale a row), so that
 
     y[m, n] = round(act(scale[m] * q_scale[n] * sum_k codes[m, k] q[n, k] + bias[n]) + row_add[m, n])
 
@@ -64,7 +64,8 @@ def _watched() -> bool:
 
 def _subclasses(*tensors) -> bool:
     """Whether one of these is of a tensor subclass, whose memory may be another tensor's and which torch's calls let
-    act for itself: the custom op does. (Asked where a class is not in ``_PLAIN``; a list or a number is the contract's.)"""
+    act for themselves: the custom op does. (Asked where a class is not in ``_PLAIN``; a list or a number is left to
+    the contract.)"""
     return any(type(t) not in _PLAIN and isinstance(t, torch.Tensor) for t in tensors)
 
 
@@ -179,7 +180,8 @@ def add_rms_norm_fp8(
 
 
 def _planned(make, *args):
-    """``make(*args)``, a launch plan, kept by the arguments' signature: for the custom ops, whose calls nothing records."""
+    """``make(*args)``, a launch plan, kept by the arguments' signature: for the custom ops, whose calls are no longer
+    recorded."""
     key = (make.__name__, *(_sig(a) if isinstance(a, torch.Tensor) else a for a in args))
     return _PLANS.get(key) or _remember(key, make(*args))
 
