@@ -502,6 +502,41 @@ def output_dtype(name: str, out: str) -> Rule:
     return rule
 
 
+# ------------------------------------------------------ norms around a block (block_norms.py)
+
+
+def finite_scale(name: str) -> Rule:
+    def rule(a: dict) -> None:
+        try:
+            v = float(a[name])
+        except (TypeError, ValueError) as exc:
+            raise ValueError(f"{name} must be a finite value, got {a[name]!r}") from exc
+        if not abs(v) <= torch.finfo(torch.float32).max:
+            raise ValueError(f"{name} must be a finite float32 value, got {v}")
+        a[name] = v
+
+    return rule
+
+
+def gate_for(name: str, ref: str) -> Rule:
+    """Optional gate: any float dtype, on ``ref``'s device, broadcastable to its shape."""
+
+    def rule(a: dict) -> None:
+        t, r = a[name], a[ref]
+        if t is None:
+            return
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor or None, got {type(t).__name__}")
+        if t.device != r.device:
+            raise ValueError(f"{name} is on {t.device} but {ref} is on {r.device}")
+        if t.dtype not in FLOAT:
+            raise TypeError(f"{name} must be {_names(FLOAT)}, got {t.dtype}")
+        if not _broadcasts(t.shape, r.shape):
+            raise ValueError(f"cannot broadcast {name} shape {tuple(t.shape)} to {tuple(r.shape)}")
+
+    return rule
+
+
 # ------------------------------------------------------------------ contract
 
 CONTRACT: dict[str, tuple[Rule, ...]] = {
@@ -546,6 +581,14 @@ CONTRACT.update({
                     weight_matrix("weight", "x", fp8=True), inner_dim("x", "weight"), row_scales("scale", "weight"),
                     activation_name("activation", "weight"), bias_of("bias", "x", "weight"),
                     row_add_for("row_add", "x", "weight"), output_dtype("dtype", "out")),
+})
+
+
+CONTRACT.update({
+    "norm_add_norm": (tensor_on_gpu("x"), has_rows("x"), tensor_on_gpu("residual"), like("residual", "x"),
+                      vector_for("post_weight", "x"), vector_for("weight", "x"), finite_eps(), gate_for("gate", "x"),
+                      finite_scale("residual_scale"), output_like("out", "x"), no_shared_elements("out"),
+                      output_like("residual_out", "x"), no_shared_elements("residual_out")),
 })
 
 

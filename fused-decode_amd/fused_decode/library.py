@@ -14,9 +14,11 @@
     torch.ops.fused_decode.rms_norm_fp8(x, weight, eps) -> (codes, scale)
     torch.ops.fused_decode.add_rms_norm_fp8(x, residual, weight, eps) -> (codes, scale, residual_out)
     torch.ops.fused_decode.linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add, dtype)
+    torch.ops.fused_decode.norm_add_norm(x, residual, post_weight, weight, eps, gate, residual_scale)
+        -> (out, residual_out)
 
 Each is the functional form (no ``out=``) of the operator of the same name in
-``fused_decode.ops``, ``fp8`` or ``w8a8``, registered as a custom op with a fake (meta) kernel, so
+``fused_decode.ops``, ``fp8``, ``w8a8`` or ``block_norms``, registered as a custom op with a fake (meta) kernel, so
 ``torch.compile``, ``torch.export`` and AOT tracing keep the HIP launch as one
 opaque node: the Python argument checks run once per call at run time, and
 graph breaks do not happen around the operators. The reference names this as a
@@ -32,7 +34,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from . import fp8, ops, w8a8
+from . import block_norms, fp8, ops, w8a8
 
 _NS = "fused_decode"
 
@@ -150,8 +152,8 @@ def _pre_attn_qkv_fp8_fake(hidden, norm_weight, w_qkv, scale, cos, sin, eps, rop
     return hidden.new_empty((*_lead(hidden), w_qkv.shape[0]))
 
 
-# The implementations look up and run their plans directly: the public w8a8 functions come here when a
-# call is recorded or transformed.
+# The implementations look up and run their plans directly: the public functions of w8a8 and of the modules after it come
+# here when a call is recorded or transformed.
 
 
 @torch.library.custom_op(f"{_NS}::quantize_rows_fp8", mutates_args=())
@@ -206,6 +208,20 @@ def _linear_w8a8_fake(x, x_scale, weight, scale, bias=None, activation=None, row
     return x.new_empty((*_lead(x), n), dtype=dtype)
 
 
+@torch.library.custom_op(f"{_NS}::norm_add_norm", mutates_args=())
+def norm_add_norm(x: Tensor, residual: Tensor, post_weight: Tensor, weight: Tensor, eps: float = 1e-6,
+                  gate: Tensor | None = None, residual_scale: float = 1.0) -> tuple[Tensor, Tensor]:
+    plan = w8a8._planned(block_norms._plan_norm_add_norm, x, residual, post_weight, weight, eps, gate, residual_scale,
+                         None, None)
+    return plan(x, residual, post_weight, weight, gate, None, None)
+
+
+@norm_add_norm.register_fake
+def _norm_add_norm_fake(x, residual, post_weight, weight, eps=1e-6, gate=None, residual_scale=1.0):
+    return x.new_empty(x.shape), x.new_empty(x.shape)
+
+
 OPS = ("rms_norm", "add_rms_norm", "rope", "swiglu", "linear_decode", "post_attn_mlp", "pre_attn_qkv",
        "linear_decode_fp8", "post_attn_mlp_fp8", "pre_attn_qkv_fp8")
 OPS_W8A8 = ("quantize_rows_fp8", "rms_norm_fp8", "add_rms_norm_fp8", "linear_w8a8")
+OPS_FP4 = ("norm_add_norm",)

@@ -492,6 +492,24 @@ enum { FD_W8A8_SHORT = 1, FD_W8A8_ONE = 2, FD_W8A8_FEW = 3, FD_W8A8_TILES = 4 };
 int fd_linear_w8a8_form(int64_t M, int64_t N, int64_t K, int* form);
 
 /*
+ * The norms around a block, with its gated and scaled residual between them:
+ *   z = x * post_w * rsqrt(mean(x^2) + eps)             (per row, after the block)
+ *   t = residual + residual_scale * gate * z            (float32); residual_out = round(t)
+ *   y = round(t * w * rsqrt(mean(t^2) + eps))           (before the next block)
+ * gate (NULL for 1) has any of the three dtypes and a layout of its own on the row grid, with
+ * strides of 0 where it is broadcast: one a channel, one a row, one an element. post_w and w have
+ * n elements each, any of the three dtypes and a stride. y and residual_out may each be x or
+ * residual in the same layout (element for element), and overlap nothing else and each other in
+ * no byte; no two of their own elements share memory (FD_EINVAL). No reference counterpart.
+ */
+int fd_norm_add_norm(void* y, void* residual_out, const void* x, const void* residual,
+                     const void* gate, int gate_dtype, const void* post_w, int post_w_dtype,
+                     int64_t post_w_stride, const void* w, int w_dtype, int64_t w_stride,
+                     const fd_rows* lx, const fd_rows* lr, const fd_rows* lg, const fd_rows* ly,
+                     const fd_rows* lro, float residual_scale, float eps, int act_dtype,
+                     void* stream);
+
+/*
  * Bandwidth roofs. dst = src over `bytes` bytes (any size; 16-byte aligned
  * pointers take the vector path). c = a + b*scale over n elements of dtype.
  * Replace kernels.py:833-858 (`launch_copy`, `launch_triad`).
