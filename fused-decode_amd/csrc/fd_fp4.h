@@ -1,0 +1,94 @@
+// Products of 16-bit activations and weights held as OCP E2M1 codes, two a byte (the first in the low half), with an E8M0
+// scale (2^(byte - 127), 255: NaN) for each group of 32 along K:
+//
+//   v[m,n] = sum_k x[m,k] * 2^(s[n, k / 32] - 127) * e2m1(w[n,k]) + bias[n]
+//   y[m,n] = round(act(v[m,n]) + row_add[m,n])
+//   FD_ACT_SWIGLU, w [2I,K]: y[m,j] = round(silu(v[m,j]) * v[m,I+j] + row_add[m,j])
+//
+// gfx950 turns two codes and a scale into two bfloat16 numbers in one instruction, and the result is exact: two bits of
+// significand and bfloat16's exponents (products past them are infinite, as they are in bfloat16). So a weight needs no
+// arithmetic of its own: the scale is in the matrix instruction's operand. float16 activations meet them as two bfloat16
+// numbers whose sum they are exactly (11 bits of significand are 8 and 3), float32 sums of both.
+//
+// A row of codes is read in pieces of 16 bytes: 32 codes, one group, one scale. v_mfma_f32_16x16x32_bf16 takes 32 k a
+// step, 8 of row L % 16 from each lane group g = L / 16; any k order that both operands share gives the same sum. Here a
+// lane has a whole piece of its row and takes it in four steps, step j its codes 8 j .. 8 j + 7, so that the four groups'
+// pieces (128 k) are four steps, and a lane's scale is one for all of them. Weights are the A operand: a lane's four sums
+// are weight rows 4 g + i of activation row L % 16.
+#pragma once
+
+#include "fd_w8a8.h"
+
+namespace fd {
+
+constexpr int kGroupK = 32;  // k of a scale, codes of a 16-byte piece
+
+// Two codes of byte B of `codes` with the scale whose exponent `scale` has.
+template <int B>
+__device__ __forceinline__ uint32_t fp4_pair(uint32_t codes, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, B));
+}
+// Eight codes.
+__device__ __forceinline__ bf16x8 fp4_to_bf16(uint32_t codes, float scale) {
+  return __builtin_bit_cast(bf16x8, u32x4{fp4_pair<0>(codes, scale), fp4_pair<1>(codes, scale),
+                                          fp4_pair<2>(codes, scale), fp4_pair<3>(codes, scale)});
+}
+// The conversion's scale of an E8M0 byte: it reads the exponent alone, 0 as 2^-127 and 255 as NaN.
+__device__ __forceinline__ float e8m0_operand(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
+
+// float16 as two bfloat16 numbers: the second one's three bits are exact, and it is 0 beside an infinity or a NaN.
+__device__ __forceinline__ void split_f16(float v, bf16& hi, bf16& lo) {
+  hi = (bf16)v;
+  const float rest = v - (float)hi;
+  lo = (bf16)(fabsf(v) <= 65504.f ? rest : 0.f);
+}
+
+// One 16-byte-per-lane DMA from a pointer a lane into LDS at byte address `lds` (wave-uniform; lane L lands at 16 L).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma16_at(const void* src, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+struct Fp4Epi {
+  const void* bias;
+  int bias_dtype;
+  int64_t sb;
+  int act;  // FD_ACT_*, not FD_ACT_SWIGLU, which is a kernel's form
+  const void* row;
+  int row_dtype;
+  int64_t srm, srn;
+};
+
+// One output from its sum (SWIGLU: and the up row's, weight row n + half).
+template <bool SWIGLU>
+__device__ __forceinline__ float fp4_out(const Fp4Epi& e, float acc, float up, int64_t m, int64_t n, int64_t half) {
+  float v = acc + (e.bias ? load_any(e.bias, e.bias_dtype, n * e.sb) : 0.f);
+  if constexpr (SWIGLU) {
+    v = times_sigmoid(v, v) * (up + (e.bias ? load_any(e.bias, e.bias_dtype, (n + half) * e.sb) : 0.f));
+  } else {
+    float one[1] = {v};
+    activate(one, e.act);
+    v = one[0];
+  }
+  if (e.row) v += load_any(e.row, e.row_dtype, m * e.srm + n * e.srn);
+  return v;
+}
+
+// A checked product: rows of codes are 16-byte aligned runs of ceil(K / 32) pieces, x has unit stride along K.
+struct Fp4Args {
+  void* y;
+  const void* x;
+  const uint8_t *w, *ws;
+  int M, N, K;  // N: rows of w
+  int64_t sxm, swn, ssn, sym, syn;
+  bool swiglu;
+  Fp4Epi e;
+  float* scratch;
+  int64_t scratch_bytes;
+  int act_dtype;
+  hipStream_t st;
+};
+
+}  // namespace fd

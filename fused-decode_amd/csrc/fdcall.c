@@ -130,6 +130,9 @@ static int (*p_linear_w8a8)(void*, const void*, const float*, const void*, const
                             const void*, int, int, const void*, int, int64_t, int64_t, int64_t,
                             int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, float*,
                             int64_t, int, void*);
+static int (*p_linear_fp4)(void*, const void*, const void*, const void*, const void*, int, int,
+                           const void*, int, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
+                           int64_t, int64_t, int64_t, int64_t, int64_t, float*, int64_t, int, void*);
 static int (*p_norm_add_norm)(void*, void*, const void*, const void*, const void*, int,
                               const void*, int, int64_t, const void*, int, int64_t, const fd_rows*,
                               const fd_rows*, const fd_rows*, const fd_rows*, const fd_rows*, float,
@@ -217,6 +220,10 @@ WRAP(linear_w8a8, "ppppppiipillllllllllplis",
                    a[6].i, a[7].i, a[8].p, a[9].i, a[10].l, a[11].l, a[12].l, a[13].l, a[14].l,
                    a[15].l, a[16].l, a[17].l, a[18].l, a[19].l, (float*)a[20].p, a[21].l, a[22].i,
                    a[23].p))
+WRAP(linear_fp4, "pppppiipilllllllllllplis",
+     p_linear_fp4(a[0].p, a[1].p, a[2].p, a[3].p, a[4].p, a[5].i, a[6].i, a[7].p, a[8].i, a[9].l,
+                  a[10].l, a[11].l, a[12].l, a[13].l, a[14].l, a[15].l, a[16].l, a[17].l, a[18].l,
+                  a[19].l, (float*)a[20].p, a[21].l, a[22].i, a[23].p))
 WRAP(norm_add_norm, "pppppipilpilrrrrrffis",
      p_norm_add_norm(a[0].p, a[1].p, a[2].p, a[3].p, a[4].p, a[5].i, a[6].p, a[7].i, a[8].l, a[9].p,
                      a[10].i, a[11].l, (const fd_rows*)a[12].p, (const fd_rows*)a[13].p,
@@ -280,6 +287,7 @@ static PyObject* w_bind(PyObject* self, PyObject* arg) {
   RESOLVE(p_rms_norm_fp8, "fd_rms_norm_fp8");
   RESOLVE(p_add_rms_norm_fp8, "fd_add_rms_norm_fp8");
   RESOLVE(p_linear_w8a8, "fd_linear_w8a8");
+  RESOLVE(p_linear_fp4, "fd_linear_fp4");
   RESOLVE(p_norm_add_norm, "fd_norm_add_norm");
   RESOLVE(p_copy, "fd_copy");
   RESOLVE(p_triad, "fd_triad");
@@ -312,6 +320,7 @@ static PyMethodDef methods[] = {
     FAST(rms_norm_fp8),
     FAST(add_rms_norm_fp8),
     FAST(linear_w8a8),
+    FAST(linear_fp4),
     FAST(norm_add_norm),
     FAST(copy),
     FAST(triad),

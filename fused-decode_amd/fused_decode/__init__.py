@@ -19,6 +19,7 @@ from .ops import (
 
 from .fp8 import dequantize_fp8, linear_decode_fp8, post_attn_mlp_fp8, pre_attn_qkv_fp8, quantize_fp8
 from .w8a8 import add_rms_norm_fp8, linear_w8a8, quantize_rows_fp8, rms_norm_fp8
+from .fp4 import dequantize_fp4, linear_fp4, quantize_fp4
 from .block_norms import norm_add_norm
 from . import library  # registers torch.ops.fused_decode.* (custom ops with fake kernels)
 
@@ -28,13 +29,16 @@ __all__ = [
     "DECODE_LINEAR_MAX_M",
     "add_rms_norm",
     "add_rms_norm_fp8",
+    "dequantize_fp4",
     "dequantize_fp8",
     "linear_decode_fp8",
     "post_attn_mlp_fp8",
     "pre_attn_qkv_fp8",
+    "quantize_fp4",
     "quantize_fp8",
     "quantize_rows_fp8",
     "linear_decode",
+    "linear_fp4",
     "linear_w8a8",
     "norm_add_norm",
     "post_attn_mlp",

@@ -502,6 +502,35 @@ def output_dtype(name: str, out: str) -> Rule:
     return rule
 
 
+# ------------------------------------------------------------------ 4-bit weights (fp4.py)
+
+FP4_GROUP = 32  # values that share a scale
+E8M0 = torch.float8_e8m0fnu
+
+
+def fp4_matrix(name: str, scale: str, ref: str) -> Rule:
+    """E2M1 codes ``[N, 16 G]``, two a byte, and their E8M0 scales ``[N, G]``, on ``ref``'s device, for ``ref [..., K]`` with
+    ``G = ceil(K / 32)``."""
+
+    def rule(a: dict) -> None:
+        w, s, r = a[name], a[scale], a[ref]
+        for what, t, dtype in ((name, w, torch.uint8), (scale, s, E8M0)):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{what} must be a tensor, got {type(t).__name__}")
+            if t.dtype != dtype:
+                raise TypeError(f"{what} must be {dtype} (see quantize_fp4), got {t.dtype}")
+            if t.device != r.device:
+                raise ValueError(f"{what} is on {t.device} but {ref} is on {r.device}")
+            if t.ndim != 2:
+                raise ValueError(f"{what} must be a rank-2 tensor, got {tuple(t.shape)}")
+        groups = -(-r.shape[-1] // FP4_GROUP)
+        if w.shape[1] != groups * FP4_GROUP // 2 or s.shape != (w.shape[0], groups):
+            raise ValueError(f"{name} and {scale} must have shapes [N, {groups * FP4_GROUP // 2}] and [N, {groups}] for "
+                             f"{ref}'s last dimension {r.shape[-1]}, got {tuple(w.shape)} and {tuple(s.shape)}")
+
+    return rule
+
+
 # ------------------------------------------------------ norms around a block (block_norms.py)
 
 
@@ -585,6 +614,9 @@ CONTRACT.update({
 
 
 CONTRACT.update({
+    "linear_fp4": (tensor_on_gpu("x"), has_rows("x"), fp4_matrix("weight", "scale", "x"),
+                   activation_name("activation", "weight"), bias_of("bias", "x", "weight"),
+                   row_add_for("row_add", "x", "weight")),
     "norm_add_norm": (tensor_on_gpu("x"), has_rows("x"), tensor_on_gpu("residual"), like("residual", "x"),
                       vector_for("post_weight", "x"), vector_for("weight", "x"), finite_eps(), gate_for("gate", "x"),
                       finite_scale("residual_scale"), output_like("out", "x"), no_shared_elements("out"),

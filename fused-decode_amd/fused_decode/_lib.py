@@ -101,6 +101,8 @@ SIGNATURES: dict[str, list] = {
     "fd_linear_w8a8": [_p, _p, _p, _p, _p, _p, _i, _i, _p, _i, _l, _l, _l, _l, _l, _l, _l, _l, _l, _l, _p, _l, _i, _p],
     "fd_linear_w8a8_scratch": [_l, _l, _l, _i, ctypes.POINTER(_l)],
     "fd_linear_w8a8_form": [_l, _l, _l, ctypes.POINTER(_i)],
+    "fd_linear_fp4": [_p, _p, _p, _p, _p, _i, _i, _p, _i, _l, _l, _l, _l, _l, _l, _l, _l, _l, _l, _l, _p, _l, _i, _p],
+    "fd_linear_fp4_scratch": [_l, _l, _l, _i, ctypes.POINTER(_l)],
     "fd_norm_add_norm": [_p, _p, _p, _p, _p, _i, _p, _i, _l, _p, _i, _l, _rows, _rows, _rows, _rows, _rows, _f, _f, _i,
                          _p],
     "fd_copy": [_p, _p, _l, _p],

@@ -14,11 +14,12 @@
     torch.ops.fused_decode.rms_norm_fp8(x, weight, eps) -> (codes, scale)
     torch.ops.fused_decode.add_rms_norm_fp8(x, residual, weight, eps) -> (codes, scale, residual_out)
     torch.ops.fused_decode.linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add, dtype)
+    torch.ops.fused_decode.linear_fp4(x, weight, scale, bias, activation, row_add)
     torch.ops.fused_decode.norm_add_norm(x, residual, post_weight, weight, eps, gate, residual_scale)
         -> (out, residual_out)
 
 Each is the functional form (no ``out=``) of the operator of the same name in
-``fused_decode.ops``, ``fp8``, ``w8a8`` or ``block_norms``, registered as a custom op with a fake (meta) kernel, so
+``fused_decode.ops``, ``fp8``, ``w8a8``, ``fp4`` or ``block_norms``, registered as a custom op with a fake (meta) kernel, so
 ``torch.compile``, ``torch.export`` and AOT tracing keep the HIP launch as one
 opaque node: the Python argument checks run once per call at run time, and
 graph breaks do not happen around the operators. The reference names this as a
@@ -34,7 +35,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from . import block_norms, fp8, ops, w8a8
+from . import block_norms, fp4, fp8, ops, w8a8
 
 _NS = "fused_decode"
 
@@ -208,6 +209,19 @@ def _linear_w8a8_fake(x, x_scale, weight, scale, bias=None, activation=None, row
     return x.new_empty((*_lead(x), n), dtype=dtype)
 
 
+@torch.library.custom_op(f"{_NS}::linear_fp4", mutates_args=())
+def linear_fp4(x: Tensor, weight: Tensor, scale: Tensor, bias: Tensor | None = None, activation: str | None = None,
+               row_add: Tensor | None = None) -> Tensor:
+    plan = w8a8._planned(fp4._plan_linear_fp4, x, weight, scale, bias, activation, row_add, None)
+    return plan(x, weight, scale, bias, row_add, None)
+
+
+@linear_fp4.register_fake
+def _linear_fp4_fake(x, weight, scale, bias=None, activation=None, row_add=None):
+    n = weight.shape[0] // 2 if activation == "swiglu" else weight.shape[0]
+    return x.new_empty((*_lead(x), n))
+
+
 @torch.library.custom_op(f"{_NS}::norm_add_norm", mutates_args=())
 def norm_add_norm(x: Tensor, residual: Tensor, post_weight: Tensor, weight: Tensor, eps: float = 1e-6,
                   gate: Tensor | None = None, residual_scale: float = 1.0) -> tuple[Tensor, Tensor]:
@@ -224,4 +238,4 @@ def _norm_add_norm_fake(x, residual, post_weight, weight, eps=1e-6, gate=None, r
 OPS = ("rms_norm", "add_rms_norm", "rope", "swiglu", "linear_decode", "post_attn_mlp", "pre_attn_qkv",
        "linear_decode_fp8", "post_attn_mlp_fp8", "pre_attn_qkv_fp8")
 OPS_W8A8 = ("quantize_rows_fp8", "rms_norm_fp8", "add_rms_norm_fp8", "linear_w8a8")
-OPS_FP4 = ("norm_add_norm",)
+OPS_FP4 = ("linear_fp4", "norm_add_norm")

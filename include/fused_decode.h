@@ -492,6 +492,33 @@ enum { FD_W8A8_SHORT = 1, FD_W8A8_ONE = 2, FD_W8A8_FEW = 3, FD_W8A8_TILES = 4 };
 int fd_linear_w8a8_form(int64_t M, int64_t N, int64_t K, int* form);
 
 /*
+ * The product of 16-bit activations x [M,K] (row stride sxm, unit stride along K) and weights held
+ * in 4 bits: w4 [N,ceil(K/32)*16] bytes (row stride swn), two OCP E2M1 codes a byte, the first in
+ * the low half, and w_scale [N,ceil(K/32)] E8M0 bytes (row stride ssn), one for each 32 along K,
+ * 2^(byte - 127), 255 NaN. Codes past K are not used. With
+ *   v[m,n] = sum_k x[m,k] * 2^(s[n,k/32] - 127) * e2m1(w4[n,k]) + bias[n]
+ *   y[m,n] = round(act(v[m,n]) + row_add[m,n])
+ * and FD_ACT_SWIGLU, gate rows above up rows (N = 2I), y [M,I]:
+ *   y[m,j] = round(silu(v[m,j]) * v[m,I+j] + row_add[m,j])
+ * Weights are exact in the product; sums and the epilogue are float32 with one rounding. bias (N
+ * values at stride sb) and row_add (strides srm, srn; 0 broadcasts) have any of the three dtypes
+ * and may be NULL. M, N and K are below 2^31 - 512; rows of codes are 16-byte aligned (else
+ * FD_EUNSUPPORTED). `scratch` (16-byte aligned, caller-owned, not shared with a call that may
+ * overlap) holds what fd_linear_fp4_scratch says (0: none): copies of activations that are
+ * float16, off 16-byte alignment or of no whole 128 along K (without it FD_EUNSUPPORTED), and,
+ * where there are few output tiles, the float32 sums of K splits, which are added in a fixed
+ * order; less lowers the split, down to none. y may be row_add element for element and overlaps
+ * no operand otherwise (FD_EUNSUPPORTED); no two of its own elements share memory (FD_EINVAL).
+ * No reference counterpart.
+ */
+int fd_linear_fp4(void* y, const void* x, const void* w4, const void* w_scale, const void* bias,
+                  int bias_dtype, int activation, const void* row_add, int row_dtype, int64_t M,
+                  int64_t N, int64_t K, int64_t sxm, int64_t swn, int64_t ssn, int64_t sb,
+                  int64_t srm, int64_t srn, int64_t sym, int64_t syn, float* scratch,
+                  int64_t scratch_bytes, int act_dtype, void* stream);
+int fd_linear_fp4_scratch(int64_t M, int64_t N, int64_t K, int act_dtype, int64_t* bytes);
+
+/*
  * The norms around a block, with its gated and scaled residual between them:
  *   z = x * post_w * rsqrt(mean(x^2) + eps)             (per row, after the block)
  *   t = residual + residual_scale * gate * z            (float32); residual_out = round(t)
