@@ -30,7 +30,8 @@ typedef union {
 
 /* Argument codes: p pointer (int or None), s stream (same), i int, l int64,
  * f float, r const fd_rows* (bytes of sizeof(fd_rows)), t const fd_tile*
- * (bytes of sizeof(fd_tile), or None). */
+ * (bytes of sizeof(fd_tile), or None). A const fd_kv_shape* is a p: the address of a struct that the
+ * caller keeps. */
 static int parse(const char* fn, PyObject* const* args, Py_ssize_t nargs, const char* fmt,
                  Arg* out) {
   const Py_ssize_t want = (Py_ssize_t)strlen(fmt);
@@ -133,6 +134,16 @@ static int (*p_linear_w8a8)(void*, const void*, const float*, const void*, const
 static int (*p_linear_fp4)(void*, const void*, const void*, const void*, const void*, int, int,
                            const void*, int, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
                            int64_t, int64_t, int64_t, int64_t, int64_t, float*, int64_t, int, void*);
+static int (*p_append_kv_fp4)(void*, void*, void*, void*, const fd_kv_shape*, const void*, const void*,
+                              int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, const int32_t*,
+                              const int32_t*, int64_t, int64_t, int64_t, int64_t, int, void*);
+static int (*p_read_kv_fp4)(void*, void*, const void*, const void*, const void*, const void*,
+                            const fd_kv_shape*, const int32_t*, const int32_t*, int64_t, int64_t,
+                            int64_t, int64_t, int, void*);
+static int (*p_attend_kv_fp4)(void*, const void*, const void*, const void*, const void*, const void*,
+                              const fd_kv_shape*, int64_t, int64_t, int64_t, const int32_t*,
+                              const int32_t*, int64_t, int64_t, int64_t, int64_t, int64_t, float,
+                              float*, int64_t, int, void*);
 static int (*p_norm_add_norm)(void*, void*, const void*, const void*, const void*, int,
                               const void*, int, int64_t, const void*, int, int64_t, const fd_rows*,
                               const fd_rows*, const fd_rows*, const fd_rows*, const fd_rows*, float,
@@ -224,6 +235,19 @@ WRAP(linear_fp4, "pppppiipilllllllllllplis",
      p_linear_fp4(a[0].p, a[1].p, a[2].p, a[3].p, a[4].p, a[5].i, a[6].i, a[7].p, a[8].i, a[9].l,
                   a[10].l, a[11].l, a[12].l, a[13].l, a[14].l, a[15].l, a[16].l, a[17].l, a[18].l,
                   a[19].l, (float*)a[20].p, a[21].l, a[22].i, a[23].p))
+WRAP(append_kv_fp4, "pppppppllllllppllllis",
+     p_append_kv_fp4(a[0].p, a[1].p, a[2].p, a[3].p, (const fd_kv_shape*)a[4].p, a[5].p, a[6].p,
+                     a[7].l, a[8].l, a[9].l, a[10].l, a[11].l, a[12].l, (const int32_t*)a[13].p,
+                     (const int32_t*)a[14].p, a[15].l, a[16].l, a[17].l, a[18].l, a[19].i, a[20].p))
+WRAP(read_kv_fp4, "pppppppppllllis",
+     p_read_kv_fp4(a[0].p, a[1].p, a[2].p, a[3].p, a[4].p, a[5].p, (const fd_kv_shape*)a[6].p,
+                   (const int32_t*)a[7].p, (const int32_t*)a[8].p, a[9].l, a[10].l, a[11].l,
+                   a[12].l, a[13].i, a[14].p))
+WRAP(attend_kv_fp4, "ppppppplllpplllllfplis",
+     p_attend_kv_fp4(a[0].p, a[1].p, a[2].p, a[3].p, a[4].p, a[5].p, (const fd_kv_shape*)a[6].p,
+                     a[7].l, a[8].l, a[9].l, (const int32_t*)a[10].p, (const int32_t*)a[11].p,
+                     a[12].l, a[13].l, a[14].l, a[15].l, a[16].l, a[17].f, (float*)a[18].p, a[19].l,
+                     a[20].i, a[21].p))
 WRAP(norm_add_norm, "pppppipilpilrrrrrffis",
      p_norm_add_norm(a[0].p, a[1].p, a[2].p, a[3].p, a[4].p, a[5].i, a[6].p, a[7].i, a[8].l, a[9].p,
                      a[10].i, a[11].l, (const fd_rows*)a[12].p, (const fd_rows*)a[13].p,
@@ -288,6 +312,9 @@ static PyObject* w_bind(PyObject* self, PyObject* arg) {
   RESOLVE(p_add_rms_norm_fp8, "fd_add_rms_norm_fp8");
   RESOLVE(p_linear_w8a8, "fd_linear_w8a8");
   RESOLVE(p_linear_fp4, "fd_linear_fp4");
+  RESOLVE(p_append_kv_fp4, "fd_append_kv_fp4");
+  RESOLVE(p_read_kv_fp4, "fd_read_kv_fp4");
+  RESOLVE(p_attend_kv_fp4, "fd_attend_kv_fp4");
   RESOLVE(p_norm_add_norm, "fd_norm_add_norm");
   RESOLVE(p_copy, "fd_copy");
   RESOLVE(p_triad, "fd_triad");
@@ -321,6 +348,9 @@ static PyMethodDef methods[] = {
     FAST(add_rms_norm_fp8),
     FAST(linear_w8a8),
     FAST(linear_fp4),
+    FAST(append_kv_fp4),
+    FAST(read_kv_fp4),
+    FAST(attend_kv_fp4),
     FAST(norm_add_norm),
     FAST(copy),
     FAST(triad),

@@ -531,6 +531,141 @@ def fp4_matrix(name: str, scale: str, ref: str) -> Rule:
     return rule
 
 
+# ------------------------------------------------------------------ 4-bit key/value cache (kv_fp4.py)
+
+KV_DIMS = (64, 96, 128, 192, 256)
+
+
+def kv_cache(*names: str) -> Rule:
+    """Codes and scales of keys and values: ``[pages, heads, page, dim / 2]`` and ``[pages, heads, page, dim / 32]`` on one
+    GPU, slots together, strides alike (those of the scales a sixteenth)."""
+
+    def rule(a: dict) -> None:
+        tensors = [a[n] for n in names]
+        for i, (n, t) in enumerate(zip(names, tensors)):
+            dtype = E8M0 if i % 2 else torch.uint8
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{n} must be a tensor, got {type(t).__name__}")
+            if not t.is_cuda:
+                raise ValueError(f"{n} must be a CUDA tensor (a HIP device), got device {t.device}")
+            if t.dtype != dtype:
+                raise TypeError(f"{n} must be {dtype}, got {t.dtype}")
+            if t.ndim != 4:
+                raise ValueError(f"{n} must have four dimensions, got shape {tuple(t.shape)}")
+        k = tensors[0]
+        pages, heads, page, half = k.shape
+        if 2 * half not in KV_DIMS:
+            raise ValueError(f"a head must have {', '.join(map(str, KV_DIMS))} channels, got {2 * half}")
+        if heads == 0 or page == 0:
+            raise ValueError(f"a cache has heads and slots, got shape {tuple(k.shape)}")
+        for i, (n, t) in enumerate(zip(names, tensors)):
+            part = 16 if i % 2 else 1  # a scale for 32 codes, two a byte
+            if t.device != k.device:
+                raise ValueError(f"{n} is on {t.device} but {names[0]} is on {k.device}")
+            if t.shape != (pages, heads, page, half // part):
+                raise ValueError(f"{n} must have shape {(pages, heads, page, half // part)}, got {tuple(t.shape)}")
+            row = half // part
+            want = [s // part for s in k.stride()[:2]] + [row, 1]
+            bad = any(size > 1 and st != w for size, st, w in zip(t.shape, t.stride(), want))
+            if bad or (i == 0 and any(size > 1 and st % 16 for size, st in zip(t.shape[:2], t.stride()[:2]))):
+                raise ValueError(f"a cache's slots must lie together and its tensors' strides be alike, multiples of 16 "
+                                 f"and a sixteenth for scales: {n} has strides {t.stride()}, {names[0]} {k.stride()}")
+
+    return rule
+
+
+def kv_rows(name: str, cache: str, *, multiple: bool = False) -> Rule:
+    """``[B, L, heads, dim]`` for a cache's heads (``multiple``: a multiple of them) and head width."""
+
+    def rule(a: dict) -> None:
+        t, c = a[name], a[cache]
+        if t.device != c.device:
+            raise ValueError(f"{name} is on {t.device} but the cache is on {c.device}")
+        heads, dim = c.shape[1], 2 * c.shape[3]
+        if t.ndim != 4 or t.shape[3] != dim or (t.shape[2] % heads if multiple else t.shape[2] != heads):
+            what = f"a multiple of {heads}" if multiple else heads
+            raise ValueError(f"{name} must have shape [B, L, {what}, {dim}], got {tuple(t.shape)}")
+
+    return rule
+
+
+def kv_tokens(lengths: str, pages: str, cache: str, batch: str | None = None) -> Rule:
+    """int32 lengths ``[B]`` and, optionally, int32 pages ``[B, n]`` on the cache's device; without pages the cache has one
+    for each sequence."""
+
+    def rule(a: dict) -> None:
+        n, p, c = a[lengths], a[pages], a[cache]
+        for name, t in ((lengths, n), (pages, p)):
+            if t is None and name == pages:
+                continue
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+            if t.dtype != torch.int32:
+                raise TypeError(f"{name} must be int32, got {t.dtype}")
+            if t.device != c.device:
+                raise ValueError(f"{name} is on {t.device} but the cache is on {c.device}")
+        if n.ndim != 1 or (batch is not None and n.shape[0] != a[batch].shape[0]):
+            raise ValueError(f"{lengths} must hold one length a sequence, got shape {tuple(n.shape)}")
+        if p is not None and (p.ndim != 2 or p.shape[0] != n.shape[0]):
+            raise ValueError(f"{pages} must have shape [{n.shape[0]}, n], got {tuple(p.shape)}")
+        if p is None and n.shape[0] > c.shape[0]:
+            raise ValueError(f"without {pages} each of the {n.shape[0]} sequences has a page: the cache has {c.shape[0]}")
+
+    return rule
+
+
+def kv_count(name: str) -> Rule:
+    def rule(a: dict) -> None:
+        v = a[name]
+        if isinstance(v, bool) or not hasattr(v, "__index__") or isinstance(v, torch.Tensor):
+            raise TypeError(f"{name} must be an integer, got {type(v).__name__}")
+        a[name] = v.__index__()
+        if a[name] < 0:
+            raise ValueError(f"{name} must not be negative, got {v}")
+
+    return rule
+
+
+def one_of(name: str, values) -> Rule:
+    def rule(a: dict) -> None:
+        if a[name] not in values:
+            raise TypeError(f"{name} must be {_names(values)}, got {a[name]}")
+
+    return rule
+
+
+def softmax_scale(name: str, ref: str) -> Rule:
+    """The scale of the scores, 1 / sqrt(dim) by default."""
+    finite = finite_scale(name)
+
+    def rule(a: dict) -> None:
+        if a[name] is None:
+            a[name] = a[ref].shape[-1] ** -0.5
+        finite(a)
+        if abs(a[name]) > 1e38:
+            raise ValueError(f"{name} must be 1e38 at most, got {a[name]}")
+
+    return rule
+
+
+def dense_output(name: str, ref: str) -> Rule:
+    """Optional contiguous output of ``ref``'s shape, dtype and device."""
+
+    def rule(a: dict) -> None:
+        t, r = a[name], a[ref]
+        if t is None:
+            return
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor or None, got {type(t).__name__}")
+        if t.dtype != r.dtype:
+            raise TypeError(f"{name} must be {r.dtype}, got {t.dtype}")
+        if t.shape != r.shape or t.device != r.device or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {tuple(r.shape)} tensor on {r.device}, got shape "
+                             f"{tuple(t.shape)} strides {t.stride()} on {t.device}")
+
+    return rule
+
+
 # ------------------------------------------------------ norms around a block (block_norms.py)
 
 
@@ -617,6 +752,12 @@ CONTRACT.update({
     "linear_fp4": (tensor_on_gpu("x"), has_rows("x"), fp4_matrix("weight", "scale", "x"),
                    activation_name("activation", "weight"), bias_of("bias", "x", "weight"),
                    row_add_for("row_add", "x", "weight")),
+    "append_kv_fp4": (kv_cache("k", "k_scale", "v", "v_scale"), tensor_on_gpu("new_k"), kv_rows("new_k", "k"),
+                      tensor_on_gpu("new_v"), like("new_v", "new_k"), kv_tokens("lengths", "pages", "k", "new_k")),
+    "read_kv_fp4": (kv_cache("k", "k_scale", "v", "v_scale"), kv_tokens("lengths", "pages", "k"), kv_count("count"),
+                    one_of("dtype", ACTIVATION)),
+    "attend_kv_fp4": (kv_cache("k", "k_scale", "v", "v_scale"), tensor_on_gpu("q"), kv_rows("q", "k", multiple=True),
+                      kv_tokens("lengths", "pages", "k", "q"), softmax_scale("scale", "q"), dense_output("out", "q")),
     "norm_add_norm": (tensor_on_gpu("x"), has_rows("x"), tensor_on_gpu("residual"), like("residual", "x"),
                       vector_for("post_weight", "x"), vector_for("weight", "x"), finite_eps(), gate_for("gate", "x"),
                       finite_scale("residual_scale"), output_like("out", "x"), no_shared_elements("out"),

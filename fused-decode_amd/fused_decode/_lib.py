@@ -53,11 +53,19 @@ class FdRows(ctypes.Structure):
     ]
 
 
+class FdKvShape(ctypes.Structure):
+    """``fd_kv_shape``: a 4-bit cache's pages, heads, slots of a page and head width, and the strides of its codes in
+    bytes."""
+
+    _fields_ = [(name, ctypes.c_int64) for name in ("pages", "heads", "page", "dim", "page_stride", "head_stride")]
+
+
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _l = ctypes.c_int64
 _f = ctypes.c_float
 _rows = ctypes.POINTER(FdRows)
+_kv = ctypes.POINTER(FdKvShape)
 
 # name -> argument types; every entry point returns an int status.
 SIGNATURES: dict[str, list] = {
@@ -103,6 +111,10 @@ SIGNATURES: dict[str, list] = {
     "fd_linear_w8a8_form": [_l, _l, _l, ctypes.POINTER(_i)],
     "fd_linear_fp4": [_p, _p, _p, _p, _p, _i, _i, _p, _i, _l, _l, _l, _l, _l, _l, _l, _l, _l, _l, _l, _p, _l, _i, _p],
     "fd_linear_fp4_scratch": [_l, _l, _l, _i, ctypes.POINTER(_l)],
+    "fd_append_kv_fp4": [_p, _p, _p, _p, _kv, _p, _p, _l, _l, _l, _l, _l, _l, _p, _p, _l, _l, _l, _l, _i, _p],
+    "fd_read_kv_fp4": [_p, _p, _p, _p, _p, _p, _kv, _p, _p, _l, _l, _l, _l, _i, _p],
+    "fd_attend_kv_fp4": [_p, _p, _p, _p, _p, _p, _kv, _l, _l, _l, _p, _p, _l, _l, _l, _l, _l, _f, _p, _l, _i, _p],
+    "fd_attend_kv_fp4_scratch": [_l, _l, _l, _l, _l, _l, ctypes.POINTER(_l)],
     "fd_norm_add_norm": [_p, _p, _p, _p, _p, _i, _p, _i, _l, _p, _i, _l, _rows, _rows, _rows, _rows, _rows, _f, _f, _i,
                          _p],
     "fd_copy": [_p, _p, _l, _p],
@@ -193,11 +205,10 @@ def fail(func: str, status: int) -> None:
     raise FusedDecodeError(func, status, native().last_error())
 
 
-def scratch_bytes(func: str, m: int, n: int, k: int, *more: int) -> int:
-    """Bytes of scratch that an [M, N, K] product prefers (``func``: a *_scratch entry point, ``more`` its further
-    arguments)."""
+def scratch_bytes(func: str, *sizes: int) -> int:
+    """Bytes of scratch that a call of these sizes prefers (``func``: a *_scratch entry point, ``sizes`` its arguments)."""
     out = ctypes.c_int64(0)
-    check(func, getattr(lib(), func)(m, n, k, *more, ctypes.byref(out)))
+    check(func, getattr(lib(), func)(*sizes, ctypes.byref(out)))
     return out.value
 
 

@@ -15,11 +15,15 @@
     torch.ops.fused_decode.add_rms_norm_fp8(x, residual, weight, eps) -> (codes, scale, residual_out)
     torch.ops.fused_decode.linear_w8a8(x, x_scale, weight, scale, bias, activation, row_add, dtype)
     torch.ops.fused_decode.linear_fp4(x, weight, scale, bias, activation, row_add)
+    torch.ops.fused_decode.append_kv_fp4(k!, k_scale!, v!, v_scale!, new_k, new_v, lengths, pages)
+    torch.ops.fused_decode.read_kv_fp4(k, k_scale, v, v_scale, lengths, count, pages, dtype) -> (k, v)
+    torch.ops.fused_decode.attend_kv_fp4(q, k, k_scale, v, v_scale, lengths, pages, scale)
     torch.ops.fused_decode.norm_add_norm(x, residual, post_weight, weight, eps, gate, residual_scale)
         -> (out, residual_out)
 
 Each is the functional form (no ``out=``) of the operator of the same name in
-``fused_decode.ops``, ``fp8``, ``w8a8``, ``fp4`` or ``block_norms``, registered as a custom op with a fake (meta) kernel, so
+``fused_decode.ops``, ``fp8``, ``w8a8``, ``fp4``, ``kv_fp4`` or ``block_norms``,
+registered as a custom op with a fake (meta) kernel, so
 ``torch.compile``, ``torch.export`` and AOT tracing keep the HIP launch as one
 opaque node: the Python argument checks run once per call at run time, and
 graph breaks do not happen around the operators. The reference names this as a
@@ -35,7 +39,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from . import block_norms, fp4, fp8, ops, w8a8
+from . import block_norms, fp4, fp8, kv_fp4, ops, w8a8
 
 _NS = "fused_decode"
 
@@ -222,6 +226,43 @@ def _linear_fp4_fake(x, weight, scale, bias=None, activation=None, row_add=None)
     return x.new_empty((*_lead(x), n))
 
 
+@torch.library.custom_op(f"{_NS}::append_kv_fp4", mutates_args=("k", "k_scale", "v", "v_scale"))
+def append_kv_fp4(k: Tensor, k_scale: Tensor, v: Tensor, v_scale: Tensor, new_k: Tensor, new_v: Tensor,
+                  lengths: Tensor, pages: Tensor | None = None) -> None:
+    w8a8._planned(kv_fp4._plan_append, k, k_scale, v, v_scale, new_k, new_v, lengths, pages)(
+        k, k_scale, v, v_scale, new_k, new_v, lengths, pages)
+
+
+@append_kv_fp4.register_fake
+def _append_kv_fp4_fake(k, k_scale, v, v_scale, new_k, new_v, lengths, pages=None):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::read_kv_fp4", mutates_args=())
+def read_kv_fp4(k: Tensor, k_scale: Tensor, v: Tensor, v_scale: Tensor, lengths: Tensor, count: int,
+                pages: Tensor | None = None, dtype: torch.dtype = torch.bfloat16) -> tuple[Tensor, Tensor]:
+    plan = w8a8._planned(kv_fp4._plan_read, k, k_scale, v, v_scale, lengths, count, pages, dtype)
+    return plan(k, k_scale, v, v_scale, lengths, pages)
+
+
+@read_kv_fp4.register_fake
+def _read_kv_fp4_fake(k, k_scale, v, v_scale, lengths, count, pages=None, dtype=torch.bfloat16):
+    shape = (lengths.shape[0], count, k.shape[1], 2 * k.shape[3])
+    return k.new_empty(shape, dtype=dtype), k.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op(f"{_NS}::attend_kv_fp4", mutates_args=())
+def attend_kv_fp4(q: Tensor, k: Tensor, k_scale: Tensor, v: Tensor, v_scale: Tensor, lengths: Tensor,
+                  pages: Tensor | None = None, scale: float | None = None) -> Tensor:
+    plan = w8a8._planned(kv_fp4._plan_attend, q, k, k_scale, v, v_scale, lengths, pages, scale, None)
+    return plan(q, k, k_scale, v, v_scale, lengths, pages, None)
+
+
+@attend_kv_fp4.register_fake
+def _attend_kv_fp4_fake(q, k, k_scale, v, v_scale, lengths, pages=None, scale=None):
+    return q.new_empty(q.shape)
+
+
 @torch.library.custom_op(f"{_NS}::norm_add_norm", mutates_args=())
 def norm_add_norm(x: Tensor, residual: Tensor, post_weight: Tensor, weight: Tensor, eps: float = 1e-6,
                   gate: Tensor | None = None, residual_scale: float = 1.0) -> tuple[Tensor, Tensor]:
@@ -238,4 +279,4 @@ def _norm_add_norm_fake(x, residual, post_weight, weight, eps=1e-6, gate=None, r
 OPS = ("rms_norm", "add_rms_norm", "rope", "swiglu", "linear_decode", "post_attn_mlp", "pre_attn_qkv",
        "linear_decode_fp8", "post_attn_mlp_fp8", "pre_attn_qkv_fp8")
 OPS_W8A8 = ("quantize_rows_fp8", "rms_norm_fp8", "add_rms_norm_fp8", "linear_w8a8")
-OPS_FP4 = ("linear_fp4", "norm_add_norm")
+OPS_FP4 = ("linear_fp4", "append_kv_fp4", "read_kv_fp4", "attend_kv_fp4", "norm_add_norm")

@@ -519,6 +519,67 @@ int fd_linear_fp4(void* y, const void* x, const void* w4, const void* w_scale, c
 int fd_linear_fp4_scratch(int64_t M, int64_t N, int64_t K, int act_dtype, int64_t* bytes);
 
 /*
+ * A key/value cache held in 4 bits: pages of `page` slots, keys and values each as E2M1 codes
+ * [pages, heads, page, dim / 2] (two a byte, the first in the low half) with E8M0 scales
+ * [pages, heads, page, dim / 32], one for each 32 along the head. page_stride and head_stride are
+ * bytes of codes (multiples of 16) and the same for keys and values; scales have a sixteenth of
+ * them. Slots lie together. dim is 64, 96, 128, 192 or 256. A sequence's pages are a row of `table`
+ * (int32, rows of table_pages at table_stride); with table NULL page b is sequence b's. Codes and
+ * outputs are 16-byte aligned. A page number outside the cache is not followed: its tokens are
+ * neither stored nor seen. lengths (int32, on the device) are a sequence's tokens, the new ones
+ * among them; tokens past what its pages hold are neither stored nor seen.
+ * No reference counterparts (it has no cache and no attention).
+ */
+typedef struct fd_kv_shape {
+  int64_t pages, heads, page, dim;
+  int64_t page_stride, head_stride;
+} fd_kv_shape;
+
+/*
+ * Store new_k and new_v [B, L, heads, dim] (strides skb, skl, skh and svb, svl, svh, unit stride
+ * along dim) as tokens lengths[b] - L .. lengths[b] - 1 of sequence b; those below 0 are skipped. A
+ * group's scale is the smallest power of two that its largest magnitude is less than 7 of (2^-126
+ * at least, 1 for zeros), codes are the nearest to v / scale, ties to the even code, 6 at most; a
+ * group with an infinity or a NaN has a NaN scale. Two tokens stored to one slot leave one of the
+ * two there, or some of each.
+ */
+int fd_append_kv_fp4(void* k, void* k_scale, void* v, void* v_scale, const fd_kv_shape* shape,
+                     const void* new_k, const void* new_v, int64_t skb, int64_t skl, int64_t skh,
+                     int64_t svb, int64_t svl, int64_t svh, const int32_t* lengths,
+                     const int32_t* table, int64_t table_stride, int64_t table_pages, int64_t B,
+                     int64_t L, int act_dtype, void* stream);
+
+/*
+ * Tokens 0 .. count - 1 of each sequence as values: out_k and out_v [B, count, heads, dim], dense,
+ * of act_dtype (float16 rounds what it does not hold); zeros for tokens that a sequence lacks.
+ */
+int fd_read_kv_fp4(void* out_k, void* out_v, const void* k, const void* k_scale, const void* v,
+                   const void* v_scale, const fd_kv_shape* shape, const int32_t* lengths,
+                   const int32_t* table, int64_t table_stride, int64_t table_pages, int64_t B,
+                   int64_t count, int act_dtype, void* stream);
+
+/*
+ * Attention of q [B, L, Hq, dim] (strides sqb, sql, sqh, unit stride along dim), whose L queries are
+ * each sequence's last L tokens, over the cache; Hq is a multiple of its heads, query head n reads
+ * head n / (Hq / heads):
+ *   y = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale * q . k_t),  t <= lengths[b] - L + l
+ * y [B, L, Hq, dim], dense; a query that sees no token gets zeros. Softmax and sums are float32;
+ * q, keys and values are exact in the products, p is held as two bfloat16 numbers. `scratch`
+ * (16-byte aligned, caller-owned, not shared with a call that may overlap) holds what
+ * fd_attend_kv_fp4_scratch says (`capacity`: tokens that a sequence's pages hold; 0: none): the sums
+ * of a sequence's shares, which a second launch joins; less lowers their number, down to one. y
+ * overlaps nothing that it is computed from (FD_EUNSUPPORTED).
+ */
+int fd_attend_kv_fp4(void* y, const void* q, const void* k, const void* k_scale, const void* v,
+                     const void* v_scale, const fd_kv_shape* shape, int64_t sqb, int64_t sql,
+                     int64_t sqh, const int32_t* lengths, const int32_t* table,
+                     int64_t table_stride, int64_t table_pages, int64_t B, int64_t L, int64_t Hq,
+                     float scale, float* scratch, int64_t scratch_bytes, int act_dtype,
+                     void* stream);
+int fd_attend_kv_fp4_scratch(int64_t B, int64_t L, int64_t Hq, int64_t heads, int64_t dim,
+                             int64_t capacity, int64_t* bytes);
+
+/*
  * The norms around a block, with its gated and scaled residual between them:
  *   z = x * post_w * rsqrt(mean(x^2) + eps)             (per row, after the block)
  *   t = residual + residual_scale * gate * z            (float32); residual_out = round(t)
