@@ -131,6 +131,9 @@ __global__ __launch_bounds__(256) void kv_read_kernel(T* ko, T* vo, KvCache c, K
 constexpr int kKvTile = 32;     // tokens of a step
 constexpr int kKvChunk = 4096;  // tokens whose places a workgroup's LDS holds
 
+// The larger one, NaN beside a NaN.
+__device__ __forceinline__ float kv_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 template <int MASK>
 __device__ __forceinline__ float xlane_fmax(float v) {
   static_assert(MASK >= 16, "between lane groups");
@@ -138,7 +141,7 @@ __device__ __forceinline__ float xlane_fmax(float v) {
   const auto r = MASK == 32 ? __builtin_amdgcn_permlane32_swap(a, a, false, false)
                             : __builtin_amdgcn_permlane16_swap(a, a, false, false);
   const unsigned r0 = r[0], r1 = r[1];
-  return fmaxf(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+  return kv_max(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
 }
 
 // N 32-bit words (2, 3, 4, 6 or 8).
@@ -196,36 +199,79 @@ __device__ __forceinline__ uint32_t kv_pair(const uint32_t* w, float scale) {
 struct KvQuery {
   int64_t sb, sl, sh;  // strides of q
   uint32_t L, Hq, G, rows;  // rows: L * G
-  float scale;              // times log2 e
+  float scale;              // its magnitude times log2 e
+  bool flip;                // whether it is negative: q's sign takes it
 };
+
+// Tokens of a step in one run of slots, or each at a place of its own (pages that end inside a step).
+enum KvMode { KV_RUN = 0, KV_PLACES = 1 };
 
 // One step's keys and values of a lane, as they lie in memory.
 //
 // Keys are the A operand of q . k: lane (r, g) has quarter g of tokens r and 16 + r. Values, the other way round, are the A
 // operand of the sum over tokens: lane (r, g) has the sixteenth r of tokens 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3,
 // the tokens whose scores it gets.
-template <int D>
+template <int D, int MODE>
 struct KvStep {
   static constexpr int KW = D / 32;                                                     // words of a quarter
   static constexpr int KS = D == 64 || D == 128 ? 1 : D == 256 ? 2 : D / 32;            // scales of it
-  static constexpr int VB = D / 32, VW = (VB + 3) / 4, VS = D == 96 || D == 192 ? 2 : 1;  // bytes of a sixteenth
+  static constexpr int VB = D / 32, VW = (VB + 3) / 4;                                  // bytes of a sixteenth
+  static constexpr int VS = D == 96 || D == 192 ? 2 : 1;                                // scales of it
+  // a run's four tokens' scales come together where they are whole words (2 or 4 bytes a token)
+  static constexpr bool PACKED = MODE == KV_RUN && (D == 64 || D == 128);
   KvWords<KW> k[2];
   uint32_t ks[2][KS];
   uint32_t v[8][VW];
-  uint32_t vs[8][VS];
-  uint32_t at[8];  // places of the value's tokens
+  uint32_t vs[PACKED ? 2 : 8][PACKED ? D / 32 : VS];
+  uint32_t at[MODE == KV_PLACES ? 8 : 1];  // places of the value's tokens
+  uint32_t some;                           // a word of the run's values' scales: the lanes have all of them
 
-  __device__ __forceinline__ void load(const uint8_t* kp, const uint8_t* ksp, const uint8_t* vp, const uint8_t* vsp,
-                                       const uint32_t* places, int r, int g) {
+  static __device__ __forceinline__ int key_first(int j, int g) {
+    return KS == 1 ? g * (D / 4) / 32 : KS == 2 ? 2 * g + j : (g * (D / 4) + 8 * j) / 32;
+  }
+  __device__ __forceinline__ void key(int s, const uint8_t* codes, const uint8_t* scales, int g) {
+    k[s].load(codes);
+#pragma unroll
+    for (int j = 0; j < KS; ++j) ks[s][j] = scales[key_first(j, g)];
+  }
+  __device__ __forceinline__ void value(int n, const uint8_t* codes) { kv_bytes<VB>(codes, v[n]); }
+  __device__ __forceinline__ void value_scale(int n, const uint8_t* scales, int r) {
+    if constexpr (!PACKED) {
+      vs[n][0] = scales[r * (D / 16) / 32];
+      if constexpr (VS == 2) vs[n][1] = scales[(r * (D / 16) + D / 16 - 1) / 32];
+    }
+  }
+  // from place `at` on, a run
+  __device__ __forceinline__ void load_run(const KvCache& c, uint64_t at, int r, int g) {
+    const uint8_t *kp = c.k + at * 16, *ksp = c.ks + at, *vp = c.v + at * 16, *vsp = c.vs + at;
+    const unsigned ko = r * (D / 2) + g * (D / 8), so = r * (D / 32), vo = 4 * g * (D / 2) + r * VB,
+                   wo = 4 * g * (D / 32);
+    typedef uint32_t u1 __attribute__((aligned(1)));
+    some = *reinterpret_cast<const u1*>(vsp + (r + 16 * g) % (D / 4) * 4);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) key(s, kp + (ko + s * 8 * D), ksp + (so + s * (D / 2)), g);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const uint32_t a = places[s * 16 + r], b = a == kNoPlace ? 0u : a;
-      k[s].load(kp + (uint64_t)b * 16 + g * (D / 8));
+      if constexpr (PACKED) {
+        typedef uint32_t uw __attribute__((ext_vector_type(D / 32), aligned(1)));
+        const uw w = *reinterpret_cast<const uw*>(vsp + (wo + s * (D / 2)));
 #pragma unroll
-      for (int j = 0; j < KS; ++j) {
-        const int first = KS == 1 ? g * (D / 4) / 32 : KS == 2 ? 2 * g + j : (g * (D / 4) + 8 * j) / 32;
-        ks[s][j] = ksp[(uint64_t)b + first];
+        for (int i = 0; i < D / 32; ++i) vs[s][i] = w[i];
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        value(s * 4 + i, vp + (vo + s * 8 * D + i * (D / 2)));
+        value_scale(s * 4 + i, vsp + (wo + s * (D / 2) + i * (D / 32)), r);
+      }
+    }
+  }
+  // 32 places, kNoPlace where there is no token
+  __device__ __forceinline__ void load_places(const KvCache& c, uint64_t head, const uint32_t* places, int r, int g) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const uint32_t a = places[s * 16 + r];
+      const uint64_t b = head + (a == kNoPlace ? 0u : a);
+      key(s, c.k + b * 16 + g * (D / 8), c.ks + b, g);
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -233,11 +279,10 @@ struct KvStep {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int n = s * 4 + i;
-        at[n] = a[i];
-        const uint32_t b = a[i] == kNoPlace ? 0u : a[i];
-        kv_bytes<VB>(vp + (uint64_t)b * 16 + r * VB, v[n]);
-        vs[n][0] = vsp[(uint64_t)b + r * (D / 16) / 32];
-        if constexpr (VS == 2) vs[n][1] = vsp[(uint64_t)b + (r * (D / 16) + D / 16 - 1) / 32];
+        if constexpr (MODE == KV_PLACES) at[n] = a[i];
+        const uint64_t b = head + (a[i] == kNoPlace ? 0u : a[i]);
+        value(n, c.v + b * 16 + r * VB);
+        value_scale(n, c.vs + b, r);
       }
     }
   }
@@ -245,11 +290,52 @@ struct KvStep {
   __device__ __forceinline__ float key_scale(int s, int j) const {
     return e8m0_operand(ks[s][KS == 1 ? 0 : KS == 2 ? j / 4 : j]);
   }
-  // of byte B of a token's values
+  // Of byte B of a token's values, as the conversion takes it: it reads the exponent alone, so a word that is turned
+  // until the byte stands there will do. `turn`: by how much, for this lane's byte of an even word.
   template <int B>
-  __device__ __forceinline__ uint32_t value_byte(int n, int r) const {
-    if constexpr (VS == 1) return vs[n][0];
-    return (r * (D / 16) + 2 * B) / 32 == r * (D / 16) / 32 ? vs[n][0] : vs[n][VS - 1];
+  __device__ __forceinline__ float value_scale_of(int n, int r, uint32_t turn) const {
+    if constexpr (PACKED) {
+      const uint32_t w = vs[n / 4][D == 128 ? n % 4 : n % 4 / 2];
+      return __builtin_bit_cast(float, __builtin_amdgcn_alignbit(w, w, D == 64 && n % 2 ? turn + 16 : turn));
+    } else {
+      const uint32_t e = VS == 1 || (r * (D / 16) + 2 * B) / 32 == r * (D / 16) / 32 ? vs[n][0] : vs[n][VS - 1];
+      return e8m0_operand(e);
+    }
+  }
+  // Scales of 1 for tokens that nobody sees (from `seen` on, or without a place): what lies there may be no number.
+  __device__ __forceinline__ void drop_unseen(int t0, int seen, int g) {
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      bool none = t0 + (n / 4) * 16 + g * 4 + n % 4 >= seen;
+      if constexpr (MODE == KV_PLACES) none = at[n] == kNoPlace;
+      if constexpr (PACKED) {
+        uint32_t& w = vs[n / 4][D == 128 ? n % 4 : n % 4 / 2];
+        const uint32_t keep = D == 128 ? 0u : n % 2 ? 0x0000ffffu : 0xffff0000u;
+        w = none ? (w & keep) | (0x7f7f7f7fu & ~keep) : w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < VS; ++j) vs[n][j] = none ? 127u : vs[n][j];
+      }
+    }
+  }
+  // Whether a scale of 2^65 or more is among the step's (from 2^126 on codes leave bfloat16's range), of which the lanes
+  // have all; MASK: behind drop_unseen.
+  template <bool MASK>
+  __device__ __forceinline__ bool any_big() const {
+    if constexpr (MODE == KV_RUN && !MASK) return (some & some << 1 & 0x80808080u) != 0;
+    uint32_t big = 0;
+    if constexpr (PACKED) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) big |= vs[s][i] & vs[s][i] << 1 & 0x80808080u;
+    } else {
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int j = 0; j < VS; ++j) big |= vs[n][j] & vs[n][j] << 1 & 0x80u;
+    }
+    return big != 0;
   }
 };
 
@@ -270,13 +356,19 @@ __device__ __forceinline__ void kv_each_byte(F&& f) {
 // neighbouring channels into pairs of neighbouring tokens, one permute each. q is bfloat16, float16 as two bfloat16
 // parts; P is two bfloat16 parts (a single one would cost as much again as the output's own rounding).
 //
+// Bound by the instructions between the loads and the matrix cores (two codes a conversion, two a permute), so addresses
+// are a wave's: a step whose tokens lie in one run of slots (KV_RUN: pages of whole steps, or a sequence in one page,
+// whose last step starts early enough to end with it) needs one place. Masks are for the steps that need them.
+//
 // An infinity or NaN among the values of one token must not reach query rows that do not see it (0 times it is NaN): a
-// step that holds a scale from which codes leave bfloat16's range is summed token by token.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_attend_kernel(T* y, float* part, const T* q, KvCache c, KvTable tb, KvQuery qa,
-                                                        FastDiv page, FastDiv group, uint32_t row16, uint32_t tiles16) {
+// step that holds a scale from which codes leave bfloat16's range is left out, and summed token by token behind the
+// others.
+template <typename T, int D, int MODE>
+__global__ __launch_bounds__(256, D <= 128 && MODE == KV_RUN ? 3 : 2) void kv_attend_kernel(T* y, float* part, const T* q, KvCache c, KvTable tb,
+                                                           KvQuery qa, FastDiv page, FastDiv group, uint32_t tiles16) {
   constexpr int H = std::is_same<T, f16>::value ? 2 : 1, VD = D / 16, PITCH = D + 4;
-  constexpr int kWords = kKvChunk > 4 * 16 * PITCH ? kKvChunk : 4 * 16 * PITCH;
+  constexpr uint32_t row16 = D / 32;
+  constexpr int kJoin = 4 * 16 * PITCH, kWords = MODE == KV_PLACES && kKvChunk > kJoin ? kKvChunk : kJoin;
   __shared__ __align__(16) uint32_t smem[kWords];
   __shared__ float stat[4][16][2];
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
@@ -285,22 +377,24 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(T* y, float* part, const
   const uint32_t split = blockIdx.x, splits = gridDim.x, b = blockIdx.z;
   const uint32_t h = blockIdx.y / tiles16, tile16 = blockIdx.y - h * tiles16;
 
-  const int64_t length = tb.lengths[b];
+  const int64_t length = __builtin_amdgcn_readfirstlane(tb.lengths[b]);
   const uint32_t seen = (uint32_t)(length < 0 ? 0 : length > tb.capacity ? tb.capacity : length);
   // this lane's query row, and the last token that it sees
   const uint32_t i0 = tile16 * 16 + r;
-  const bool mine = i0 < qa.rows;
   uint32_t gi;
-  const uint32_t l = group.divmod(mine ? i0 : qa.rows - 1, gi);
+  const uint32_t l = group.divmod(i0 < qa.rows ? i0 : qa.rows - 1, gi);
   const int64_t last64 = length - qa.L + l;
   const int last = (int)(last64 < 0 ? -1 : last64 > 0x7ffffffe ? 0x7ffffffe : last64);
+  const int whole = (int)(length - qa.L < -1 ? -1 : length - qa.L);  // tokens up to here every query sees
 
   bf16x8 qf[H][D / 32];
   {
     const T* p = q + b * qa.sb + l * qa.sl + (h * qa.G + gi) * qa.sh + g * (D / 4);
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
-      const typename Vec8<T>::type in = load8_any<T>(p + j * 8);
+      u32x4 bits = __builtin_bit_cast(u32x4, load8_any<T>(p + j * 8));
+      if (qa.flip) bits ^= 0x80008000u;
+      const typename Vec8<T>::type in = __builtin_bit_cast(typename Vec8<T>::type, bits);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if constexpr (H == 2) {
@@ -318,13 +412,24 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(T* y, float* part, const
   f32x4 acc[VD];
 #pragma unroll
   for (int n = 0; n < VD; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float top = -INFINITY, sum = 0.f;  // sum: of this lane's tokens
-
+  float top = -INFINITY, sum = 0.f;  // top: of q . k, before its scale; sum: of this lane's tokens
+  const float scale = qa.scale;
   const uint64_t head = (uint64_t)h * c.head_step;
-  const uint8_t *kp = c.k + head * 16, *ksp = c.ks + head, *vp = c.v + head * 16, *vsp = c.vs + head;
+  // this lane's byte of four tokens' scales, turned to where an exponent stands
+  const uint32_t turn = ((D == 128 ? r / 4 : r / 8) * 8 + 9) & 31;
 
-  // one step: tokens t0 .. t0 + 31
-  auto step = [&](const KvStep<D>& s, int t0) {
+  bool left_out = false;  // whether a step was
+
+  // One step: tokens t0 .. t0 + 31; MASK: those before `low` and after a row's last are left out; SLOW: its values token
+  // by token. KV_RUN: at `place` of head 0.
+  auto one = [&](auto mask, auto slow, KvStep<D, MODE>& s, int t0, int low, uint32_t place) {
+    constexpr bool MASK = decltype(mask)::value, SLOW = decltype(slow)::value;
+    if constexpr (MASK) s.drop_unseen(t0, (int)seen, g);
+    const bool big = __builtin_amdgcn_ballot_w64(s.template any_big<MASK>()) != 0;
+    if (big != SLOW) {
+      left_out = left_out || big;
+      return;
+    }
     f32x4 sc[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -336,48 +441,51 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(T* y, float* part, const
         for (int f = 0; f < H; ++f) sc[u] = mfma16(a, qf[f][j], sc[u]);
       }
     }
-    float p[8], most = -INFINITY;
+    auto here = [&](int n) {
+      const int t = t0 + (n / 4) * 16 + g * 4 + n % 4;
+      return t <= last && t >= low && (MODE == KV_RUN || s.at[MODE == KV_PLACES ? n : 0] != kNoPlace);
+    };
+    float p[8];
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      const int t = t0 + (n / 4) * 16 + g * 4 + n % 4;
-      p[n] = s.at[n] != kNoPlace && t <= last ? sc[n / 4][n % 4] * qa.scale : -INFINITY;
-      most = fmaxf(most, p[n]);
+      p[n] = sc[n / 4][n % 4];
+      if constexpr (MASK) p[n] = here(n) ? p[n] : -INFINITY;
     }
+    float most = kv_max(kv_max(kv_max(p[0], p[1]), kv_max(p[2], p[3])), kv_max(kv_max(p[4], p[5]), kv_max(p[6], p[7])));
     most = xlane_fmax<32>(xlane_fmax<16>(most));
     if (__builtin_amdgcn_ballot_w64(most > top)) {
-      const float now = fmaxf(top, most), safe = now == -INFINITY ? 0.f : now;
-      const float f = __builtin_amdgcn_exp2f(top - safe);
+      const float now = kv_max(top, most);
+      const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((top - now) * scale);
       top = now;
       sum *= f;
 #pragma unroll
       for (int n = 0; n < VD; ++n) acc[n] *= f;
     }
-    const float safe = top == -INFINITY ? 0.f : top;
-    uint32_t big = 0;
+    const float from = -top * scale;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      p[n] = __builtin_amdgcn_exp2f(p[n] - safe);
-      sum += p[n];
-      if (s.at[n] != kNoPlace) {
+      p[n] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[n], scale, from));
+      // (a row that has seen nothing yet has no maximum, and a scale of 0 no -infinity)
+      if constexpr (MASK) p[n] = here(n) ? p[n] : 0.f;
+    }
+    sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    if constexpr (!SLOW) {
+      // P's high halves as they are, and what they leave out rounded
+      u32x4 hi, lo;
 #pragma unroll
-        for (int j = 0; j < KvStep<D>::VS; ++j) big = max(big, s.vs[n][j]);
+      for (int n = 0; n < 4; ++n) {
+        const uint32_t a = __builtin_bit_cast(uint32_t, p[2 * n]), b = __builtin_bit_cast(uint32_t, p[2 * n + 1]);
+        hi[n] = __builtin_amdgcn_perm(b, a, 0x07060302);
+        const float x = p[2 * n] - __builtin_bit_cast(float, a & 0xffff0000u);
+        const float z = p[2 * n + 1] - __builtin_bit_cast(float, b & 0xffff0000u);
+        lo[n] = __builtin_bit_cast(uint32_t, bf16x2{(bf16)x, (bf16)z});
       }
-    }
-    bf16x8 ph, pl;
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      ph[n] = (bf16)p[n];
-      pl[n] = (bf16)(p[n] - (float)ph[n]);
-    }
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(big >= 253u) == 0, 1)) {
+      const bf16x8 ph = __builtin_bit_cast(bf16x8, hi), pl = __builtin_bit_cast(bf16x8, lo);
       kv_each_byte<D, 0>([&](auto byte) {
         constexpr int B = decltype(byte)::value;
         uint32_t w[8];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const uint32_t e = s.template value_byte<B>(n, r);
-          w[n] = kv_pair<B>(s.v[n], e8m0_operand(s.at[n] != kNoPlace ? e : 127u));
-        }
+        for (int n = 0; n < 8; ++n) w[n] = kv_pair<B>(s.v[n], s.template value_scale_of<B>(n, r, turn));
         u32x4 even, odd;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
@@ -386,8 +494,8 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(T* y, float* part, const
         }
         const bf16x8 a0 = __builtin_bit_cast(bf16x8, even), a1 = __builtin_bit_cast(bf16x8, odd);
         acc[2 * B] = mfma16(a0, ph, acc[2 * B]);
-        acc[2 * B] = mfma16(a0, pl, acc[2 * B]);
         acc[2 * B + 1] = mfma16(a1, ph, acc[2 * B + 1]);
+        acc[2 * B] = mfma16(a0, pl, acc[2 * B]);
         acc[2 * B + 1] = mfma16(a1, pl, acc[2 * B + 1]);
       });
     } else {
@@ -395,52 +503,136 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(T* y, float* part, const
 #pragma unroll 1
       for (int t = 0; t < kKvTile; ++t) {
         const int from = ((t % 16) / 4) * 16 + r, n = (t / 16) * 4 + t % 4;
-        float mine_p = 0.f;
-        uint32_t place = kNoPlace;
+        float mine = 0.f;
+        uint32_t at = place + t * row16;
 #pragma unroll
         for (int m = 0; m < 8; ++m) {
           if (m == n) {
-            mine_p = p[m];
-            place = s.at[m];
+            mine = p[m];
+            if constexpr (MODE == KV_PLACES) at = s.at[m];
           }
         }
-        const float pt = __shfl(mine_p, from);
-        place = (uint32_t)__shfl((int)place, from);
-        const bool seen_here = place != kNoPlace && t0 + t <= last;
-        const uint64_t from_place = seen_here ? place : 0u;
+        const float pt = __shfl(mine, from);
+        if constexpr (MODE == KV_PLACES) at = (uint32_t)__shfl((int)at, from);
+        const bool sees = t0 + t <= last && t0 + t >= low && at != kNoPlace;
+        const uint64_t to = head + (sees ? at : 0u);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int m = 0; m < VD; ++m) {
             const int d = VD * (4 * g + i) + m;
-            const uint32_t code = vp[from_place * 16 + d / 2], e = vsp[from_place + d / 32];
-            const uint32_t pair = fp4_pair<0>(code, e8m0_operand(e));
+            const uint32_t pair = fp4_pair<0>(c.v[to * 16 + d / 2], e8m0_operand(c.vs[to + d / 32]));
             const float v = pt * __builtin_bit_cast(float, d & 1 ? pair & 0xffff0000u : pair << 16);
-            acc[m][i] += seen_here ? v : 0.f;
+            acc[m][i] += sees ? v : 0.f;
           }
       }
     }
   };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
 
-  // this workgroup's steps: a share of whole rounds of its four waves
+  // This workgroup's steps are a share of whole rounds of its four waves, this wave's each fourth. The next one's loads
+  // are on the way while a step is computed, where the registers hold both.
+  constexpr bool TWO = D <= 128;
   const uint32_t steps = (seen + kKvTile - 1) / kKvTile, rounds = (steps + 3) / 4, per = (rounds + splits - 1) / splits;
-  const uint32_t from = min(split * per * 4 * kKvTile, seen), to = min((split + 1) * per * 4 * kKvTile, seen);
-  for (uint32_t c0 = from; c0 < to; c0 += kKvChunk) {
-    const uint32_t n = min(to - c0, (uint32_t)kKvChunk), padded = (n + kKvTile - 1) / kKvTile * kKvTile;
-    __syncthreads();  // the places before these have been read
-    for (uint32_t t = tid; t < padded; t += 256)
-      smem[t] = t < n ? kv_place(c, tb, page, row16, b, c0 + t) : kNoPlace;
-    __syncthreads();
-    const uint32_t here = padded / kKvTile;
-    if ((uint32_t)wave < here) {
-      KvStep<D> s0, s1;
-      s0.load(kp, ksp, vp, vsp, smem + wave * kKvTile, r, g);
-      for (uint32_t i = wave; i < here; i += 8) {
-        if (i + 4 < here) s1.load(kp, ksp, vp, vsp, smem + (i + 4) * kKvTile, r, g);
-        step(s0, (int)(c0 + i * kKvTile));
-        if (i + 4 >= here) break;
-        if (i + 8 < here) s0.load(kp, ksp, vp, vsp, smem + (i + 8) * kKvTile, r, g);
-        step(s1, (int)(c0 + (i + 4) * kKvTile));
+  if constexpr (MODE == KV_RUN) {
+    const uint32_t first = min(split * per * 4, steps) + wave, end = min((split + 1) * per * 4, steps);
+    // where step i's tokens begin: a page that ends inside a step is the last one, and the step ends with it
+    auto start = [&](uint32_t i) { return min(i * kKvTile, tb.capacity - kKvTile); };
+    // its page's number, by a scalar load that nothing waits for until it is a place; kNoPlace past `to`
+    auto page_of = [&](uint32_t i, uint32_t to) -> uint32_t {
+      if (i >= to) return kNoPlace;
+      if (!tb.pages) return b;
+      typedef const __attribute__((address_space(4))) uint32_t* Scalar;
+      return ((Scalar)(uintptr_t)tb.pages)[b * tb.step + page.div(start(i))];
+    };
+    auto place_of = [&](uint32_t i, uint32_t id) -> uint32_t {
+      uint32_t slot;
+      page.divmod(start(i), slot);
+      return id < c.pages ? (uint32_t)(id * c.page_step) + slot * row16 : kNoPlace;
+    };
+    // steps up to here need no mask
+    const uint32_t plain = min(end, whole < kKvTile - 1 ? 0u : ((uint32_t)whole + 1) / kKvTile);
+    KvStep<D, MODE> s0, s1;
+    uint32_t i = first, id0 = page_of(i, plain), id1 = page_of(i + 4, plain), id2 = page_of(i + 8, plain);
+    const uint32_t mark = first + (plain > first ? (plain - first + 3) / 4 * 4 : 0), marked = page_of(mark, end);
+    uint32_t p0 = place_of(i, id0), p1 = place_of(i + 4, id1);
+    // Loads stand under no condition (page 0's for a step that has none): behind one the compiler would wait for all.
+    auto load = [&](KvStep<D, MODE>& s, uint32_t at) { s.load_run(c, head + (at == kNoPlace ? 0u : at), r, g); };
+    if constexpr (TWO) load(s0, p0);
+    // those that do, first: their loads wait beside the others'
+    for (uint32_t j = mark; j < end; j += 4) {
+      const uint32_t at = place_of(j, j == mark ? marked : page_of(j, end));
+      if (at == kNoPlace) continue;
+      s1.load_run(c, head + at, r, g);
+      one(yes, no, s1, (int)start(j), (int)(j * kKvTile), at);
+    }
+    while (i < plain) {
+      const uint32_t p2 = place_of(i + 8, id2);
+      id2 = page_of(i + 12, plain);
+      if constexpr (TWO) {
+        load(s1, p1);
+        if (p0 != kNoPlace) one(no, no, s0, (int)(i * kKvTile), 0, p0);
+        i += 4;
+        if (i >= plain) break;
+        const uint32_t p3 = place_of(i + 8, id2);
+        id2 = page_of(i + 12, plain);
+        load(s0, p2);
+        if (p1 != kNoPlace) one(no, no, s1, (int)(i * kKvTile), 0, p1);
+        i += 4;
+        p0 = p2;
+        p1 = p3;
+      } else {
+        if (p0 != kNoPlace) {
+          s0.load_run(c, head + p0, r, g);
+          one(no, no, s0, (int)(i * kKvTile), 0, p0);
+        }
+        i += 4;
+        p0 = p1;
+        p1 = p2;
+      }
+    }
+    if (left_out) {
+#pragma unroll 1
+      for (uint32_t j = first; j < end; j += 4) {
+        const uint32_t at = place_of(j, page_of(j, end));
+        if (at == kNoPlace) continue;
+        s0.load_run(c, head + at, r, g);
+        one(yes, yes, s0, (int)start(j), (int)(j * kKvTile), at);
+      }
+    }
+  } else {
+    const uint32_t from = min(split * per * 4 * kKvTile, seen), to = min((split + 1) * per * 4 * kKvTile, seen);
+    for (uint32_t c0 = from; c0 < to; c0 += kKvChunk) {
+      const uint32_t n = min(to - c0, (uint32_t)kKvChunk), padded = (n + kKvTile - 1) / kKvTile * kKvTile;
+      __syncthreads();  // the places before these have been read
+      for (uint32_t t = tid; t < padded; t += 256)
+        smem[t] = t < n ? kv_place(c, tb, page, row16, b, c0 + t) : kNoPlace;
+      __syncthreads();
+      const uint32_t here = padded / kKvTile;
+      KvStep<D, MODE> s0, s1;
+      left_out = false;
+      if constexpr (TWO) {
+        if ((uint32_t)wave < here) s0.load_places(c, head, smem + wave * kKvTile, r, g);
+        for (uint32_t i = wave; i < here; i += 8) {
+          s1.load_places(c, head, smem + min(i + 4, here - 1) * kKvTile, r, g);
+          one(yes, no, s0, (int)(c0 + i * kKvTile), 0, 0u);
+          if (i + 4 >= here) break;
+          s0.load_places(c, head, smem + min(i + 8, here - 1) * kKvTile, r, g);
+          one(yes, no, s1, (int)(c0 + (i + 4) * kKvTile), 0, 0u);
+        }
+      } else {
+        for (uint32_t i = wave; i < here; i += 4) {
+          s0.load_places(c, head, smem + i * kKvTile, r, g);
+          one(yes, no, s0, (int)(c0 + i * kKvTile), 0, 0u);
+        }
+      }
+      if (left_out) {
+#pragma unroll 1
+        for (uint32_t i = wave; i < here; i += 4) {
+          s0.load_places(c, head, smem + i * kKvTile, r, g);
+          one(yes, yes, s0, (int)(c0 + i * kKvTile), 0, 0u);
+        }
       }
     }
   }
@@ -456,7 +648,7 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(T* y, float* part, const
   float all = stat[0][r][0];
 #pragma unroll
   for (int w = 1; w < 4; ++w) all = fmaxf(all, stat[w][r][0]);
-  const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - all);
+  const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((top - all) * scale);
   float* const rows = reinterpret_cast<float*>(smem);
   float* const out = rows + (wave * 16 + r) * PITCH + g * (D / 4);
 #pragma unroll
@@ -478,7 +670,7 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(T* y, float* part, const
     for (int w = 0; w < 4; ++w) {
       const float t = stat[w][row][0];
       if (t == -INFINITY) continue;
-      total += stat[w][row][1] * __builtin_amdgcn_exp2f(t - m);
+      total += stat[w][row][1] * __builtin_amdgcn_exp2f((t - m) * scale);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += rows[(w * 16 + row) * PITCH + d + j];
     }
@@ -505,45 +697,55 @@ __global__ __launch_bounds__(256) void kv_attend_kernel(T* y, float* part, const
   }
 }
 
-// The shares' sums of one query row: eight of them at a time, four channels a lane.
+// The shares' sums of one query row, added by a workgroup: a thread a share for their weights, then four channels a lane
+// and several shares at a time.
+constexpr int kKvShares = 256;
+
 template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_join_kernel(T* y, const float* part, uint32_t splits, uint32_t units,
-                                                      KvQuery qa, FastDiv group, uint32_t tiles16) {
+__global__ __launch_bounds__(256) void kv_join_kernel(T* y, const float* part, uint32_t splits, KvQuery qa,
+                                                      FastDiv group, FastDiv rows, uint32_t tiles16) {
   constexpr int LANES = D / 4, PAR = 256 / LANES;
+  __shared__ float weight[kKvShares];
   __shared__ float sums[PAR][D];
-  __shared__ float totals[PAR];
-  const uint32_t unit = blockIdx.x / 16, row = blockIdx.x % 16;  // unit: (sequence, head, tile of rows)
-  const uint32_t tile16 = unit % tiles16, i = tile16 * 16 + row;
-  if (i >= qa.rows) return;
-  const float* p = part + ((uint64_t)unit * splits * 16 + row) * (D + 4);
+  __shared__ float tops[4], totals[4];
+  uint32_t i, gi;
+  const uint32_t bh = rows.divmod(blockIdx.x, i);  // (sequence, head) and query row
+  const uint32_t unit = bh * tiles16 + i / 16;
+  const float* p = part + ((uint64_t)unit * splits * 16 + i % 16) * (D + 4);
   const int64_t step = 16 * (D + 4);
-  float m = -INFINITY;
-  for (uint32_t s = 0; s < splits; ++s) m = fmaxf(m, p[s * step + D]);
-  const int lane = threadIdx.x % LANES, at = threadIdx.x / LANES;
+  const int t = threadIdx.x, wave = t / kWave;
+  const bool mine = (uint32_t)t < splits;
+  const float own = mine ? p[t * step + D] : -INFINITY, count = mine ? p[t * step + D + 1] : 0.f;
+  float m = kv_max(own, xlane_dpp<1>(own));
+  m = kv_max(m, xlane_dpp<2>(m));
+  m = kv_max(m, xlane_dpp<4>(m));
+  m = kv_max(m, xlane_dpp<8>(m));
+  m = xlane_fmax<32>(xlane_fmax<16>(m));
+  if (t % kWave == 0) tops[wave] = m;
+  __syncthreads();
+  m = kv_max(kv_max(tops[0], tops[1]), kv_max(tops[2], tops[3]));
+  const float w = own == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((own - m) * qa.scale);
+  weight[t] = w;
+  const float all = wave_sum(own == -INFINITY ? 0.f : count * w);
+  if (t % kWave == 0) totals[wave] = all;
+  __syncthreads();
+  const int lane = t % LANES, at = t / LANES;
   if (at < PAR) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    float total = 0.f;
+#pragma unroll 4
     for (uint32_t s = at; s < splits; s += PAR) {
-      const float t = p[s * step + D];
-      if (t == -INFINITY) continue;
-      const float f = __builtin_amdgcn_exp2f(t - m);
-      total += p[s * step + D + 1] * f;
-      v += *reinterpret_cast<const f32x4*>(p + s * step + lane * 4) * f;
+      const float f = weight[s];
+      if (f != 0.f) v += *reinterpret_cast<const f32x4*>(p + s * step + lane * 4) * f;  // (NaN is not 0)
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) sums[at][lane * 4 + j] = v[j];
-    if (lane == 0) totals[at] = total;
   }
   __syncthreads();
-  const uint32_t bh = unit / tiles16, heads = qa.Hq / qa.G, b = bh / heads, h = bh - b * heads;
-  uint32_t gi;
-  const uint32_t l = group.divmod(i, gi);
-  float total = 0.f;
-#pragma unroll
-  for (int s = 0; s < PAR; ++s) total += totals[s];
+  const uint32_t heads = qa.Hq / qa.G, b = bh / heads, h = bh - b * heads, l = group.divmod(i, gi);
+  const float total = (totals[0] + totals[1]) + (totals[2] + totals[3]);
   const float inv = m == -INFINITY ? 0.f : 1.f / total;
   T* to = y + (((uint64_t)b * qa.L + l) * qa.Hq + h * qa.G + gi) * D;
-  for (int d = threadIdx.x; d < D; d += 256) {
+  for (int d = t; d < D; d += 256) {
     float v = 0.f;
 #pragma unroll
     for (int s = 0; s < PAR; ++s) v += sums[s][d];
@@ -596,15 +798,16 @@ bool kv_meets(const fd_kv_shape& s, const KvCache& c, const void* p, int64_t n) 
          overlaps(p, n, c.vs, scales);
 }
 
-// Query rows of a workgroup's tile, and the shares that a sequence's tokens are cut into: as many as give every CU about
-// four workgroups, each with 256 tokens at least of a cache that is full.
+// Query rows of a workgroup's tile, and the shares that a sequence's tokens are cut into: as many as give every CU two
+// workgroups, each with 256 tokens at least of a cache that is full. (One, two, three, four workgroups a CU, with the
+// join: one sequence of 131072 tokens, 8 heads of 128, 55, 45, 48, 51 us; 32 of 2048 to 8192, 85, 56, 57, 58.)
 int64_t kv_tiles(int64_t L, int64_t G) { return (L * G + 15) / 16; }
 int64_t kv_splits(int64_t B, int64_t L, int64_t Hq, int64_t heads, int64_t capacity) {
   const int64_t units = B * heads * kv_tiles(L, Hq / heads);
-  int64_t s = units > 0 ? (4 * device_cus() + units - 1) / units : 1;
+  int64_t s = units > 0 ? (2 * device_cus() + units - 1) / units : 1;
   const int64_t most = (capacity + 255) / 256;
   if (s > most) s = most;
-  return s < 1 ? 1 : s > 256 ? 256 : s;
+  return s < 1 ? 1 : s > kKvShares ? kKvShares : s;
 }
 
 template <typename T, int D>
@@ -612,11 +815,14 @@ int kv_attend_launch(T* y, float* scratch, const T* q, const KvCache& c, const K
                      int64_t splits, hipStream_t st) {
   const int64_t tiles = kv_tiles(qa.L, qa.G);
   const FastDiv group(qa.G);
-  hipLaunchKernelGGL((kv_attend_kernel<T, D>), dim3((unsigned)splits, (unsigned)(c.heads * tiles), (unsigned)B), dim3(256),
-                     0, st, y, scratch, q, c, tb, qa, FastDiv(c.page), group, (uint32_t)(D / 32), (uint32_t)tiles);
+  // steps in one run of slots: pages of whole steps, or a sequence in one page of a step at least
+  const bool run = tb.pages ? c.page % kKvTile == 0 && tb.capacity > 0 : c.page >= kKvTile;
+  auto kernel = run ? kv_attend_kernel<T, D, KV_RUN> : kv_attend_kernel<T, D, KV_PLACES>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)splits, (unsigned)(c.heads * tiles), (unsigned)B), dim3(256), 0, st, y,
+                     scratch, q, c, tb, qa, FastDiv(c.page), group, (uint32_t)tiles);
   if (splits > 1)
-    hipLaunchKernelGGL((kv_join_kernel<T, D>), dim3((unsigned)(B * c.heads * tiles * 16)), dim3(256), 0, st, y, scratch,
-                       (uint32_t)splits, (uint32_t)(B * c.heads * tiles), qa, group, (uint32_t)tiles);
+    hipLaunchKernelGGL((kv_join_kernel<T, D>), dim3((unsigned)(B * c.heads * qa.rows)), dim3(256), 0, st, y, scratch,
+                       (uint32_t)splits, qa, group, FastDiv(qa.rows), (uint32_t)tiles);
   return FD_OK;
 }
 
@@ -761,7 +967,8 @@ extern "C" int fd_attend_kv_fp4(void* y, const void* q, const void* k, const voi
   int64_t splits = kv_splits(B, L, Hq, shape->heads, tb.capacity);
   while (splits > 1 && (!scratch || scratch_bytes < B * shape->heads * tiles * splits * 16 * (shape->dim + 4) * 4))
     --splits;
-  const KvQuery qa{sqb, sql, sqh, (uint32_t)L, (uint32_t)Hq, (uint32_t)G, (uint32_t)(L * G), scale * 1.4426950408889634f};
+  const KvQuery qa{sqb, sql, sqh, (uint32_t)L, (uint32_t)Hq, (uint32_t)G, (uint32_t)(L * G),
+                   std::fabs(scale) * 1.4426950408889634f, scale < 0.f};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (act_dtype == FD_F16)
     kv_attend_pick<f16>(shape->dim, static_cast<f16*>(y), scratch, static_cast<const f16*>(q), c, tb, qa, B, splits, st);
