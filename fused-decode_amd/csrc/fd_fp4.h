@@ -36,11 +36,31 @@ __device__ __forceinline__ bf16x8 fp4_to_bf16(uint32_t codes, float scale) {
 // The conversion's scale of an E8M0 byte: it reads the exponent alone, 0 as 2^-127 and 255 as NaN.
 __device__ __forceinline__ float e8m0_operand(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
 
-// float16 as two bfloat16 numbers: the second one's three bits are exact, and it is 0 beside an infinity or a NaN.
-__device__ __forceinline__ void split_f16(float v, bf16& hi, bf16& lo) {
-  hi = (bf16)v;
-  const float rest = v - (float)hi;
-  lo = (bf16)(fabsf(v) <= 65504.f ? rest : 0.f);
+// float16 as two bfloat16 numbers: its first eight bits, and the three behind them, which are exact; 0 beside an infinity
+// or a NaN.
+__device__ __forceinline__ void split_f16(f16x8 v, bf16x8& hi, bf16x8& lo) {
+  u32x4 a, b;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = (float)v[2 * i], y = (float)v[2 * i + 1];
+    const uint32_t xb = __builtin_bit_cast(uint32_t, x), yb = __builtin_bit_cast(uint32_t, y);
+    const float xl = x - __builtin_bit_cast(float, xb & 0xffff0000u), yl = y - __builtin_bit_cast(float, yb & 0xffff0000u);
+    a[i] = __builtin_amdgcn_perm(yb, xb, 0x07060302);
+    b[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, yl), __builtin_bit_cast(uint32_t, xl), 0x07060302);
+  }
+  const u32x4 bits = __builtin_bit_cast(u32x4, v), top = bits & 0x7c007c00u;
+  uint32_t odd = 0;  // bit 15 of a half: its exponent is all ones
+#pragma unroll
+  for (int i = 0; i < 4; ++i) odd |= top[i] + 0x04000400u;
+  if (__builtin_amdgcn_ballot_w64(odd & 0x80008000u)) {  // rare, and the same for the whole wave
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t bad = top[i] + 0x04000400u;
+      b[i] &= (bad & 0x8000u ? 0u : 0xffffu) | (bad & 0x80000000u ? 0u : 0xffff0000u);
+    }
+  }
+  hi = __builtin_bit_cast(bf16x8, a);
+  lo = __builtin_bit_cast(bf16x8, b);
 }
 
 // One 16-byte-per-lane DMA from a pointer a lane into LDS at byte address `lds` (wave-uniform; lane L lands at 16 L).
@@ -90,5 +110,12 @@ struct Fp4Args {
   int act_dtype;
   hipStream_t st;
 };
+
+// One row (fp4_one.hip): any K.
+int fp4_one_launch(const Fp4Args& a);
+
+// Few rows (fp4_few.hip): whether a product fits, and its launch.
+bool fp4_few_fits(int64_t M, int64_t K, bool swiglu);
+int fp4_few_launch(const Fp4Args& a);
 
 }  // namespace fd

@@ -209,13 +209,7 @@ __global__ __launch_bounds__(256) void fp4_x_kernel(bf16* to, int64_t lo_off, co
   }
   if constexpr (std::is_same<T, f16>::value) {
     bf16x8 hi, lo;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      bf16 h, l;
-      split_f16(to_f32(in[i]), h, l);
-      hi[i] = h;
-      lo[i] = l;
-    }
+    split_f16(in, hi, lo);
     store8<bf16>(to + (int64_t)v * 8, hi);
     store8<bf16>(to + lo_off + (int64_t)v * 8, lo);
   } else {
@@ -225,7 +219,7 @@ __global__ __launch_bounds__(256) void fp4_x_kernel(bf16* to, int64_t lo_off, co
 
 namespace {
 
-constexpr int64_t kF4Most = 0x7fffffffLL - 512;  // indexes run to the end of the last tile and stage
+constexpr int64_t kF4Most = 0x7fffffffLL - 8192;  // indexes run to the end of the last tile, stage and chunk
 
 struct Fp4Plan {
   int splits;
@@ -277,6 +271,8 @@ int f4_pick(const Fp4Args& a, const bf16* x, int64_t lo_off, int64_t sxm, int sp
 
 template <typename T, bool SWIGLU>
 int f4_product(Fp4Args a) {
+  if (a.M == 1) return fp4_one_launch(a);
+  if (fp4_few_fits(a.M, a.K, SWIGLU)) return fp4_few_launch(a);
   constexpr bool F16 = std::is_same<T, f16>::value;
   const bf16* x = static_cast<const bf16*>(a.x);
   int64_t sxm = a.sxm, lo_off = 0;
@@ -318,6 +314,7 @@ extern "C" int fd_linear_fp4_scratch(int64_t M, int64_t N, int64_t K, int act_dt
   if (!bytes) return set_error(FD_EINVAL, "null pointer argument");
   *bytes = 0;
   if (M == 0 || N == 0 || K == 0 || M > kF4Most || N > kF4Most || K > kF4Most) return FD_OK;
+  if (M == 1 || (fp4_few_fits(M, K, false) && fp4_few_fits(M, K, true))) return FD_OK;
   *bytes = f4_copy_bytes(M, K, act_dtype);
   const int s = f4_splits(M, N, K);
   if (s > 1) *bytes += (int64_t)s * M * N * 4;

@@ -395,17 +395,10 @@ __global__ __launch_bounds__(256, D <= 128 && MODE == KV_RUN ? 3 : 2) void kv_at
       u32x4 bits = __builtin_bit_cast(u32x4, load8_any<T>(p + j * 8));
       if (qa.flip) bits ^= 0x80008000u;
       const typename Vec8<T>::type in = __builtin_bit_cast(typename Vec8<T>::type, bits);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (H == 2) {
-          bf16 hi, lo;
-          split_f16(to_f32(in[i]), hi, lo);
-          qf[0][j][i] = hi;
-          qf[H - 1][j][i] = lo;
-        } else {
-          qf[0][j][i] = in[i];
-        }
-      }
+      if constexpr (H == 2)
+        split_f16(in, qf[0][j], qf[H - 1][j]);
+      else
+        qf[0][j] = in;
     }
   }
 

@@ -502,7 +502,7 @@ int fd_linear_w8a8_form(int64_t M, int64_t N, int64_t K, int* form);
  *   y[m,j] = round(silu(v[m,j]) * v[m,I+j] + row_add[m,j])
  * Weights are exact in the product; sums and the epilogue are float32 with one rounding. bias (N
  * values at stride sb) and row_add (strides srm, srn; 0 broadcasts) have any of the three dtypes
- * and may be NULL. M, N and K are below 2^31 - 512; rows of codes are 16-byte aligned (else
+ * and may be NULL. M, N and K are below 2^31 - 8192; rows of codes are 16-byte aligned (else
  * FD_EUNSUPPORTED). `scratch` (16-byte aligned, caller-owned, not shared with a call that may
  * overlap) holds what fd_linear_fp4_scratch says (0: none): copies of activations that are
  * float16, off 16-byte alignment or of no whole 128 along K (without it FD_EUNSUPPORTED), and,
