@@ -13,6 +13,14 @@
 // The run of a workgroup is N / workgroups rows, to the row; a last tile shorter than 16 rows reads its last row again in
 // the lanes past it.
 //
+// Bound by a launch's start and end, the activations' and the scales' way into registers and LDS in front of the stream,
+// and then by the stream: 13 x 28672 x 4096 SWIGLU float16 20.8 us (3.0 TB/s of weights), of which the units alone, nothing
+// multiplied, take 17.6, the scales 2 and the activations 0.5; 13 x 4096 x 14336 bfloat16 21.9 (units alone 12.3,
+// activations 4.3, scales 2.2), float16, whose two parts take twice the registers and so more phases, 29; 13 x 6144 x 4096
+// 10.2; 29 x 5003 x 2051 float16 23. Activations loaded 64 bytes of a row at a time and exchanged between lane groups took
+// as long (20.7, 22.6, 10.5), and loading them and the scales before the first units longer (22.4, 23.9, 11.6): the stream
+// then starts later.
+//
 // Slot layout: 16 rows of 8 pieces of 16 bytes, piece c at c ^ (row mod 8).
 #include "fd_fp4.h"
 
@@ -21,10 +29,7 @@ namespace fd {
 constexpr int kF4Waves = 8;
 constexpr int kF4Step = 256;   // k of a unit
 constexpr int kF4Tiles = 16;   // tiles of a workgroup at most
-#ifndef FP4_FEW_D
-#define FP4_FEW_D 5
-#endif
-constexpr int kF4Ring = FP4_FEW_D;
+constexpr int kF4Ring = 5;     // slots of a wave (4, 5, 6, 7: 13 x 28672 x 4096 26.2, 26.8, 27.6, 28.1 us captured)
 
 // Bytes of a scale row in LDS: whole words, and an odd number of them, so that 16 rows' bytes lie in different banks.
 __host__ __device__ __forceinline__ int f4_scale_pitch(int pieces) { return (((pieces + 7) / 8 * 8) / 4 | 1) * 4; }

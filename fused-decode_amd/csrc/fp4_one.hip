@@ -3,11 +3,12 @@
 //
 // A wave owns R weight rows (SWIGLU: R / 2 outputs' gate and up rows) over all of K. A chunk is 64 pieces of a row, one a
 // lane: 16 bytes of codes, their scale, and the 32 activations that all rows share, which a workgroup has in LDS, quarters
-// of the pieces together (a lane's 64 bytes straight from memory are a line a lane and load: 19.7 us where this takes
-// ONE_G1). bfloat16 codes take their scale in the conversion; float16 ones are converted without it (they would leave
+// of the pieces together (a lane's 64 bytes straight from memory are a line a lane and load: 6144 x 4096 7.2 us captured
+// where this takes 6.15). bfloat16 codes take their scale in the conversion; float16 ones are converted without it (they would leave
 // float16's range) and a piece's sum takes it, exactly. v_dot2 adds two products in float32. Two chunks are on the way.
 //
-// Bound by a launch's start and end and by the weights' stream.
+// Bound by a launch's start and end and by the instructions around the weights' stream, half of them outside of the
+// products: 6144 x 4096 5.4 us (2.5 TB/s), 28672 x 4096 SWIGLU 13.5 (4.6), 4096 x 14336 8.4 (3.7).
 #include "fd_fp4.h"
 
 namespace fd {
@@ -161,12 +162,13 @@ int fp4_one_go(const Fp4Args& a) {
   return FD_OK;
 }
 
-#ifndef FP4_ONE_R
-#define FP4_ONE_R 2
-#endif
+// Rows of a wave: two and four take the same time where there are many (28672 x 4096 SWIGLU 18.4, 18.5 us captured), two
+// less where there are few (6144 x 4096 6.15, 6.65; 4096 x 14336 10.8, 11.3).
+constexpr int kOneRows = 2;
+
 template <typename T>
 int fp4_one_pick(const Fp4Args& a) {
-  return a.swiglu ? fp4_one_go<T, FP4_ONE_R, true>(a) : fp4_one_go<T, FP4_ONE_R, false>(a);
+  return a.swiglu ? fp4_one_go<T, kOneRows, true>(a) : fp4_one_go<T, kOneRows, false>(a);
 }
 
 }  // namespace

@@ -34,6 +34,18 @@ With weights="fp8" the four projections hold E4M3 codes with per-row scales
 with the residual) and post_attn_mlp_fp8: four launches per layer, with the same
 row-sum handoff from 5 rows.
 
+With weights="fp4" a layer is whole: E2M1 projections (quantize_fp4), attention over a key/value cache held in 4 bits
+(``context`` tokens a sequence, the new one among them), and norms on both sides of each block, nine launches a layer or
+ten where the attention is cut into shares:
+
+    qkv  = linear_fp4(y, *w_qkv)                          # y: the block's normed input, of the norms before
+    q, k = rope(qkv[:, :5120])
+    append_kv_fp4(cache, k, v, lengths)
+    o    = linear_fp4(attend_kv_fp4(q, cache, lengths), *w_o)
+    y, h = norm_add_norm(o, x, post_attn_norm, mlp_norm)
+    mid  = linear_fp4(y, *w_gate_up, activation="swiglu")
+    y, x = norm_add_norm(linear_fp4(mid, *w_down), h, post_mlp_norm, next_attn_norm)
+
 Weights per layer: 436,207,616 bytes in fp16 (13.96 GB for 32 layers), half that
 plus the scales in fp8, random with the benchmark distributions (no checkpoint
 is loaded).
@@ -46,9 +58,12 @@ import json
 
 import torch
 
+from .block_norms import norm_add_norm
+from .fp4 import linear_fp4, quantize_fp4
 from .kernels import _MFMA_MIN_M
+from .kv_fp4 import KvCacheFp4, append_kv_fp4, attend_kv_fp4
 from .fp8 import linear_decode_fp8, post_attn_mlp_fp8, pre_attn_qkv_fp8, quantize_fp8
-from .ops import add_rms_norm, linear_decode, post_attn_mlp, pre_attn_qkv, rope
+from .ops import add_rms_norm, linear_decode, post_attn_mlp, pre_attn_qkv, rms_norm, rope
 from .rowsq import (linear_fp8_sumsq, linear_sumsq, post_attn_mlp_fp8_sumsq, post_attn_mlp_sumsq,
                     pre_attn_qkv_fp8_sumsq, pre_attn_qkv_sumsq, sumsq_buffer)
 
@@ -70,15 +85,15 @@ class DecodeStep:
 
     def __init__(self, m: int = 1, layers: int = 32, dtype=torch.float16, device="cuda",
                  seed: int = 0, h: int = H, i: int = I, kind: str | None = None, position: int = 1024,
-                 fused: bool = True, weights: str = "fp16", rowsq: bool = True):
-        if weights not in ("fp16", "fp8"):
-            raise ValueError("weights must be 'fp16' (the activation dtype) or 'fp8'")
+                 fused: bool = True, weights: str = "fp16", rowsq: bool = True, context: int = 1024):
+        if weights not in ("fp16", "fp8", "fp4"):
+            raise ValueError("weights must be 'fp16' (the activation dtype), 'fp8' or 'fp4'")
         self.m, self.layers, self.dtype, self.kind, self.fused = m, layers, dtype, kind, fused
-        self.fp8 = weights == "fp8"
+        self.fp8, self.fp4 = weights == "fp8", weights == "fp4"
         # the row-sum handoff needs the MFMA kernels (the fp8 forms take them from
         # 5 rows whatever the kind)
         mfma = m >= _MFMA_MIN_M and (self.fp8 or (kind or "dot") == "dot")
-        self.rowsq = rowsq and fused and mfma
+        self.rowsq = rowsq and fused and mfma and not self.fp4
         self.h, self.i = h, i
         heads = h // HEAD_DIM
         kv = max(1, heads // 4)
@@ -90,8 +105,9 @@ class DecodeStep:
             t = torch.randn(*shape, generator=g, device=device, dtype=torch.float32)
             return (t * scale + mean).to(dtype)
 
-        # projections as activation-dtype weights, or as E4M3 codes + per-row scales
-        proj = (lambda *shape, scale: quantize_fp8(rnd(*shape, scale=scale))) if self.fp8 else rnd
+        # projections as activation-dtype weights, as E4M3 codes + per-row scales, or as E2M1 codes + scales of 32
+        quantize = quantize_fp8 if self.fp8 else quantize_fp4
+        proj = (lambda *shape, scale: quantize(rnd(*shape, scale=scale))) if self.fp8 or self.fp4 else rnd
         self.w = []
         for _ in range(layers):
             self.w.append({
@@ -103,6 +119,13 @@ class DecodeStep:
                 "down": proj(h, i, scale=i ** -0.5),
                 "attn_out": rnd(m, h),  # stand-in for the attention output of this layer
             })
+        if self.fp4:
+            self.lengths = torch.full((m,), context, dtype=torch.int32, device=device)
+            for w in self.w:
+                w["post_attn"], w["post_mlp"] = (rnd(h, scale=0.1, mean=1.0) for _ in range(2))
+                w["cache"] = KvCacheFp4.empty(m, kv, context, HEAD_DIM, device=device)
+                append_kv_fp4(w["cache"], rnd(m, context, kv, HEAD_DIM), rnd(m, context, kv, HEAD_DIM), self.lengths)
+            position = context - 1
         cos, sin = llama3_angles(position, device=device)
         self.cos, self.sin = cos.to(dtype), sin.to(dtype)
         self.x_in = rnd(m, h)
@@ -122,13 +145,17 @@ class DecodeStep:
     def weight_bytes(self) -> int:
         e = torch.empty((), dtype=self.dtype).element_size()
         proj = self.qkv_n * self.h + self.h * self.h + 3 * self.h * self.i
-        if self.fp8:  # one byte per weight plus a float32 scale per row
+        if self.fp4:  # half a byte per weight plus a byte for 32 of them, four norms
+            per = proj * 17 // 32 + 4 * self.h * e
+        elif self.fp8:  # one byte per weight plus a float32 scale per row
             per = proj + 4 * (self.qkv_n + self.h + 2 * self.i + self.h) + 2 * self.h * e
         else:
             per = proj * e + 2 * self.h * e
         return per * self.layers
 
     def step(self) -> torch.Tensor:
+        if self.fp4:
+            return self._step_fp4()
         if self.rowsq:
             return self._step_rowsq()
         if self.fp8:
@@ -179,6 +206,24 @@ class DecodeStep:
         self.out.copy_(x)
         return self.out
 
+    def _step_fp4(self) -> torch.Tensor:
+        """The whole layer in 4 bits: projections, cache and attention, norms on both sides of each block."""
+        x, kv = self.x_in, (self.qkv_n // HEAD_DIM - self.qk_heads)
+        heads = self.qk_heads - kv
+        y = rms_norm(x, self.w[0]["attn_norm"], 1e-5)
+        for li, w in enumerate(self.w):
+            after = self.w[(li + 1) % self.layers]["attn_norm"]
+            qkv = linear_fp4(y, *w["qkv"]).view(self.m, 1, -1, HEAD_DIM)
+            qk = qkv[:, :, : self.qk_heads]
+            rope(qk, self.cos, self.sin, out=qk)
+            append_kv_fp4(w["cache"], qkv[:, :, heads : self.qk_heads], qkv[:, :, self.qk_heads :], self.lengths)
+            o = linear_fp4(attend_kv_fp4(qkv[:, :, :heads], w["cache"], self.lengths).view(self.m, -1), *w["o"])
+            y, hid = norm_add_norm(o, x, w["post_attn"], w["mlp_norm"], 1e-5)
+            mid = linear_fp4(y, *w["gate_up"], activation="swiglu")
+            y, x = norm_add_norm(linear_fp4(mid, *w["down"]), hid, w["post_mlp"], after, 1e-5)
+        self.out.copy_(x)
+        return self.out
+
     def _step_fused(self) -> torch.Tensor:
         x = self.x_in
         rope_cols = self.qk_heads * HEAD_DIM
@@ -207,6 +252,8 @@ class DecodeStep:
         """HIP launches one layer issues (the fused QKV folds its norm in at every M;
         the MLP is two launches, three where its fp16/bf16 MFMA form from 9 rows runs
         a row kernel for its RMSNorm)."""
+        if self.fp4:  # four products, the rotation, the store, the attention (one of a short cache), two pairs of norms
+            return 9
         row_kernel = (self.kind or "dot") == "dot" and self.m > 8 and not self.fp8 and not self.rowsq
         mlp = 3 if row_kernel else 2
         if self.fp8 or self.fused:
@@ -390,7 +437,9 @@ def main() -> None:
     ap.add_argument("--steps", type=int, default=20)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--unfused", action="store_true", help="compose the reference's operators (6 launches/layer at M < 5)")
-    ap.add_argument("--weights", choices=["fp16", "fp8"], default="fp16", help="projection weights (fp8: E4M3 + row scales)")
+    ap.add_argument("--weights", choices=["fp16", "fp8", "fp4"], default="fp16",
+                    help="projection weights (fp8: E4M3 + row scales; fp4: E2M1 + scales of 32, with attention over a 4-bit cache)")
+    ap.add_argument("--context", type=int, default=1024, help="with --weights fp4: tokens in each sequence's cache")
     ap.add_argument("--no-rowsq", action="store_true", help="no row-sum handoff (each RMSNorm derives its sums from its own input)")
     ap.add_argument("--replays", type=int, default=0,
                     help="time this many graph replays one by one, each between two clock probes")
@@ -409,12 +458,12 @@ def main() -> None:
         return
     for m in args.m:
         ds = DecodeStep(m=m, layers=args.layers, dtype=dtype, fused=not args.unfused, weights=args.weights,
-                        rowsq=not args.no_rowsq)
+                        rowsq=not args.no_rowsq, context=args.context)
         eager = time_step(ds, args.steps, args.warmup, graph=False)
         graph = time_step(ds, args.steps, args.warmup, graph=True)
         wb = ds.weight_bytes
         print(json.dumps({
-            "workload": f"decode step minus attention, {args.layers} layers, Llama-3-8B widths, M={m}, {args.dtype}, "
+            "workload": f"decode step {f'with attention over {args.context} tokens' if ds.fp4 else 'minus attention'}, {args.layers} layers, Llama-3-8B widths, M={m}, {args.dtype}, "
                         f"{'unfused' if args.unfused else 'fused'}, {args.weights} weights",
             "eager_us": round(eager, 2),
             "graph_us": round(graph, 2),

@@ -60,15 +60,17 @@ class KvCacheFp4(NamedTuple):
         return cls(*pair(), *pair())
 
 
-def _plain(*tensors) -> bool:
-    """Whether a launch on the pointers of these says all that torch's calls would."""
+def _plain(cache, lengths, pages, *floats) -> bool:
+    """Whether a launch on the pointers of these says all that torch's calls would. (Only floats have gradients.)"""
     if _watched():
         return False
     grad = _grad()
-    for t in tensors:
-        if t is not None and ((grad and t.requires_grad) or t.is_neg()):
-            return False
-    return all(t.__class__ in _PLAIN for t in tensors) or not _subclasses(*tensors)
+    for t in floats:
+        if t.__class__ not in _PLAIN or (grad and t.requires_grad) or t.is_neg():
+            return not isinstance(t, torch.Tensor)  # anything else is the contract's to name
+    k, ks, v, vs = cache
+    return (k.__class__ is ks.__class__ is v.__class__ is vs.__class__ is lengths.__class__ is torch.Tensor
+            and (pages is None or pages.__class__ is torch.Tensor)) or not _subclasses(k, ks, v, vs, lengths, pages)
 
 
 def _cache_sig(c: KvCacheFp4) -> tuple:
@@ -110,7 +112,7 @@ def append_kv_fp4(
     ``lengths - L .. lengths - 1`` of each sequence, in one launch. Positions below 0 are skipped, so a batch whose
     sequences have fewer than ``L`` new tokens is padded on the left. Of two tokens stored to one slot either may stay."""
     try:
-        plain = _plain(*cache, k, v, lengths, pages)
+        plain = _plain(cache, lengths, pages, k, v)
         key = ("append_kv_fp4", _cache_sig(cache), _sig(k), _sig(v), _sig(lengths), _sig(pages))
         plan = _PLANS.get(key) if plain else None
     except (AttributeError, TypeError, ValueError):  # a non-tensor argument: checked below
@@ -172,7 +174,7 @@ def read_kv_fp4(
     bfloat16), zeros where a sequence has no such token: what an attention of the caller's own takes, say over a
     prompt's cached prefix."""
     try:
-        plain = _plain(*cache, lengths, pages)
+        plain = _plain(cache, lengths, pages)
         key = ("read_kv_fp4", _cache_sig(cache), _sig(lengths), count, _sig(pages), dtype)
         plan = _PLANS.get(key) if plain else None
     except (AttributeError, TypeError, ValueError):
@@ -225,7 +227,7 @@ def attend_kv_fp4(
     ``softmax(scale * q k^T) v`` with ``scale`` 1 / sqrt(dim) by default. Query heads are a multiple of the cache's, each run
     of them reading one. One launch, and another one that joins where a sequence's tokens are cut into shares."""
     try:
-        plain = _plain(q, *cache, lengths, pages) and (out is None or out.__class__ in _PLAIN)
+        plain = _plain(cache, lengths, pages, q) and (out is None or out.__class__ in _PLAIN)
         key = ("attend_kv_fp4", _sig(q), _cache_sig(cache), _sig(lengths), _sig(pages), scale,
                None if out is None else _out_sig(out))
         plan = _PLANS.get(key) if plain else None

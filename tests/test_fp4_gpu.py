@@ -56,7 +56,8 @@ SIZES = [(1, 1, 1), (1, 16, 128), (1, 33, 4096), (1, 300, 100), (2, 130, 272), (
          (5, 40, 131), (7, 257, 1008), (13, 96, 2064), (16, 640, 512), (16, 100, 8192), (17, 128, 640), (20, 100, 2051),
          (31, 200, 144), (32, 1000, 1024), (33, 48, 96), (64, 127, 256), (65, 129, 128), (70, 140, 1023), (100, 384, 400),
          (128, 128, 8192), (129, 260, 160), (257, 255, 384), (300, 515, 48), (513, 769, 272), (9, 24, 15), (12, 9, 33),
-         (1, 5000, 31), (8, 5003, 2051)]
+         (1, 5000, 31), (8, 5003, 2051),
+         (5, 20, 3), (20, 33, 7), (6, 40, 8), (30, 21, 9)]
 
 
 @pytest.mark.parametrize("dtype", BOTH)

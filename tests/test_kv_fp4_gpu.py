@@ -392,3 +392,20 @@ def test_a_layer_held_in_four_bits(dtype):
         torch.testing.assert_close(y.float(), want.float(), rtol=4 * tol["rtol"], atol=4 * tol["atol"])
         torch.testing.assert_close(stream.float(), wstream.float(), rtol=4 * tol["rtol"], atol=4 * tol["atol"])
         assert bool(torch.isfinite(last).all()) and bool(torch.isfinite(stream2).all())
+
+
+@pytest.mark.parametrize("m", [1, 6])
+def test_the_decode_step_in_four_bits(m):
+    """The step's operators in its order give what its graph gives, replay for replay; a token of the cache that changes
+    changes them."""
+    from fused_decode.decode_step import DecodeStep
+
+    ds = DecodeStep(m=m, layers=2, h=512, i=768, seed=3, weights="fp4", context=300)
+    eager = ds.step().clone()
+    assert bool(torch.isfinite(eager).all()) and ds.weight_bytes == 2 * ((768 * 512 + 512 * 512 + 3 * 512 * 768) * 17 // 32
+                                                                         + 4 * 512 * 2)
+    for _ in range(3):
+        assert torch.equal(ds.replay(), eager)
+        assert torch.equal(ds.step(), eager)
+    ds.w[0]["cache"].v[0, :, 7] ^= 0x77
+    assert not torch.equal(ds.replay(), eager)
