@@ -110,7 +110,8 @@ def append_kv_fp4(
 ) -> None:
     """Store ``k`` and ``v`` ``[B, L, heads, dim]`` (float16 or bfloat16) in the cache, in place, as tokens
     ``lengths - L .. lengths - 1`` of each sequence, in one launch. Positions below 0 are skipped, so a batch whose
-    sequences have fewer than ``L`` new tokens is padded on the left. Of two tokens stored to one slot either may stay."""
+    sequences have fewer than ``L`` new tokens is padded on the left. Two tokens of one call must
+    not share a slot: it may then hold parts of both."""
     try:
         plain = _plain(cache, lengths, pages, k, v)
         key = ("append_kv_fp4", _cache_sig(cache), _sig(k), _sig(v), _sig(lengths), _sig(pages))
