@@ -452,7 +452,7 @@ __global__ __launch_bounds__(256, D <= 128 && MODE == KV_RUN ? 3 : 2) void kv_at
     }
     float most = kv_max(kv_max(kv_max(p[0], p[1]), kv_max(p[2], p[3])), kv_max(kv_max(p[4], p[5]), kv_max(p[6], p[7])));
     most = xlane_fmax<32>(xlane_fmax<16>(most));
-    if (__builtin_amdgcn_ballot_w64(most > top)) {
+    if (__builtin_amdgcn_ballot_w64(!(most <= top))) {  // (a NaN is the maximum too: the row's sums are NaN from here on)
       const float now = kv_max(top, most);
       const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((top - now) * scale);
       top = now;
@@ -646,7 +646,7 @@ __global__ __launch_bounds__(256, D <= 128 && MODE == KV_RUN ? 3 : 2) void kv_at
   __syncthreads();
   float all = stat[0][r][0];
 #pragma unroll
-  for (int w = 1; w < 4; ++w) all = fmaxf(all, stat[w][r][0]);
+  for (int w = 1; w < 4; ++w) all = kv_max(all, stat[w][r][0]);
   const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((top - all) * scale);
   float* const rows = reinterpret_cast<float*>(smem);
   float* const out = rows + (wave * 16 + r) * PITCH + g * (D / 4);
@@ -661,7 +661,7 @@ __global__ __launch_bounds__(256, D <= 128 && MODE == KV_RUN ? 3 : 2) void kv_at
     if (i >= qa.rows) continue;
     float m = stat[0][row][0];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) m = fmaxf(m, stat[w][row][0]);
+    for (int w = 1; w < 4; ++w) m = kv_max(m, stat[w][row][0]);
     float total = 0.f, v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = 0.f;
