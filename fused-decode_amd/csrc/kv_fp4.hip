@@ -550,8 +550,9 @@ __global__ __launch_bounds__(256, D <= 128 && MODE == KV_RUN ? 3 : 2) void kv_at
       page.divmod(start(i), slot);
       return id < c.pages ? (uint32_t)(id * c.page_step) + slot * row16 : kNoPlace;
     };
-    // steps up to here need no mask
-    const uint32_t plain = min(end, whole < kKvTile - 1 ? 0u : ((uint32_t)whole + 1) / kKvTile);
+    // steps up to here need no mask: every query sees all of their tokens, and they end by themselves where the tokens do
+    // (a length may be past the tokens; a step moved back to end with them has tokens of the one before it)
+    const uint32_t plain = min(end, whole < 0 ? 0u : min((uint32_t)whole + 1, seen) / kKvTile);
     KvStep<D, MODE> s0, s1;
     uint32_t i = first, id0 = page_of(i, plain), id1 = page_of(i + 4, plain), id2 = page_of(i + 8, plain);
     const uint32_t mark = first + (plain > first ? (plain - first + 3) / 4 * 4 : 0), marked = page_of(mark, end);
