@@ -454,7 +454,17 @@ __global__ __launch_bounds__(256, D <= 128 && MODE == KV_RUN ? 3 : 2) void kv_at
     most = xlane_fmax<32>(xlane_fmax<16>(most));
     if (__builtin_amdgcn_ballot_w64(!(most <= top))) {  // (a NaN is the maximum too: the row's sums are NaN from here on)
       const float now = kv_max(top, most);
-      const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((top - now) * scale);
+      const bool first = top == -INFINITY;
+      const float f = first ? 0.f : __builtin_amdgcn_exp2f((top - now) * scale);
+      // Scores of -infinity below a maximum of -infinity have made the sums NaN, as a softmax of nothing else is. Below a
+      // larger one they weigh 0. (A lane's sum is of its own tokens, its row's channels are of all: the row's lanes drop both.)
+      if (__builtin_amdgcn_ballot_w64(first && sum != 0.f)) {
+        if (first && now != -INFINITY) {
+          sum = 0.f;
+#pragma unroll
+          for (int n = 0; n < VD; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+      }
       top = now;
       sum *= f;
 #pragma unroll
@@ -669,7 +679,10 @@ __global__ __launch_bounds__(256, D <= 128 && MODE == KV_RUN ? 3 : 2) void kv_at
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float t = stat[w][row][0];
-      if (t == -INFINITY) continue;
+      if (t == -INFINITY) {  // its sum is 0, or NaN where the row sees tokens, which counts if no wave has more
+        if (m == -INFINITY) total += stat[w][row][1];
+        continue;
+      }
       total += stat[w][row][1] * __builtin_amdgcn_exp2f((t - m) * scale);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += rows[(w * 16 + row) * PITCH + d + j];
@@ -677,7 +690,7 @@ __global__ __launch_bounds__(256, D <= 128 && MODE == KV_RUN ? 3 : 2) void kv_at
     if (splits == 1) {
       uint32_t gi;
       const uint32_t l = group.divmod(i, gi);
-      const float inv = m == -INFINITY ? 0.f : 1.f / total;
+      const float inv = m == -INFINITY && total == 0.f ? 0.f : 1.f / total;  // (zeros where no token is seen)
       typename Vec8<T>::type o;
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j] = from_f32<T>(v[j] * inv);
@@ -726,7 +739,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(T* y, const float* part, u
   m = kv_max(kv_max(tops[0], tops[1]), kv_max(tops[2], tops[3]));
   const float w = own == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((own - m) * qa.scale);
   weight[t] = w;
-  const float all = wave_sum(own == -INFINITY ? 0.f : count * w);
+  const float all = wave_sum(own != -INFINITY ? count * w : m == -INFINITY ? count : 0.f);  // (as between waves)
   if (t % kWave == 0) totals[wave] = all;
   __syncthreads();
   const int lane = t % LANES, at = t / LANES;
@@ -743,7 +756,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(T* y, const float* part, u
   __syncthreads();
   const uint32_t heads = qa.Hq / qa.G, b = bh / heads, h = bh - b * heads, l = group.divmod(i, gi);
   const float total = (totals[0] + totals[1]) + (totals[2] + totals[3]);
-  const float inv = m == -INFINITY ? 0.f : 1.f / total;
+  const float inv = m == -INFINITY && total == 0.f ? 0.f : 1.f / total;
   T* to = y + (((uint64_t)b * qa.L + l) * qa.Hq + h * qa.G + gi) * D;
   for (int d = t; d < D; d += 256) {
     float v = 0.f;
