@@ -355,7 +355,8 @@ __device__ __forceinline__ void kv_each_byte(F&& f) {
 // The scores of a step, S = K Q^T, come out of the matrix cores with a query row a lane column and 4 tokens a lane group
 // and half: exactly as the second product, Y^T += V^T P^T, takes P. Nothing is transposed but the codes' pairs of
 // neighbouring channels into pairs of neighbouring tokens, one permute each. q is bfloat16, float16 as two bfloat16
-// parts; P is two bfloat16 parts (a single one would cost as much again as the output's own rounding).
+// parts. P is two bfloat16 parts, each to the nearest: within 2^-18 of p, where a single one (2^-9) would cost as much
+// again as the output's own rounding, and a third two more matrix instructions to every four.
 //
 // Bound by the instructions between the loads and the matrix cores (two codes a conversion, two a permute), so addresses
 // are a wave's: a step whose tokens lie in one run of slots (KV_RUN: pages of whole steps, or a sequence in one page,
@@ -479,14 +480,13 @@ __global__ __launch_bounds__(256, D <= 128 && MODE == KV_RUN ? 3 : 2) void kv_at
     }
     sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
     if constexpr (!SLOW) {
-      // P's high halves as they are, and what they leave out rounded
+      // P rounded, and what that leaves out, rounded: half a step of half a step, 2^-18 of p
       u32x4 hi, lo;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const uint32_t a = __builtin_bit_cast(uint32_t, p[2 * n]), b = __builtin_bit_cast(uint32_t, p[2 * n + 1]);
-        hi[n] = __builtin_amdgcn_perm(b, a, 0x07060302);
-        const float x = p[2 * n] - __builtin_bit_cast(float, a & 0xffff0000u);
-        const float z = p[2 * n + 1] - __builtin_bit_cast(float, b & 0xffff0000u);
+        hi[n] = __builtin_bit_cast(uint32_t, bf16x2{(bf16)p[2 * n], (bf16)p[2 * n + 1]});
+        const float x = p[2 * n] - __builtin_bit_cast(float, hi[n] << 16);
+        const float z = p[2 * n + 1] - __builtin_bit_cast(float, hi[n] & 0xffff0000u);
         lo[n] = __builtin_bit_cast(uint32_t, bf16x2{(bf16)x, (bf16)z});
       }
       const bf16x8 ph = __builtin_bit_cast(bf16x8, hi), pl = __builtin_bit_cast(bf16x8, lo);
