@@ -355,7 +355,7 @@ __device__ __forceinline__ void kv_each_byte(F&& f) {
 // The scores of a step, S = K Q^T, come out of the matrix cores with a query row a lane column and 4 tokens a lane group
 // and half: exactly as the second product, Y^T += V^T P^T, takes P. Nothing is transposed but the codes' pairs of
 // neighbouring channels into pairs of neighbouring tokens, one permute each. q is bfloat16, float16 as two bfloat16
-// parts. P is two bfloat16 parts, each to the nearest: within 2^-18 of p, where a single one (2^-9) would cost as much
+// parts. P is two bfloat16 parts, each to the nearest: within 2^-17 of p, where a single one (2^-8) would cost as much
 // again as the output's own rounding, and a third two more matrix instructions to every four.
 //
 // Bound by the instructions between the loads and the matrix cores (two codes a conversion, two a permute), so addresses
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(256, D <= 128 && MODE == KV_RUN ? 3 : 2) void kv_at
     }
     sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
     if constexpr (!SLOW) {
-      // P rounded, and what that leaves out, rounded: half a step of half a step, 2^-18 of p
+      // P rounded, and what that leaves out (2^-8 of p at most, so a step of it is 2^-16) rounded: within 2^-17
       u32x4 hi, lo;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
