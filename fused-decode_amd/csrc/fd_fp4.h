@@ -36,6 +36,18 @@ __device__ __forceinline__ bf16x8 fp4_to_bf16(uint32_t codes, float scale) {
 // The conversion's scale of an E8M0 byte: it reads the exponent alone, 0 as 2^-127 and 255 as NaN.
 __device__ __forceinline__ float e8m0_operand(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
 
+// Word J of a row's last piece without the codes past K, `left` = K % 32 of them before it: the activations are zero there,
+// but 0 times what a large scale makes of a code is NaN.
+template <int J>
+__device__ __forceinline__ uint32_t fp4_tail_word(uint32_t codes, int left) {
+  const int n = left - 8 * J;
+  return n >= 8 ? codes : n <= 0 ? 0u : codes & ((1u << (4 * n)) - 1u);
+}
+__device__ __forceinline__ u32x4 fp4_tail(const u32x4& c, int left) {
+  return u32x4{fp4_tail_word<0>(c[0], left), fp4_tail_word<1>(c[1], left), fp4_tail_word<2>(c[2], left),
+               fp4_tail_word<3>(c[3], left)};
+}
+
 // float16 as two bfloat16 numbers: its first eight bits, and the three behind them, which are exact; 0 beside an infinity
 // or a NaN.
 __device__ __forceinline__ void split_f16(f16x8 v, bf16x8& hi, bf16x8& lo) {

@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void fp4_one_kernel(T* y, const T* x, const ui
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int half = N / 2, cols = SWIGLU ? half : N;
   const int o0 = ((int)blockIdx.x * 4 + wave) * O;
-  const int pieces = (K + kGroupK - 1) / kGroupK, chunks = (pieces + kWave - 1) / kWave;
+  const int pieces = (K + kGroupK - 1) / kGroupK, chunks = (pieces + kWave - 1) / kWave, left = K % kGroupK;
 
   const uint8_t *wr[R], *sr[R];
 #pragma unroll
@@ -106,7 +106,13 @@ __global__ __launch_bounds__(256) void fp4_one_kernel(T* y, const T* x, const ui
     if (c0) __syncthreads();  // the block before has been read
     for (int v = tid; v < vectors; v += 256) xs[(v & 3) * (here * kWave) + v / 4] = fp4_load_x(x, k0 + v * 8, K);
     __syncthreads();
-    auto multiply = [&](const Chunk& b, int c) {
+    auto multiply = [&](Chunk& b, int c) {
+      if constexpr (std::is_same<T, bf16>::value) {  // (float16 codes take no scale)
+        if (left && c0 + c == chunks - 1 && (c0 + c) * kWave + lane == pieces - 1) {
+#pragma unroll
+          for (int i = 0; i < R; ++i) b.c[i] = fp4_tail(b.c[i], left);
+        }
+      }
       V8 xv[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) xv[j] = xs[j * (here * kWave) + c * kWave + lane];
