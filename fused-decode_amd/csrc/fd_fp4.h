@@ -126,8 +126,9 @@ struct Fp4Args {
 // One row (fp4_one.hip): any K.
 int fp4_one_launch(const Fp4Args& a);
 
-// Few rows (fp4_few.hip): whether a product fits, and its launch.
+// Few rows (fp4_few.hip): whether a product fits, whether it takes less time there than in tiles, and its launch.
 bool fp4_few_fits(int64_t M, int64_t K, bool swiglu);
+bool fp4_few_wins(int64_t M, int64_t K, int act_dtype);
 int fp4_few_launch(const Fp4Args& a);
 
 }  // namespace fd

@@ -251,6 +251,12 @@ int64_t f4_copy_bytes(int64_t M, int64_t K, int act_dtype) {
   return M * ((K + kF4Stage - 1) / kF4Stage * kF4Stage) * (act_dtype == FD_F16 ? 4 : 2);
 }
 
+// Scratch bytes of a product in tiles: the copies, and the sums of K splits.
+int64_t f4_scratch_bytes(int64_t M, int64_t N, int64_t K, int act_dtype) {
+  const int64_t s = f4_splits(M, N, K);
+  return f4_copy_bytes(M, K, act_dtype) + (s > 1 ? s * M * N * 4 : 0);
+}
+
 template <typename T, int H, int NT, int MT, bool SWIGLU, int FORM, bool TAIL>
 int f4_tile_tail(const Fp4Args& a, const bf16* x, int64_t lo_off, int64_t sxm, int splits) {
   constexpr size_t lds = 2 * (size_t)f4_stage_bytes<H, NT, MT>();
@@ -285,7 +291,9 @@ int f4_pick(const Fp4Args& a, const bf16* x, int64_t lo_off, int64_t sxm, int sp
 template <typename T, bool SWIGLU>
 int f4_product(Fp4Args a) {
   if (a.M == 1) return fp4_one_launch(a);
-  if (fp4_few_fits(a.M, a.K, SWIGLU)) return fp4_few_launch(a);
+  if (fp4_few_fits(a.M, a.K, SWIGLU) && (fp4_few_wins(a.M, a.K, a.act_dtype) ||
+                                         a.scratch_bytes < f4_scratch_bytes(a.M, a.N, a.K, a.act_dtype)))
+    return fp4_few_launch(a);  // (it needs none)
   constexpr bool F16 = std::is_same<T, f16>::value;
   const bf16* x = static_cast<const bf16*>(a.x);
   int64_t sxm = a.sxm, lo_off = 0;
@@ -327,10 +335,8 @@ extern "C" int fd_linear_fp4_scratch(int64_t M, int64_t N, int64_t K, int act_dt
   if (!bytes) return set_error(FD_EINVAL, "null pointer argument");
   *bytes = 0;
   if (M == 0 || N == 0 || K == 0 || M > kF4Most || N > kF4Most || K > kF4Most) return FD_OK;
-  if (M == 1 || (fp4_few_fits(M, K, false) && fp4_few_fits(M, K, true))) return FD_OK;
-  *bytes = f4_copy_bytes(M, K, act_dtype);
-  const int s = f4_splits(M, N, K);
-  if (s > 1) *bytes += (int64_t)s * M * N * 4;
+  if (M == 1 || (fp4_few_wins(M, K, act_dtype) && fp4_few_fits(M, K, false) && fp4_few_fits(M, K, true))) return FD_OK;
+  *bytes = f4_scratch_bytes(M, N, K, act_dtype);
   return FD_OK;
 }
 

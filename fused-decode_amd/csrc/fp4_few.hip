@@ -295,6 +295,26 @@ bool fp4_few_fits(int64_t M, int64_t K, bool swiglu) {
   return K > 0 && ((M <= 16 && f4_most_outputs<1>(K, swiglu) > 0) || (M <= 32 && f4_most_outputs<2>(K, swiglu) > 0));
 }
 
+// Every workgroup brings all of the activations to its registers, in phases where K is long, in 2-byte loads where rows lie
+// at odd elements; tiles bring them once a tile. Captured, weights from HBM, here and in tiles (us):
+//
+//   rows x N x K                      here    tiles        rows x N x K                      here    tiles
+//   32 x 4096 x 4096     bfloat16     13.2    14.5         32 x 4096 x 4096     float16      15.5    18.5
+//   32 x 4096 x 5120     bfloat16     21.8    18.7         32 x 2048 x 8192     float16      25.2    21.2
+//   16 x 2048 x 8192     bfloat16     13.3    14.8         16 x 8192 x 8192     float16      20.4    23.4
+//   4 x 4096 x 14336     bfloat16     17.7    20.0         4 x 4096 x 11008     float16      22.5    20.8
+//   13 x 4096 x 14336    bfloat16     22.2    20.6         2 x 4096 x 14336     float16      27.6    22.6
+//   16 x 28672 x 2051    bfloat16     19.8    22.6         12 x 16384 x 3001    float16      17.6    19.4
+//   29 x 5003 x 2051     bfloat16     18      14.5         29 x 5003 x 2051     float16      23.5    16.7
+//
+// Over 526 products (30 shapes, 2 to 32 rows, both types) the rule's choice takes 0.2 in 100 more than the better of the
+// two, 13 in the worst; this kernel always, 10, and twice as long in the worst.
+bool fp4_few_wins(int64_t M, int64_t K, int act_dtype) {
+  if (K % 2) return K <= 4096 && (M > 16 ? 32 : M) * K <= 49152;
+  if (K > (M > 16 ? 4096 : act_dtype == FD_F16 ? 8192 : 16384)) return false;
+  return K <= 8192 || M * K <= 65536;
+}
+
 int fp4_few_launch(const Fp4Args& a) {
   if (a.act_dtype == FD_F16) return a.swiglu ? f4_few_pick<f16, true>(a) : f4_few_pick<f16, false>(a);
   return a.swiglu ? f4_few_pick<bf16, true>(a) : f4_few_pick<bf16, false>(a);

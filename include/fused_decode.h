@@ -507,7 +507,8 @@ int fd_linear_w8a8_form(int64_t M, int64_t N, int64_t K, int* form);
  * overlap) holds what fd_linear_fp4_scratch says (0: none): copies of activations that are
  * float16, off 16-byte alignment or of no whole 128 along K (without it FD_EUNSUPPORTED), and,
  * where there are few output tiles, the float32 sums of K splits, which are added in a fixed
- * order; less lowers the split, down to none. y may be row_add element for element and overlaps
+ * order; less lowers the split, down to none. 2 to 32 rows that have less than that take a
+ * kernel that needs none, if slower (K of up to 65536). y may be row_add element for element and overlaps
  * no operand otherwise (FD_EUNSUPPORTED); no two of its own elements share memory (FD_EINVAL).
  * No reference counterpart.
  */
