@@ -29,7 +29,7 @@ namespace fd {
 constexpr int kF4Waves = 8;
 constexpr int kF4Step = 256;   // k of a unit
 constexpr int kF4Tiles = 16;   // tiles of a workgroup at most
-constexpr int kF4Ring = 5;     // slots of a wave (4, 5, 6, 7: 13 x 28672 x 4096 26.2, 26.8, 27.6, 28.1 us captured)
+constexpr int kF4Ring = 4;     // slots of a wave (4, 5, 6: 13 x 28672 x 4096 SwiGLU float16 20.2, 20.7, 21.2 us captured)
 
 // Bytes of a scale row in LDS: whole words, and an odd number of them, so that 16 rows' bytes lie in different banks.
 __host__ __device__ __forceinline__ int f4_scale_pitch(int pieces) { return (((pieces + 7) / 8 * 8) / 4 | 1) * 4; }
