@@ -40,22 +40,34 @@ __all__ = ["dequantize_fp4", "linear_fp4", "quantize_fp4"]
 _VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0)
 
 
+def _to_float32(w: torch.Tensor) -> torch.Tensor:
+    """Float32 values on the same side of every border between codes or scales as ``w``: float64 is rounded to the odd
+    neighbour (the borders are even), so that a second rounding is as if it were the first."""
+    v = w.float()
+    if w.dtype != torch.float64:
+        return v
+    back = v.double()
+    inexact = (back != w) & torch.isfinite(v)
+    bits = v.view(torch.int32)
+    return torch.where(inexact, (bits - (back.abs() > w.abs()).int()) | 1, bits).view(torch.float32)
+
+
 def quantize_fp4(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``[N, K]`` float weight -> (E2M1 codes ``[N, 16 G]`` as uint8, two a byte, E8M0 scales ``[N, G]``) with
-    ``G = ceil(K / 32)``; codes past K are 0."""
+    ``G = ceil(K / 32)``; codes past K are 0. (Magnitudes beyond float32's are infinities.)"""
     if not isinstance(weight, torch.Tensor) or weight.ndim != 2:
         raise ValueError("weight must be a rank-2 tensor [N, K]")
     if not weight.is_floating_point():
         raise TypeError("weight must be a floating-point tensor")
     n, k = weight.shape
     groups = -(-k // FP4_GROUP)
-    w = torch.nn.functional.pad(weight.detach().float(), (0, groups * FP4_GROUP - k)).reshape(n, groups, FP4_GROUP)
+    w = torch.nn.functional.pad(_to_float32(weight.detach()), (0, groups * FP4_GROUP - k)).reshape(n, groups, FP4_GROUP)
     top = w.abs().amax(dim=-1) if groups else w.new_zeros(n, 0)
     # the exponent of top / 4, one more from 1.75 times a power of two on
     byte = (((top.view(torch.int32) + 0x200000) >> 23) - 2).clamp(1, 254)
     byte = torch.where(top > 0, byte, 127)
     bad = ~torch.isfinite(top)
-    inverse = ((254 - byte) << 23).view(torch.float32)  # exact: byte is 252 at most
+    inverse = ((254 - byte) << 23).view(torch.float32)  # exact: byte is 253 at most
     v = torch.where(bad[..., None], 0.0, w * inverse[..., None])
     a = v.abs()
     code = (a > 0.25).to(torch.uint8)
