@@ -61,7 +61,8 @@ class KvCacheFp4(NamedTuple):
 
 
 def _plain(cache, lengths, pages, *floats) -> bool:
-    """Whether a launch on the pointers of these says all that torch's calls would. (Only floats have gradients.)"""
+    """Whether a launch on the pointers of these says all that torch's calls would. (Only floats have gradients, a cache's
+    scales among them.)"""
     if _watched():
         return False
     grad = _grad()
@@ -69,6 +70,8 @@ def _plain(cache, lengths, pages, *floats) -> bool:
         if t.__class__ not in _PLAIN or (grad and t.requires_grad) or t.is_neg():
             return not isinstance(t, torch.Tensor)  # anything else is the contract's to name
     k, ks, v, vs = cache
+    if grad and (ks.requires_grad or vs.requires_grad):
+        return False
     return (k.__class__ is ks.__class__ is v.__class__ is vs.__class__ is lengths.__class__ is torch.Tensor
             and (pages is None or pages.__class__ is torch.Tensor)) or not _subclasses(k, ks, v, vs, lengths, pages)
 
