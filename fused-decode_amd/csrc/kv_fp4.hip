@@ -770,9 +770,9 @@ namespace {
 
 bool kv_dim(int64_t d) { return d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
 
-// Bytes from the first to past the last code of a cache's tensor.
-int64_t kv_span(const fd_kv_shape& s, int64_t row) {
-  return (s.pages - 1) * s.page_stride + (s.heads - 1) * s.head_stride + s.page * row;
+// Bytes from the first to past the last code of a cache's tensor (below 2^36 where kv_check passes; strides may be any).
+__int128 kv_span(const fd_kv_shape& s, int64_t row) {
+  return (__int128)(s.pages - 1) * s.page_stride + (__int128)(s.heads - 1) * s.head_stride + s.page * row;
 }
 
 int kv_check(const fd_kv_shape* s, const void* k, const void* ks, const void* v, const void* vs, const int32_t* lengths,
@@ -806,7 +806,7 @@ int kv_check(const fd_kv_shape* s, const void* k, const void* ks, const void* v,
 
 // Whether [p, p + n) meets one of the cache's tensors.
 bool kv_meets(const fd_kv_shape& s, const KvCache& c, const void* p, int64_t n) {
-  const int64_t codes = s.pages > 0 ? kv_span(s, s.dim / 2) : 0, scales = codes / 16;
+  const int64_t codes = s.pages > 0 ? (int64_t)kv_span(s, s.dim / 2) : 0, scales = codes / 16;
   return overlaps(p, n, c.k, codes) || overlaps(p, n, c.v, codes) || overlaps(p, n, c.ks, scales) ||
          overlaps(p, n, c.vs, scales);
 }
@@ -816,6 +816,11 @@ bool kv_meets(const fd_kv_shape& s, const KvCache& c, const void* p, int64_t n) 
 // join: one sequence of 131072 tokens, 8 heads of 128, 55, 45, 48, 51 us; 32 of 2048 to 8192, 85, 56, 57, 58; captured,
 // while the step's loads were still under a condition.)
 int64_t kv_tiles(int64_t L, int64_t G) { return (L * G + 15) / 16; }
+// Whether a launch holds the query rows of L queries and G heads for each of the cache's `heads`.
+bool kv_rows_fit(int64_t L, int64_t G, int64_t heads) {
+  constexpr int64_t most = 0x7fffffffLL;
+  return L <= most && G <= most && L * G <= most && kv_tiles(L, G) <= 65535 / heads;
+}
 int64_t kv_splits(int64_t B, int64_t L, int64_t Hq, int64_t heads, int64_t capacity) {
   const int64_t units = B * heads * kv_tiles(L, Hq / heads);
   int64_t s = units > 0 ? (2 * device_cus() + units - 1) / units : 1;
@@ -875,7 +880,7 @@ extern "C" int fd_append_kv_fp4(void* k, void* k_scale, void* v, void* v_scale, 
   if (rc != FD_OK) return rc;
   if (B == 0 || L == 0 || tb.capacity == 0 || shape->pages == 0) return FD_OK;
   if (!new_k || !new_v) return set_error(FD_EINVAL, "null pointer argument");
-  const int64_t codes = kv_span(*shape, shape->dim / 2), scales = codes / 16;
+  const int64_t codes = (int64_t)kv_span(*shape, shape->dim / 2), scales = codes / 16;
   const void* t[4] = {k, k_scale, v, v_scale};
   for (int i = 0; i < 4; ++i)
     for (int j = 0; j < i; ++j)
@@ -886,8 +891,9 @@ extern "C" int fd_append_kv_fp4(void* k, void* k_scale, void* v, void* v_scale, 
   if (kv_meets(*shape, c, new_k, nk) || kv_meets(*shape, c, new_v, nv) || kv_meets(*shape, c, lengths, B * 4) ||
       (table && kv_meets(*shape, c, table, ((B - 1) * table_stride + table_pages) * 4)))
     return set_error(FD_EINVAL, "a cache must not overlap what is stored into it");
-  const int64_t lanes = shape->dim / 8, half = B * L * shape->heads * lanes;
-  if (half > 0x7fffff00LL || L > 0x7fffffffLL) return set_error(FD_EUNSUPPORTED, "too large");
+  const int64_t lanes = shape->dim / 8, of_token = B * shape->heads * lanes;
+  if (L > 0x7fffff00LL / of_token) return set_error(FD_EUNSUPPORTED, "too large");
+  const int64_t half = of_token * L;
   const dim3 blocks((unsigned)((2 * half + 255) / 256));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   auto go = [&](auto one) {
@@ -946,7 +952,7 @@ extern "C" int fd_attend_kv_fp4_scratch(int64_t B, int64_t L, int64_t Hq, int64_
   if (!kv_dim(dim)) return set_error(FD_EUNSUPPORTED, "dim must be 64, 96, 128, 192 or 256, got %lld", (long long)dim);
   if (!bytes) return set_error(FD_EINVAL, "null pointer argument");
   *bytes = 0;
-  if (B == 0 || L == 0 || Hq == 0) return FD_OK;
+  if (B == 0 || L == 0 || Hq == 0 || B > 65535 || heads > 65535 || !kv_rows_fit(L, Hq / heads, heads)) return FD_OK;
   const int64_t s = kv_splits(B, L, Hq, heads, capacity);
   if (s > 1) *bytes = B * heads * kv_tiles(L, Hq / heads) * s * 16 * (dim + 4) * 4;
   return FD_OK;
@@ -971,8 +977,9 @@ extern "C" int fd_attend_kv_fp4(void* y, const void* q, const void* k, const voi
   if (!y || !q) return set_error(FD_EINVAL, "null pointer argument");
   if (!aligned16(y)) return set_error(FD_EUNSUPPORTED, "y must be 16-byte aligned");
   if (shape->pages == 0) return set_error(FD_EUNSUPPORTED, "a cache without pages");
-  const int64_t G = Hq / shape->heads, tiles = kv_tiles(L, G);
-  if (L * G > 0x7fffffffLL || tiles * shape->heads > 65535) return set_error(FD_EUNSUPPORTED, "too many query rows");
+  const int64_t G = Hq / shape->heads;
+  if (!kv_rows_fit(L, G, shape->heads)) return set_error(FD_EUNSUPPORTED, "too many query rows");
+  const int64_t tiles = kv_tiles(L, G);
   const int64_t ny = B * L * Hq * shape->dim * 2;
   if (overlaps(y, ny, q, kv_q_span(B, L, Hq, shape->dim, sqb, sql, sqh)) || kv_meets(*shape, c, y, ny) ||
       overlaps(y, ny, lengths, B * 4) || (table && overlaps(y, ny, table, ((B - 1) * table_stride + table_pages) * 4)))
