@@ -20,6 +20,7 @@
 // Two kernels:
 //   norm_pair_kernel     - unit column strides, rows of any alignment, 8 <= n <= 32768: LPR lanes a row.
 //   norm_pair_gen_kernel - any strides and any n: a workgroup a row, three times over the row.
+#include <numeric>
 #include <type_traits>
 
 #include "fd_device.h"
@@ -291,6 +292,25 @@ int64_t pair_bytes(const fd_rows& l, int elem) {
              : 0;
 }
 
+// Whether operands share a byte. Rows of unit column stride begin at multiples of the greatest common divisor of all row
+// strides from their bases, so they lie beside each other (halves of a wider buffer's rows) where the bases are a row
+// apart within it, both ways round.
+bool pair_meet(const void* pa, const fd_rows& la, int ea, const void* pb, const fd_rows& lb, int eb) {
+  if (!overlaps(pa, pair_bytes(la, ea), pb, pair_bytes(lb, eb))) return false;
+  if (la.n > 1 && (la.col != 1 || lb.col != 1)) return true;
+  int64_t step = 0;
+  for (const fd_rows* l : {&la, &lb}) {
+    const int e = l == &la ? ea : eb;
+    if (l->a > 1) step = std::gcd(step, l->sa * e);
+    if (l->b > 1) step = std::gcd(step, l->sb * e);
+    if (l->c > 1) step = std::gcd(step, l->sc * e);
+  }
+  if (step == 0) return true;
+  const int64_t apart = (int64_t)(reinterpret_cast<uintptr_t>(pb) - reinterpret_cast<uintptr_t>(pa)) % step;
+  const int64_t d = apart < 0 ? apart + step : apart;
+  return !(d >= la.n * ea && d + lb.n * eb <= step);
+}
+
 bool pair_same(const fd_rows& a, const fd_rows& b) {
   return (a.a == 1 || a.sa == b.sa) && (a.b == 1 || a.sb == b.sb) && (a.c == 1 || a.sc == b.sc) &&
          (a.n == 1 || a.col == b.col);
@@ -327,19 +347,18 @@ extern "C" int fd_norm_add_norm(void* y, void* residual_out, const void* x, cons
   if (a.rows > 0x7fffffffLL) return set_error(FD_EUNSUPPORTED, "too many rows (>= 2^31)");
   // outputs are stored while other rows are still read
   if (rows_meet(*ly) || rows_meet(*lro)) return set_error(FD_EINVAL, "an output's elements must not share memory");
-  const int64_t ny = pair_bytes(*ly, 2), nro = pair_bytes(*lro, 2), nx = pair_bytes(*lx, 2), nr = pair_bytes(*lr, 2);
   const int64_t npw = ((n - 1) * post_w_stride + 1) * dtype_bytes(post_w_dtype);
   const int64_t nw = ((n - 1) * w_stride + 1) * dtype_bytes(w_dtype);
-  const int64_t ng = gate ? pair_bytes(*lg, dtype_bytes(gate_dtype)) : 0;
-  if (overlaps(y, ny, residual_out, nro)) return set_error(FD_EINVAL, "the outputs must not overlap each other");
+  if (pair_meet(y, *ly, 2, residual_out, *lro, 2)) return set_error(FD_EINVAL, "the outputs must not overlap each other");
   const void* out[2] = {y, residual_out};
-  const int64_t len[2] = {ny, nro};
   const fd_rows* lo[2] = {ly, lro};
   for (int i = 0; i < 2; ++i) {
-    if (overlaps(out[i], len[i], post_w, npw) || overlaps(out[i], len[i], w, nw) || overlaps(out[i], len[i], gate, ng))
+    const int64_t len = pair_bytes(*lo[i], 2);
+    if (overlaps(out[i], len, post_w, npw) || overlaps(out[i], len, w, nw) ||
+        (gate && pair_meet(out[i], *lo[i], 2, gate, *lg, dtype_bytes(gate_dtype))))
       return set_error(FD_EINVAL, "an output must not overlap a weight or the gate");
-    if ((overlaps(out[i], len[i], x, nx) && !(out[i] == x && pair_same(*lo[i], *lx))) ||
-        (overlaps(out[i], len[i], residual, nr) && !(out[i] == residual && pair_same(*lo[i], *lr))))
+    if ((pair_meet(out[i], *lo[i], 2, x, *lx, 2) && !(out[i] == x && pair_same(*lo[i], *lx))) ||
+        (pair_meet(out[i], *lo[i], 2, residual, *lr, 2) && !(out[i] == residual && pair_same(*lo[i], *lr))))
       return set_error(FD_EINVAL, "an output must not overlap an input, other than as x or residual itself");
   }
   return act_dtype == FD_F16 ? dispatch_pair<f16>(a) : dispatch_pair<bf16>(a);
