@@ -242,7 +242,18 @@ void launch_pair(const PairArgs& a) {
 constexpr int64_t kPairMaxN = 32768;  // 512 lanes of eight vectors
 
 // Lanes of a row and vectors of eight a lane: 16 lanes up to 128 elements, a wave up to 1024, 256 lanes up to 8192, then 512,
-// so that a row stays in registers. The bounds were not swept; 4096 elements (256 lanes, two vectors) is the size measured.
+// so that a row stays in registers. Captured, bfloat16, a gate a channel, us of one row and of many (33 million elements), beside other lanes:
+//
+//   elements      rule              other lanes
+//   64            16: 3.0   63      64: 3.0   195
+//   256           64: 3.0   59      16: 3.8    54
+//   512           64: 2.9   44.5    16: 4.1    46
+//   1024          64: 3.3   45     256: 3.1    55
+//   2048         256: 3.2   48      64: 4.1    47
+//   4096         256: 3.6   49      64: 5.7    60     512: 3.5   47
+//   8192         256: 4.6   48     512: 4.0    50
+//   16384        512: 5.2   55     256: 6.3    64    1024: 5.2   57
+//   32768        512: 8.1   56    1024: 8.4    59
 template <typename T, typename W, int GATE>
 void pick_pair(const PairArgs& a) {
   const int64_t nv = (a.lx.n + 7) / 8;
