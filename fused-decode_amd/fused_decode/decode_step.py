@@ -35,8 +35,8 @@ with the residual) and post_attn_mlp_fp8: four launches per layer, with the same
 row-sum handoff from 5 rows.
 
 With weights="fp4" a layer is whole: E2M1 projections (quantize_fp4), attention over a key/value cache held in 4 bits
-(``context`` tokens a sequence, the new one among them), and norms on both sides of each block, nine launches a layer or
-ten where the attention is cut into shares:
+(``context`` tokens a sequence, the new one among them), and norms on both sides of each block, nine launches a layer, one
+more where the attention is cut into shares and up to two more for each product that runs in tiles:
 
     qkv  = linear_fp4(y, *w_qkv)                          # y: the block's normed input, of the norms before
     q, k = rope(qkv[:, :5120])
@@ -58,6 +58,8 @@ import json
 
 import torch
 
+from . import _lib
+from ._lib import DTYPE_CODE
 from .block_norms import norm_add_norm
 from .fp4 import linear_fp4, quantize_fp4
 from .kernels import _MFMA_MIN_M
@@ -94,7 +96,7 @@ class DecodeStep:
         # 5 rows whatever the kind)
         mfma = m >= _MFMA_MIN_M and (self.fp8 or (kind or "dot") == "dot")
         self.rowsq = rowsq and fused and mfma and not self.fp4
-        self.h, self.i = h, i
+        self.h, self.i, self.context = h, i, context
         heads = h // HEAD_DIM
         kv = max(1, heads // 4)
         self.qk_heads = heads + kv
@@ -252,13 +254,27 @@ class DecodeStep:
         """HIP launches one layer issues (the fused QKV folds its norm in at every M;
         the MLP is two launches, three where its fp16/bf16 MFMA form from 9 rows runs
         a row kernel for its RMSNorm)."""
-        if self.fp4:  # four products, the rotation, the store, the attention (one of a short cache), two pairs of norms
-            return 9
+        if self.fp4:
+            return self._launches_fp4()
         row_kernel = (self.kind or "dot") == "dot" and self.m > 8 and not self.fp8 and not self.rowsq
         mlp = 3 if row_kernel else 2
         if self.fp8 or self.fused:
             return 1 + 1 + mlp
         return 4 + mlp
+
+    def _launches_fp4(self) -> int:
+        """The rotation, the store, two pairs of norms; the attention, and the join where its tokens are cut into shares;
+        four products, with the copy of activations and the sum of K splits where they run in tiles. The last ones are told
+        by the scratch that they ask for."""
+        heads = self.h // HEAD_DIM
+        kv = self.qk_heads - heads
+        launches = 5 + (_lib.scratch_bytes("fd_attend_kv_fp4_scratch", self.m, 1, heads, kv, HEAD_DIM, self.context) > 0)
+        f16 = self.dtype == torch.float16
+        for n, k in ((self.qkv_n, self.h), (self.h, self.h), (2 * self.i, self.h), (self.h, self.i)):
+            size = _lib.scratch_bytes("fd_linear_fp4_scratch", self.m, n, k, DTYPE_CODE[self.dtype])
+            copies = self.m * -(-k // 128) * 128 * (4 if f16 else 2)
+            launches += 1 + (size > 0 and (f16 or k % 128 != 0)) + (size > copies)
+        return launches
 
     def capture(self) -> None:
         side = torch.cuda.Stream()
