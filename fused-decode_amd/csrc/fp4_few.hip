@@ -1,4 +1,4 @@
-// Products with E2M1 weights for few activation rows (2 to 32): the weights stream through LDS once, the activations
+// Products with E2M1 weights for few activation rows (2 to 32, where fp4_few_wins says so): the weights stream through LDS once, the activations
 // stay in registers (fd_fp4.h has the mathematics).
 //
 // A workgroup of eight waves, one to a CU, owns a run of outputs and walks them in tiles of 16 weight rows (SWIGLU: 8 gate
@@ -14,12 +14,13 @@
 // the lanes past it.
 //
 // Bound by a launch's start and end, the activations' and the scales' way into registers and LDS in front of the stream,
-// and then by the stream: 13 x 28672 x 4096 SWIGLU float16 20.8 us (3.0 TB/s of weights), of which the units alone, nothing
-// multiplied, take 17.6, the scales 2 and the activations 0.5; 13 x 4096 x 14336 bfloat16 21.9 (units alone 12.3,
-// activations 4.3, scales 2.2), float16, whose two parts take twice the registers and so more phases, 29; 13 x 6144 x 4096
-// 10.2; 29 x 5003 x 2051 float16 23. Activations loaded 64 bytes of a row at a time and exchanged between lane groups took
-// as long (20.7, 22.6, 10.5), and loading them and the scales before the first units longer (22.4, 23.9, 11.6): the stream
-// then starts later.
+// and then by the stream. Traced medians: 13 x 28672 x 4096 SWIGLU float16 20.6 us (3.0 TB/s of weights), bfloat16 18.3;
+// 13 x 6144 x 4096 11.7 and 10.0; 32 x 4096 x 4096 15.6 and 13.2. With five slots in the ring and parts of the work left
+// out, the first took 22.3, without activations 21.4, without scales 19.2, without either 18.7, the units alone, nothing
+// multiplied, 19.6. A long K leaves more before the stream (13 x 4096 x 14336 bfloat16 23.8: without activations 18.4, scales
+// 20.5, either 16.1, units alone 12.1) and goes to the tiles. Activations loaded 64 bytes of a row at a time and exchanged
+// between lane groups took as long, and loading them and the scales before the first units longer (22.4 us of the first):
+// the stream then starts later.
 //
 // Slot layout: 16 rows of 8 pieces of 16 bytes, piece c at c ^ (row mod 8).
 #include "fd_fp4.h"

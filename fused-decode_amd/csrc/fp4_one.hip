@@ -8,7 +8,8 @@
 // float16's range) and a piece's sum takes it, exactly. v_dot2 adds two products in float32. Two chunks are on the way.
 //
 // Bound by a launch's start and end and by the instructions around the weights' stream, half of them outside of the
-// products: 6144 x 4096 5.4 us (2.5 TB/s), 28672 x 4096 SWIGLU 13.5 (4.6), 4096 x 14336 8.4 (3.7).
+// products; a wave has two chunks of a K of 4096, and loads two past the end. Traced, median (least), bfloat16: 6144 x 4096
+// 6.1 us (4.6; 2.2 TB/s in the median), 28672 x 4096 SWIGLU 15.6 (13.3; 4.0), 4096 x 14336 9.4 (7.8; 3.3).
 #include "fd_fp4.h"
 
 namespace fd {

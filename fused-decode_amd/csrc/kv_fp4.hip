@@ -42,8 +42,8 @@ __device__ __forceinline__ uint32_t kv_place(const KvCache& c, const KvTable& tb
 
 // ------------------------------------------------------------------ store and read
 
-// Eight values a lane, four lanes a group; bound by a launch's start and end (one token: 2.8 us) and by HBM (4 x 2048 tokens
-// of 8 heads of 128: 12.8 us, 3.3 TB/s, keys and values in two halves of the grid).
+// Eight values a lane, four lanes a group; bound by a launch's start and end (one token: 2.7 us) and by its stores of 4 and 1
+// bytes (4 x 2048 tokens of 8 heads of 128: 12.6 us, 3.4 TB/s, keys and values in two halves of the grid).
 template <typename T>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvCache c, KvTable tb, const T* k, const T* v, int64_t skb,
                                                         int64_t skl, int64_t skh, int64_t svb, int64_t svl, int64_t svh,
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvCache c, KvTable tb, c
 }
 
 // Eight values a lane; rows in the order of four tokens, heads, tokens, so that what is read and what is written both
-// lie together: 4 x 8192 tokens of 8 heads of 128 in 27.9 us, 6.1 TB/s, four fifths of it writes.
+// lie together: 4 x 8192 tokens of 8 heads of 128 in 26.8 us, 6.3 TB/s, four fifths of it writes.
 template <typename T>
 __global__ __launch_bounds__(256) void kv_read_kernel(T* ko, T* vo, KvCache c, KvTable tb, uint32_t count, uint32_t dim,
                                                       uint32_t row16, FastDiv lanes, FastDiv heads, FastDiv quads,
@@ -362,10 +362,14 @@ __device__ __forceinline__ void kv_each_byte(F&& f) {
 // are a wave's: a step whose tokens lie in one run of slots (KV_RUN: pages of whole steps, or a sequence in one page,
 // whose last step starts early enough to end with it) needs one place. Masks are for the steps that need them.
 //
-// One sequence of 131072 tokens, 32 query and 8 key/value heads of 128, float16: 31 us (4.6 TB/s); 32 sequences of 2048 to
-// 8192, bfloat16: 43 (4.2 TB/s); the joins 5.4 and 4.8. A step's loop body is 245 instructions (472 with a place a token and
-// masks in every step, 66 and 68 us). The next step's loads stand under no condition: with three workgroups a CU 41 and 47 us
+// Traced medians: one sequence of 131072 tokens, 32 query and 8 key/value heads of 128, float16: 31 us (4.6 TB/s); 32
+// sequences of 2048 to 8192, bfloat16: 44 (4.2 TB/s); the joins 5.2 and 5.0. Counted, 257 and 232 vector instructions a step,
+// which keep the vector units busy 0.6 of the cycles and the matrix cores 0.29 and 0.24. With a place a token and masks in
+// every step they took 66 and 68 us. The next step's loads stand under no condition: with three workgroups a CU 41 and 47 us
 // under one, 32 and 44 without.
+//
+// Scores that are no numbers are a row's maximum, and so in all of its sums. Scores of -infinity weigh 0 beside larger ones;
+// a row that has nothing else is NaN, one that sees no token 0, and the sum beside a maximum of -infinity says which.
 //
 // An infinity or NaN among the values of one token must not reach query rows that do not see it (0 times it is NaN): a
 // step that holds a scale from which codes leave bfloat16's range is left out, and summed token by token behind the

@@ -242,7 +242,8 @@ void launch_pair(const PairArgs& a) {
 constexpr int64_t kPairMaxN = 32768;  // 512 lanes of eight vectors
 
 // Lanes of a row and vectors of eight a lane: 16 lanes up to 128 elements, a wave up to 1024, 256 lanes up to 8192, then 512,
-// so that a row stays in registers. Captured, bfloat16, a gate a channel, us of one row and of many (33 million elements), beside other lanes:
+// so that a row stays in registers. Captured, bfloat16, a gate a channel, us of one row and of many (33 million elements),
+// beside other lanes:
 //
 //   elements      rule              other lanes
 //   64            16: 3.0   63      64: 3.0   195

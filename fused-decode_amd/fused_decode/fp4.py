@@ -6,8 +6,9 @@
 Two codes a byte, the first in the low half. A group's scale is the smallest power of two that its largest magnitude is
 less than 7 of (2^-126 at least; 1 for a group of zeros), and a code is the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
 negatives to w / scale, ties to the even code: a value up to 7 rounds to 6, as far off as halves of E2M1's last step
-are. A group that holds an infinity or a NaN gets a NaN scale. Codes and scales are OCP's MXFP4, so weights quantised
-elsewhere to that format are taken as they are. The kernels decode them exactly and sum in float32:
+are. (OCP's own recipe takes the largest magnitude's exponent less 2 for the scale, so that a value of 7 saturates at 6.) A
+group that holds an infinity or a NaN gets a NaN scale. Codes and scales are in OCP's MXFP4 format, so weights quantised
+elsewhere to it are taken as they are. The kernels decode them exactly and sum in float32:
 
     y[m, n] = round(act(sum_k x[m, k] * scale[n, k / 32] * e2m1(codes[n, k]) + bias[n]) + row_add[m, n])
 

@@ -7,8 +7,10 @@
 
 ``lengths`` (int32, on the device) are the sequences' tokens, the new ones among them: the same tensor serves the store and
 the attention. ``pages`` (int32 ``[B, n]``) are each sequence's pages in order; without it page ``b`` is sequence ``b``'s.
-Query ``l`` of ``L`` sees tokens ``0 .. lengths - L + l``; one that sees none gets zeros. The format is ``quantize_fp4``'s, along
-the head. Heads of 64, 96, 128, 192 or 256. A layer of a decode step around it:
+Query ``l`` of ``L`` sees tokens ``0 .. lengths - L + l``; one that sees none gets zeros, and one that sees a key or value
+that is no number gets NaN where it counts. Scores, the softmax and its sums are float32; its weights meet the values as
+two bfloat16 numbers, within 2^-17 of them (a step of a bfloat16 output is 2^-7). The format is ``quantize_fp4``'s, along the
+head. Heads of 64, 96, 128, 192 or 256. A layer of a decode step around it:
 
     qkv = pre_attn_qkv(x, attn_norm, w_qkv, cos, sin, eps, rope_cols=...)        # q and k rotated
     q, k, v = qkv.view(B, 1, heads + 2 * kv_heads, dim).split([heads, kv_heads, kv_heads], dim=2)

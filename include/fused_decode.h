@@ -564,8 +564,9 @@ int fd_read_kv_fp4(void* out_k, void* out_v, const void* k, const void* k_scale,
  * each sequence's last L tokens, over the cache; Hq is a multiple of its heads, query head n reads
  * head n / (Hq / heads):
  *   y = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale * q . k_t),  t <= lengths[b] - L + l
- * y [B, L, Hq, dim], dense; a query that sees no token gets zeros. Softmax and sums are float32;
- * q, keys and values are exact in the products, p is held as two bfloat16 numbers. `scratch`
+ * y [B, L, Hq, dim], dense; a query that sees no token gets zeros, one that sees a score that is
+ * no number, or only scores of -infinity, NaN. Softmax and sums are float32; q, keys and values are
+ * exact in the products, p is held as two bfloat16 numbers (within 2^-17 of it). `scratch`
  * (16-byte aligned, caller-owned, not shared with a call that may overlap) holds what
  * fd_attend_kv_fp4_scratch says (`capacity`: tokens that a sequence's pages hold; 0: none): the sums
  * of a sequence's shares, which a second launch joins; less lowers their number, down to one. y
